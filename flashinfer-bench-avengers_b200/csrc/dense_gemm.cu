@@ -1,0 +1,505 @@
+// Dense GEMMs over CTA pairs (sm_100a): D[m, n] = sum_k A[m, k] B[n, k] with
+// 16-bit or 4-bit microscaled operands, fp32 sums in tensor memory.
+//
+// One tile is 256 output rows x up to 256 output columns, computed by a pair
+// of CTAs with tcgen05.mma.cta_group::2: each CTA stages its 128 rows of A
+// and its half of B's rows, so a 128-byte K slice costs 32 KB of shared
+// memory per CTA instead of the 48 KB of a single-CTA 128 x 256 tile, and
+// each B byte is fetched once per pair. Persistent: one pair per two SMs
+// walks the tiles; two accumulators in tensor memory let the epilogue of one
+// tile run under the MMAs of the next.
+//
+// Roles per CTA: warp 0 TMA producer, warp 1 MMA issuer (of the pair's first
+// CTA only), warp 2 owns tensor memory, warps 4-7 epilogue, one 32-lane
+// quarter of the accumulator each. The pair's loads all count on the first
+// CTA's `full` barrier; its commits free the stage in both CTAs.
+//
+// Each epilogue thread owns an output row and writes 32-byte sectors: full
+// sectors need no staging through shared memory, and L2 merges a row's
+// sectors before they reach HBM.
+//
+// The operands may be stored along K or along the output dimension (the
+// gradients need W^T and X^T): the shared-memory descriptors take both, so
+// nothing is transposed in memory.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+#include <cstring>
+
+#include "../../include/moe_b200.h"
+#include "dense_gemm.h"
+#include "dense_ptx.cuh"
+#include "ffn_math.cuh"
+#include "host_common.h"
+#include "moe_kernels.cuh"
+
+namespace moe {
+
+__device__ uint32_t g_dense_status;
+
+uint32_t* dense_status_word() {
+  void* p = nullptr;
+  return cudaGetSymbolAddress(&p, g_dense_status) == cudaSuccess ? static_cast<uint32_t*>(p) : nullptr;
+}
+
+namespace {
+
+constexpr int kTileBytes = 16384;   // 128 rows (or 128 MN elements x 64 K) of 128 bytes
+
+template <bool kMx>
+struct PairTraits {
+  static constexpr int kStages = 6;
+  static constexpr int kScaleBytes = kMx ? 3072 : 0;   // A: 2 K tiles, B: 2 row tiles x 2 K tiles of 512 bytes
+  static constexpr int kStageBytes = 2 * kTileBytes + kScaleBytes;
+  // Tensor memory: two accumulators of up to 256 columns. With 4-bit
+  // operands 48 columns hold the staged exponents (2 x 24), and the
+  // accumulators overlap in 48 columns, which the epilogue drains first.
+  static constexpr int kAcc1 = kMx ? 208 : 256;
+  static constexpr int kScaleCol = 464;
+  static constexpr int kOffBars = kStages * kStageBytes;
+  static constexpr int kNumBars = 2 * kStages + 4;
+  static constexpr int kSmemBytes = kOffBars + kNumBars * 8 + 16 + 1024;
+  static_assert(kSmemBytes <= 227 * 1024, "shared memory");
+};
+
+constexpr int kPairThreads = 256;
+constexpr int kEpiWarps = 4;
+
+struct Tile {
+  int m0, n0;   // first output row of the pair, first output column
+};
+
+// Tiles in bands of 8 row tiles, rows fastest: the pairs running at one time
+// cover a near-square block of the output, so A and B slices are re-read
+// from L2.
+__device__ __forceinline__ Tile tile_at(int t, const DenseParams& p) {
+  constexpr int kBand = 8;
+  const int per_band = kBand * p.n_tiles;
+  const int band = t / per_band;
+  const int r = t - band * per_band;
+  const int rows = min(kBand, p.m_tiles - band * kBand);
+  Tile o;
+  o.n0 = (r / rows) * p.n_step;
+  o.m0 = (band * kBand + r % rows) * 256;
+  return o;
+}
+
+// Writes 16 consecutive 16-bit outputs (columns c .. c+15 of a row with n
+// columns, n and c multiples of 8).
+__device__ __forceinline__ void store_row16(uint16_t* row, int c, int n, const uint32_t* v, bool vec32) {
+  if (vec32 && c + 16 <= n) {
+    st_global_32(row + c, v);
+  } else {
+    if (c + 8 <= n) *reinterpret_cast<uint4*>(row + c) = make_uint4(v[0], v[1], v[2], v[3]);
+    if (c + 16 <= n) *reinterpret_cast<uint4*>(row + c + 8) = make_uint4(v[4], v[5], v[6], v[7]);
+  }
+}
+
+}  // namespace
+
+template <bool kMx, bool kAMn, bool kBMn, int kEpi>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+    dense_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
+                      const __grid_constant__ CUtensorMap tm_sfa, const __grid_constant__ CUtensorMap tm_sfb,
+                      const DenseParams p) {
+  using Tr = PairTraits<kMx>;
+  constexpr bool kGate = kEpi == kEpiGated || kEpi == kEpiGatedQuant;
+  constexpr int kS = Tr::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Tr::kOffBars);
+  uint64_t* full_bar = bars;             // first CTA: both CTAs' copies of a stage have landed
+  uint64_t* empty_bar = bars + kS;       // the stage's MMAs are done
+  uint64_t* accf_bar = bars + 2 * kS;    // accumulator complete
+  uint64_t* acce_bar = accf_bar + 2;     // first CTA: both CTAs' epilogues are through with an accumulator
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bars + Tr::kNumBars);
+  volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_cta_rank();
+  const int pair = blockIdx.x >> 1;
+  const int pairs = gridDim.x >> 1;
+  const int tiles = p.m_tiles * p.n_tiles;
+
+  if (warp == 0 && lane == 0) {
+    prefetch_tmap(&tm_a);
+    prefetch_tmap(&tm_b);
+    for (int s = 0; s < kS; ++s) {
+      mbar_init(smem_u32(&full_bar[s]), 1);
+      mbar_init(smem_u32(&empty_bar[s]), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(smem_u32(&accf_bar[b]), 1);
+      mbar_init(smem_u32(&acce_bar[b]), 2 * kEpiWarps);
+    }
+    *s_abort = 0;
+    fence_mbar_init();
+    fence_proxy_async_smem();
+  }
+  if (warp == 2) {
+    tmem_alloc_pair(smem_u32(s_tmem), 512);
+    tmem_relinquish_pair();
+  }
+  pdl_launch_next();
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem = *s_tmem;
+  // Everything above overlaps the previous kernel's tail.
+  pdl_wait();
+
+  if (warp == 0) {
+    // ---------------------------------------------------------- producer
+    if (lane == 0) {
+      const int b_rows = p.bn >> 1;                          // B rows this CTA stages
+      const int b_atoms = kBMn ? (b_rows + 63) >> 6 : 0;
+      const uint32_t bytes =
+          kTileBytes + (kBMn ? static_cast<uint32_t>(b_atoms) * 8192u : static_cast<uint32_t>(b_rows) * 128u) +
+          Tr::kScaleBytes;
+      int stage = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int t = pair; ok && t < tiles; t += pairs) {
+        const Tile tl = tile_at(t, p);
+        const int am = tl.m0 + static_cast<int>(rank) * 128;
+        const int bnr = tl.n0 + static_cast<int>(rank) * p.b_half;
+        for (int kb = 0; kb < p.k_iters; ++kb) {
+          if (!mbar_wait(smem_u32(&empty_bar[stage]), ph ^ 1u, s_abort, p.status, kStatusTimeoutProducer)) {
+            ok = false;
+            break;
+          }
+          const uint32_t bar = map_to_cta(smem_u32(&full_bar[stage]), 0);
+          if (rank == 0) mbar_arrive_expect_tx(smem_u32(&full_bar[stage]), 2u * bytes);
+          const uint32_t sa = smem_u32(smem + stage * Tr::kStageBytes);
+          const uint32_t sb = sa + kTileBytes;
+          if constexpr (kMx) {
+            tma_load_2d_pair(sa, &tm_a, bar, kb * 128, am);
+            tma_load_2d_pair(sb, &tm_b, bar, kb * 128, bnr);
+            const int kt = (p.k + 127) >> 7;                 // exponent tiles along K
+            const uint32_t sc = sb + kTileBytes;
+            tma_load_2d_pair(sc, &tm_sfa, bar, 0, (am >> 7) * kt + 2 * kb);
+            tma_load_2d_pair(sc + 1024, &tm_sfb, bar, 0, (tl.n0 >> 7) * kt + 2 * kb);
+            tma_load_2d_pair(sc + 2048, &tm_sfb, bar, 0, ((tl.n0 + p.b_half) >> 7) * kt + 2 * kb);
+          } else {
+            if constexpr (kAMn) {
+              tma_load_2d_pair(sa, &tm_a, bar, am, kb * 64);
+              tma_load_2d_pair(sa + 8192, &tm_a, bar, am + 64, kb * 64);
+            } else {
+              tma_load_2d_pair(sa, &tm_a, bar, kb * 64, am);
+            }
+            if constexpr (kBMn) {
+              for (int j = 0; j < b_atoms; ++j) tma_load_2d_pair(sb + j * 8192, &tm_b, bar, bnr + 64 * j, kb * 64);
+            } else {
+              tma_load_2d_pair(sb, &tm_b, bar, kb * 64, bnr);
+            }
+          }
+          if (++stage == kS) {
+            stage = 0;
+            ph ^= 1u;
+          }
+        }
+      }
+      if (!ok) drain_copies();
+    }
+  } else if (warp == 1) {
+    // --------------------------------------------------------------- MMA
+    if (lane == 0 && rank == 0) {
+      int stage = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      int it = 0;   // tiles done by this pair
+      int sfi = 0;  // stages done (exponent buffers alternate)
+      const uint32_t idesc0 = kMx ? idesc_mxf4(256, 256, 0) : idesc_f16(256, p.bn, p.type == kTypeFp16, kAMn, kBMn);
+      const uint32_t idesc1 = kMx ? idesc_mxf4(256, 256, 2) : idesc0;
+      for (int t = pair; ok && t < tiles; t += pairs, ++it) {
+        const int buf = it & 1;
+        const uint32_t d = tmem + (buf ? Tr::kAcc1 : 0);
+        if (kMx ? it >= 1 : it >= 2) {
+          const uint32_t bar = smem_u32(&acce_bar[kMx ? 0 : buf]);
+          const uint32_t par = kMx ? static_cast<uint32_t>(it - 1) & 1u : (static_cast<uint32_t>(it >> 1) - 1u) & 1u;
+          if (!mbar_wait_cluster(bar, par, s_abort, p.status, kStatusTimeoutMma)) break;
+          tc_fence_after();
+        }
+        for (int kb = 0; kb < p.k_iters; ++kb) {
+          if (!mbar_wait(smem_u32(&full_bar[stage]), ph, s_abort, p.status, kStatusTimeoutMma)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t sa = smem_u32(smem + stage * Tr::kStageBytes);
+          const uint32_t sb = sa + kTileBytes;
+          if constexpr (kMx) {
+            // The exponent columns written now were last read two stages ago.
+            if (sfi >= 2) {
+              const int old = sfi - 2;
+              if (!mbar_wait(smem_u32(&empty_bar[old % kS]), static_cast<uint32_t>(old / kS) & 1u, s_abort, p.status,
+                             kStatusTimeoutMma)) {
+                ok = false;
+                break;
+              }
+            }
+            const uint32_t sfa = tmem + Tr::kScaleCol + (sfi & 1) * 24;
+            const uint32_t sfb = sfa + 8;
+            const uint32_t sc = sb + kTileBytes;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              tmem_copy_scales<2>(sfa + 4 * j, scale_copy_desc(sc + 512 * j));
+              tmem_copy_scales<2>(sfb + 8 * j, scale_copy_desc(sc + 1024 + 512 * j));
+              tmem_copy_scales<2>(sfb + 8 * j + 4, scale_copy_desc(sc + 2048 + 512 * j));
+            }
+            const int steps = min(4, (p.k - kb * 256 + 63) >> 6);
+            for (int k = 0; k < steps; ++k)
+              umma_mxf4<2>(d, sw128_kmajor_desc(sa + k * 32), sw128_kmajor_desc(sb + k * 32), k & 1 ? idesc1 : idesc0,
+                           sfa + 4 * (k >> 1), sfb + 8 * (k >> 1), kb | k);
+            ++sfi;
+          } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const uint64_t da = kAMn ? sw128_mnmajor_desc(sa + k * 2048, 8192) : sw128_kmajor_desc(sa + k * 32);
+              const uint64_t db = kBMn ? sw128_mnmajor_desc(sb + k * 2048, 8192) : sw128_kmajor_desc(sb + k * 32);
+              umma_f16<2>(d, da, db, idesc0, kb | k);
+            }
+          }
+          umma_commit_pair(smem_u32(&empty_bar[stage]));
+          if (++stage == kS) {
+            stage = 0;
+            ph ^= 1u;
+          }
+        }
+        if (ok) umma_commit_pair(smem_u32(&accf_bar[buf]));
+      }
+    }
+  } else if (warp >= 4) {
+    // ---------------------------------------------------------- epilogue
+    const int quarter = warp & 3;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+    const int width = kGate ? p.n_step : p.bn;   // output columns of a tile
+    const int chunks = (width + 31) >> 5;
+    const bool vec32 = p.vec32 != 0;
+    int it = 0;
+    for (int t = pair; t < tiles; t += pairs, ++it) {
+      const Tile tl = tile_at(t, p);
+      const int buf = it & 1;
+      const bool ready = mbar_wait(smem_u32(&accf_bar[buf]), static_cast<uint32_t>(it >> 1) & 1u, s_abort, p.status,
+                                   kStatusTimeoutEpilogue);
+      if (!__all_sync(0xffffffffu, ready)) break;
+      tc_fence_after();
+      const uint32_t acc = lanes + (buf ? Tr::kAcc1 : 0);
+      const int64_t row = static_cast<int64_t>(tl.m0) + rank * 128 + quarter * 32 + lane;
+      const bool live = row < p.m;
+      uint32_t scale_word = 0;
+      for (int i = 0; i < chunks; ++i) {
+        // 4-bit operands: the columns shared with the other accumulator first
+        const int c = 32 * (kMx && buf == 0 ? chunks - 1 - i : i);
+        uint32_t r[32];
+        __syncwarp();
+        if constexpr (kGate) {
+          uint32_t g[32];
+          tmem_ld32(acc + c, r);
+          tmem_ld32(acc + p.n_step + c, g);
+          tmem_wait_ld();
+          if (kMx && i == (chunks > 1 ? 1 : 0)) {
+            tc_fence_before();
+            if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&acce_bar[0]), 0));
+            __syncwarp();
+          }
+          if (live && tl.n0 + c < p.n) {
+            if constexpr (kEpi == kEpiGated) {
+              if (p.preact != nullptr) {
+                float* pre = p.preact + row * (2 * static_cast<int64_t>(p.n)) + tl.n0 + c;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                  if (tl.n0 + c + 8 * j < p.n) {
+                    st_global_32(pre + 8 * j, r + 8 * j);
+                    st_global_32(pre + p.n + 8 * j, g + 8 * j);
+                  }
+              }
+            }
+            float h[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) h[j] = act_value(__uint_as_float(g[j]), p.act) * __uint_as_float(r[j]);
+            if constexpr (kEpi == kEpiGated) {
+              uint16_t* out = static_cast<uint16_t*>(p.out) + row * p.ldo;
+              uint32_t v[16];
+#pragma unroll
+              for (int j = 0; j < 16; ++j) v[j] = pack_16(h[2 * j], h[2 * j + 1], p.type);
+              store_row16(out, tl.n0 + c, p.n, v, vec32);
+              store_row16(out, tl.n0 + c + 16, p.n, v + 8, vec32);
+            } else {
+              uint32_t amax = 0;
+#pragma unroll
+              for (int j = 0; j < 32; ++j) amax = max(amax, __float_as_uint(h[j]) & 0x7fffffffu);
+              const uint32_t byte = mx_exponent(amax);
+              uint4 v = make_uint4(0, 0, 0, 0);
+              if (byte != 255u) {
+                const float inv = mx_inverse(byte);
+                v = make_uint4(mx_pack8(h, inv), mx_pack8(h + 8, inv), mx_pack8(h + 16, inv), mx_pack8(h + 24, inv));
+              }
+              *reinterpret_cast<uint4*>(p.q + (row * p.n + tl.n0 + c) / 2) = v;
+              scale_word |= byte << ((c >> 5) * 8);
+            }
+          }
+        } else {
+          tmem_ld32(acc + c, r);
+          tmem_wait_ld();
+          if (kMx && i == (chunks > 1 ? 1 : 0)) {
+            tc_fence_before();
+            if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&acce_bar[0]), 0));
+            __syncwarp();
+          }
+          if (live && tl.n0 + c < p.n) {
+            if constexpr (kEpi == kEpiStore) {
+              if (p.out_type == kTypeFp32) {
+                float* out = static_cast<float*>(p.out) + row * p.ldo + tl.n0 + c;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  if (vec32 && tl.n0 + c + 8 * j + 8 <= p.n) {
+                    st_global_32(out + 8 * j, r + 8 * j);
+                  } else {
+                    for (int e = 0; e < 8; ++e)
+                      if (tl.n0 + c + 8 * j + e < p.n) out[8 * j + e] = __uint_as_float(r[8 * j + e]);
+                  }
+                }
+              } else {
+                uint16_t* out = static_cast<uint16_t*>(p.out) + row * p.ldo;
+                uint32_t v[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                  v[j] = pack_16(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]), p.out_type);
+                if (kMx && !vec32) {
+                  // any n: column by column
+                  for (int j = 0; j < 32; ++j)
+                    if (tl.n0 + c + j < p.n) out[tl.n0 + c + j] = static_cast<uint16_t>(v[j >> 1] >> (16 * (j & 1)));
+                } else {
+                  store_row16(out, tl.n0 + c, p.n, v, vec32);
+                  store_row16(out, tl.n0 + c + 16, p.n, v + 8, vec32);
+                }
+              }
+            } else {   // kEpiDact
+              const float* pre = p.preact + row * (2 * static_cast<int64_t>(p.n)) + tl.n0 + c;
+              uint16_t* out = static_cast<uint16_t*>(p.out) + row * p.ldo;
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                uint32_t u[16] = {}, g[16] = {};
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                  if (tl.n0 + c + 16 * j + 8 * e < p.n) {
+                    ld_global_32(u + 8 * e, pre + 16 * j + 8 * e);
+                    ld_global_32(g + 8 * e, pre + p.n + 16 * j + 8 * e);
+                  }
+                uint32_t du[8], dg[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                  float v[2], w[2];
+#pragma unroll
+                  for (int l = 0; l < 2; ++l) {
+                    float value, slope;
+                    act_value_slope(__uint_as_float(g[2 * e + l]), p.act, value, slope);
+                    const float dh = __uint_as_float(r[16 * j + 2 * e + l]);
+                    v[l] = dh * value;
+                    w[l] = dh * __uint_as_float(u[2 * e + l]) * slope;
+                  }
+                  du[e] = pack_16(v[0], v[1], p.type);
+                  dg[e] = pack_16(w[0], w[1], p.type);
+                }
+                store_row16(out, tl.n0 + c + 16 * j, p.n, du, vec32);
+                store_row16(out + p.n, tl.n0 + c + 16 * j, p.n, dg, vec32);
+              }
+            }
+          }
+        }
+      }
+      if constexpr (kEpi == kEpiGatedQuant) {
+        if (live)
+          *reinterpret_cast<uint32_t*>(p.q_scale + mx_scale_offset(row, tl.n0 >> 5, (p.n + 127) >> 7)) = scale_word;
+      }
+      if (!kMx) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&acce_bar[buf]), 0));
+      }
+    }
+  }
+
+  // No CTA leaves while the other may still reach its shared or tensor memory.
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  tc_fence_after();
+  if (warp == 2) tmem_dealloc_pair(tmem, 512);
+}
+
+namespace {
+
+template <bool kMx, bool kAMn, bool kBMn, int kEpi>
+int launch_pair(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& sfa, const CUtensorMap& sfb,
+                const DenseParams& p, int sm_count, bool dependent, cudaStream_t s) {
+  auto kern = dense_pair_kernel<kMx, kAMn, kBMn, kEpi>;
+  constexpr int smem = PairTraits<kMx>::kSmemBytes;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    return MOE_B200_ERR_CUDA;
+  const int64_t tiles = static_cast<int64_t>(p.m_tiles) * p.n_tiles;
+  const int pairs = static_cast<int>(tiles < sm_count / 2 ? tiles : sm_count / 2);
+  return launch_kernel(kern, 2 * pairs, kPairThreads, smem, s, dependent, a, b, sfa, sfb, p) == cudaSuccess
+             ? MOE_B200_OK
+             : MOE_B200_ERR_CUDA;
+}
+
+}  // namespace
+
+int launch_dense_pair(DenseEpi epi, const DenseOperand& a, bool a_mn, const DenseOperand& b, bool b_mn, DenseParams p,
+                      int sm_count, bool dependent, cudaStream_t s) {
+  const bool gate = epi == kEpiGated;
+  p.bn = 256;
+  p.n_step = gate ? p.bn / 2 : p.bn;
+  p.b_half = gate ? p.n : p.bn / 2;
+  p.m_tiles = static_cast<int>(div_up(p.m, 256));
+  p.n_tiles = static_cast<int>(div_up(p.n, p.n_step));
+  p.k_iters = static_cast<int>(div_up(p.k, 64));
+  const int64_t dact_half = epi == kEpiDact ? static_cast<int64_t>(p.n) * 2 : 0;
+  p.vec32 = aligned(p.out, 32) && (p.ldo * 2) % 32 == 0 && dact_half % 32 == 0;
+  CUtensorMap ta, tb;
+  if (!encode_2d(&ta, a.base, 2, a.cols, a.rows, a.pitch, 64, a_mn ? 64 : 128) ||
+      !encode_2d(&tb, b.base, 2, b.cols, b.rows, b.pitch, 64, b_mn ? 64 : p.bn / 2))
+    return MOE_B200_ERR_DRIVER;
+  if (epi == kEpiGated && !a_mn && !b_mn)
+    return launch_pair<false, false, false, kEpiGated>(ta, tb, ta, tb, p, sm_count, dependent, s);
+  if (epi == kEpiDact && !a_mn && b_mn)
+    return launch_pair<false, false, true, kEpiDact>(ta, tb, ta, tb, p, sm_count, dependent, s);
+  if (epi == kEpiStore && !a_mn && !b_mn)
+    return launch_pair<false, false, false, kEpiStore>(ta, tb, ta, tb, p, sm_count, dependent, s);
+  if (epi == kEpiStore && !a_mn && b_mn)
+    return launch_pair<false, false, true, kEpiStore>(ta, tb, ta, tb, p, sm_count, dependent, s);
+  if (epi == kEpiStore && a_mn && b_mn)
+    return launch_pair<false, true, true, kEpiStore>(ta, tb, ta, tb, p, sm_count, dependent, s);
+  return MOE_B200_ERR_INVALID_ARGUMENT;
+}
+
+int launch_mx_pair(DenseEpi epi, const MxOperand& a, const MxOperand& b, DenseParams p, int sm_count, bool dependent,
+                   cudaStream_t s) {
+  const bool gate = epi == kEpiGatedQuant;
+  p.bn = 256;
+  p.n_step = gate ? 128 : 256;
+  p.b_half = gate ? p.n : 128;
+  p.m_tiles = static_cast<int>(div_up(p.m, 256));
+  p.n_tiles = static_cast<int>(div_up(p.n, p.n_step));
+  p.k_iters = static_cast<int>(div_up(p.k, 256));
+  const int esz = p.out_type == kTypeFp32 ? 4 : 2;
+  p.vec32 = aligned(p.out, 32) && (p.ldo * esz) % 32 == 0 && p.n % 8 == 0;
+  const int64_t kt = div_up(p.k, 128);
+  CUtensorMap ta, tb, tsa, tsb;
+  if (!encode_2d(&ta, a.q, 1, p.k / 2, a.rows, p.k / 2, 128, 128) ||
+      !encode_2d(&tb, b.q, 1, p.k / 2, b.rows, p.k / 2, 128, 128) ||
+      !encode_2d(&tsa, a.scale, 2, 256, div_up(a.rows, 128) * kt, 512, 256, 2, false) ||
+      !encode_2d(&tsb, b.scale, 2, 256, div_up(b.rows, 128) * kt, 512, 256, 2, false))
+    return MOE_B200_ERR_DRIVER;
+  if (gate) return launch_pair<true, false, false, kEpiGatedQuant>(ta, tb, tsa, tsb, p, sm_count, dependent, s);
+  return launch_pair<true, false, false, kEpiStore>(ta, tb, tsa, tsb, p, sm_count, dependent, s);
+}
+
+}  // namespace moe

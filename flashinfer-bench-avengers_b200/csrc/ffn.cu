@@ -1,0 +1,377 @@
+// C ABI of the dense feed-forward block and of 4-bit microscaled matrices
+// (declared in include/moe_b200.h): argument checks, workspaces, the choice
+// of kernel, launches. The reference has no counterpart: it implements the
+// routed experts of a layer only.
+#include <cuda_runtime.h>
+
+#include <cstdint>
+#include <cstring>
+
+#include "../../include/moe_b200.h"
+#include "dense_gemm.h"
+#include "ffn_math.cuh"
+#include "host_common.h"
+#include "moe_kernels.cuh"
+#include "mxfp4.cuh"
+
+namespace moe {
+namespace {
+
+constexpr int64_t kMaxDim = 65536;
+// Up to this many tokens the forward GEMMs stream the weights through
+// dense_skinny.cu; above, they run over CTA pairs.
+constexpr int64_t kSkinnyMaxTokens = 128;
+
+size_t round256(size_t x) { return (x + 255) / 256 * 256; }
+
+bool type16(int t) { return t == MOE_B200_TYPE_BF16 || t == MOE_B200_TYPE_FP16; }
+bool any_type(int t) { return type16(t) || t == MOE_B200_TYPE_FP32; }
+bool valid_act(int a) { return a == MOE_B200_ACT_SILU || a == MOE_B200_ACT_GELU_TANH; }
+bool tokens_ok(int64_t t) { return t >= 0 && t <= MOE_B200_MAX_TOKENS; }
+bool dim_ok(int64_t d, int64_t multiple) { return d >= multiple && d <= kMaxDim && d % multiple == 0; }
+// Pitch of a row-major operand in elements.
+bool pitch_ok(int64_t pitch, int64_t cols) { return pitch >= cols && pitch <= (int64_t(1) << 32); }
+bool pitch_aligned(int64_t pitch, int bytes) { return pitch * bytes % 16 == 0; }
+
+struct Device {
+  int sm_count;
+  uint32_t* status;
+};
+
+int open_device(Device* d) {
+  DeviceInfo di;
+  const int st = current_device_info(&di);
+  if (st != MOE_B200_OK) return st;
+  d->sm_count = di.sm_count;
+  d->status = dense_status_word();
+  return d->status != nullptr ? MOE_B200_OK : MOE_B200_ERR_CUDA;
+}
+
+DenseOperand rows_of(const void* base, int64_t rows, int64_t cols, int64_t pitch_elems) {
+  return DenseOperand{base, rows, cols, pitch_elems * 2};
+}
+
+// ---- the forward GEMMs: out = x w^T, gated or plain ------------------------
+int forward_gemm(DenseEpi epi, const DenseOperand& x, const DenseOperand& w, const DenseParams& p, const Device& d,
+                 bool dependent, cudaStream_t s) {
+  if (p.m <= kSkinnyMaxTokens) return launch_dense_skinny(epi, x, w, p, d.sm_count, dependent, s);
+  return launch_dense_pair(epi, x, false, w, false, p, d.sm_count, dependent, s);
+}
+
+// ---- 4-bit matrices ---------------------------------------------------------
+size_t mx_scale_bytes(int64_t rows, int64_t cols) {
+  return static_cast<size_t>(div_up(rows, 128)) * static_cast<size_t>(div_up(cols, 128)) * 512;
+}
+
+struct MxBuffers {
+  uint8_t* q;
+  uint8_t* scale;
+};
+
+size_t mx_bytes(int64_t rows, int64_t cols) {
+  return round256(static_cast<size_t>(rows) * cols / 2) + round256(mx_scale_bytes(rows, cols));
+}
+
+MxBuffers mx_place(uint8_t* at, int64_t rows, int64_t cols) {
+  return MxBuffers{at, at + round256(static_cast<size_t>(rows) * cols / 2)};
+}
+
+int quantize(const void* x, int type, int64_t rows, int64_t cols, int64_t pitch, uint8_t* q, uint8_t* scale,
+             bool pad, cudaStream_t s) {
+  const int k_tiles = static_cast<int>(div_up(cols, 128));
+  const int64_t pad_rows = pad ? div_up(rows, 128) * 128 : rows;
+  const unsigned grid = static_cast<unsigned>(div_up(pad_rows * 4 * k_tiles, 256));
+  const int64_t pitch_bytes = pitch * (type == MOE_B200_TYPE_FP32 ? 4 : 2);
+  const int vec32 = aligned(x, 32) && pitch_bytes % 32 == 0;
+  const uint8_t* src = static_cast<const uint8_t*>(x);
+  auto kern = type == MOE_B200_TYPE_BF16   ? mxfp4_quantize_kernel<kTypeBf16>
+              : type == MOE_B200_TYPE_FP16 ? mxfp4_quantize_kernel<kTypeFp16>
+                                           : mxfp4_quantize_kernel<kTypeFp32>;
+  kern<<<grid, 256, 0, s>>>(src, pitch_bytes, static_cast<int>(rows), static_cast<int>(cols / 32), k_tiles,
+                            static_cast<int>(pad_rows), vec32, q, scale);
+  return cudaGetLastError() == cudaSuccess ? MOE_B200_OK : MOE_B200_ERR_CUDA;
+}
+
+int mx_gemm(const MxOperand& a, const MxOperand& b, const DenseParams& p, const Device& d, bool dependent,
+            cudaStream_t s) {
+  if (p.m <= kSkinnyMaxTokens) return launch_mx_skinny(a, b, p, d.sm_count, dependent, s);
+  return launch_mx_pair(kEpiStore, a, b, p, d.sm_count, dependent, s);
+}
+
+DenseParams params(const Device& d, int64_t m, int64_t n, int64_t k, int type, int act, void* out, int64_t ldo,
+                   int out_type) {
+  DenseParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.m = m;
+  p.n = static_cast<int>(n);
+  p.k = static_cast<int>(k);
+  p.act = act;
+  p.type = type;
+  p.out = out;
+  p.ldo = ldo;
+  p.out_type = out_type;
+  p.status = d.status;
+  return p;
+}
+
+// The 4-bit block with its hidden quantised in the GEMM's epilogue needs the
+// gate rows to start on an exponent tile.
+bool fused_gate_quant(int64_t T, int64_t I) { return T > kSkinnyMaxTokens && I % 128 == 0; }
+
+size_t mx_ffn_bytes(int64_t T, int64_t H, int64_t I) {
+  return mx_bytes(T, H) + mx_bytes(T, I) + (fused_gate_quant(T, I) ? 0 : round256(static_cast<size_t>(T) * I * 8));
+}
+
+}  // namespace
+}  // namespace moe
+
+using namespace moe;
+
+extern "C" {
+
+size_t moe_b200_gated_ffn_workspace_bytes(int64_t num_tokens, int64_t hidden_size, int64_t inter_size) {
+  if (!tokens_ok(num_tokens) || !dim_ok(hidden_size, 8) || !dim_ok(inter_size, 8)) return 0;
+  return round256(static_cast<size_t>(num_tokens) * inter_size * 2) + 256;
+}
+
+int moe_b200_gated_ffn(const void* x, int64_t x_pitch, const void* w13, const void* w2, int dtype, int activation,
+                       int64_t num_tokens, int64_t hidden_size, int64_t inter_size, void* output, float* preact,
+                       void* hidden, void* workspace, size_t workspace_bytes, void* stream) {
+  const int64_t T = num_tokens, H = hidden_size, I = inter_size;
+  if (!tokens_ok(T) || !dim_ok(H, 8) || !dim_ok(I, 8) || !type16(dtype) || !valid_act(activation) ||
+      !pitch_ok(x_pitch, H))
+    return MOE_B200_ERR_INVALID_ARGUMENT;
+  if (T == 0) return MOE_B200_OK;
+  if (!x || !w13 || !w2 || !output || (!hidden && !workspace)) return MOE_B200_ERR_INVALID_ARGUMENT;
+  if (!aligned(x, 16) || !pitch_aligned(x_pitch, 2) || !aligned(w13, 16) || !aligned(w2, 16) || !aligned(output, 16) ||
+      !aligned(preact, 32) || !aligned(hidden, 16) || !aligned(workspace, 256))
+    return MOE_B200_ERR_MISALIGNED;
+  if (!hidden && workspace_bytes < moe_b200_gated_ffn_workspace_bytes(T, H, I))
+    return MOE_B200_ERR_WORKSPACE_TOO_SMALL;
+  Device d;
+  int st = open_device(&d);
+  if (st != MOE_B200_OK) return st;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  void* h = hidden ? hidden : workspace;
+  DenseParams p = params(d, T, I, H, dtype, activation, h, I, dtype);
+  p.preact = preact;
+  st = forward_gemm(kEpiGated, rows_of(x, T, H, x_pitch), rows_of(w13, 2 * I, H, H), p, d, false, s);
+  if (st != MOE_B200_OK) return st;
+  return forward_gemm(kEpiStore, rows_of(h, T, I, I), rows_of(w2, H, I, I),
+                      params(d, T, H, I, dtype, activation, output, H, dtype), d, true, s);
+}
+
+size_t moe_b200_gated_ffn_backward_workspace_bytes(int64_t num_tokens, int64_t hidden_size, int64_t inter_size) {
+  if (!tokens_ok(num_tokens) || !dim_ok(hidden_size, 8) || !dim_ok(inter_size, 8)) return 0;
+  return round256(static_cast<size_t>(num_tokens) * inter_size * 4) + 256;
+}
+
+int moe_b200_gated_ffn_backward(const void* grad_output, int64_t grad_pitch, const void* x, int64_t x_pitch,
+                                const void* w13, const void* w2, const float* preact, const void* hidden, int dtype,
+                                int activation, int64_t num_tokens, int64_t hidden_size, int64_t inter_size,
+                                void* grad_x, void* grad_w13, void* grad_w2, void* workspace, size_t workspace_bytes,
+                                void* stream) {
+  const int64_t T = num_tokens, H = hidden_size, I = inter_size;
+  if (!tokens_ok(T) || !dim_ok(H, 8) || !dim_ok(I, 8) || !type16(dtype) || !valid_act(activation) ||
+      !pitch_ok(x_pitch, H) || !pitch_ok(grad_pitch, H))
+    return MOE_B200_ERR_INVALID_ARGUMENT;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (T == 0) {
+    // sums over no tokens
+    if ((grad_w13 && cudaMemsetAsync(grad_w13, 0, static_cast<size_t>(4 * I * H), s) != cudaSuccess) ||
+        (grad_w2 && cudaMemsetAsync(grad_w2, 0, static_cast<size_t>(2 * I * H), s) != cudaSuccess))
+      return MOE_B200_ERR_CUDA;
+    return MOE_B200_OK;
+  }
+  const bool need_dact = grad_x || grad_w13;
+  if (!grad_output || (need_dact && (!w2 || !preact || !workspace)) || (grad_x && !w13) || (grad_w13 && !x) ||
+      (grad_w2 && !hidden))
+    return MOE_B200_ERR_INVALID_ARGUMENT;
+  if (!aligned(grad_output, 16) || !pitch_aligned(grad_pitch, 2) || !aligned(x, 16) || !pitch_aligned(x_pitch, 2) ||
+      !aligned(w13, 16) || !aligned(w2, 16) || !aligned(preact, 32) || !aligned(hidden, 16) || !aligned(grad_x, 16) ||
+      !aligned(grad_w13, 16) || !aligned(grad_w2, 16) || !aligned(workspace, 256))
+    return MOE_B200_ERR_MISALIGNED;
+  if (need_dact && workspace_bytes < moe_b200_gated_ffn_backward_workspace_bytes(T, H, I))
+    return MOE_B200_ERR_WORKSPACE_TOO_SMALL;
+  Device d;
+  int st = open_device(&d);
+  if (st != MOE_B200_OK) return st;
+  const DenseOperand dy = rows_of(grad_output, T, H, grad_pitch);
+  const DenseOperand dact = rows_of(workspace, T, 2 * I, 2 * I);
+  bool dependent = false;
+  if (need_dact) {
+    // dh = dy W2, and in its epilogue [du | dg]
+    DenseParams p = params(d, T, I, H, dtype, activation, workspace, 2 * I, dtype);
+    p.preact = const_cast<float*>(preact);
+    st = launch_dense_pair(kEpiDact, dy, false, rows_of(w2, H, I, I), true, p, d.sm_count, dependent, s);
+    if (st != MOE_B200_OK) return st;
+    dependent = true;
+  }
+  if (grad_w2) {
+    st = launch_dense_pair(kEpiStore, dy, true, rows_of(hidden, T, I, I), true,
+                           params(d, H, I, T, dtype, activation, grad_w2, I, dtype), d.sm_count, dependent, s);
+    if (st != MOE_B200_OK) return st;
+    dependent = true;
+  }
+  if (grad_x) {
+    st = launch_dense_pair(kEpiStore, dact, false, rows_of(w13, 2 * I, H, H), true,
+                           params(d, T, H, 2 * I, dtype, activation, grad_x, H, dtype), d.sm_count, dependent, s);
+    if (st != MOE_B200_OK) return st;
+  }
+  if (grad_w13) {
+    st = launch_dense_pair(kEpiStore, dact, true, rows_of(x, T, H, x_pitch), true,
+                           params(d, 2 * I, H, T, dtype, activation, grad_w13, H, dtype), d.sm_count, dependent, s);
+    if (st != MOE_B200_OK) return st;
+  }
+  return MOE_B200_OK;
+}
+
+size_t moe_b200_mxfp4_scale_bytes(int64_t rows, int64_t cols) {
+  if (!tokens_ok(rows) || !dim_ok(cols, 32)) return 0;
+  return mx_scale_bytes(rows, cols);
+}
+
+int moe_b200_mxfp4_quantize(const void* x, int64_t x_pitch, int dtype, int64_t rows, int64_t cols, void* q, void* scale,
+                            void* stream) {
+  if (!tokens_ok(rows) || !dim_ok(cols, 32) || !any_type(dtype) || !pitch_ok(x_pitch, cols))
+    return MOE_B200_ERR_INVALID_ARGUMENT;
+  if (rows == 0) return MOE_B200_OK;
+  if (!x || !q || !scale) return MOE_B200_ERR_INVALID_ARGUMENT;
+  if (!aligned(x, 16) || !pitch_aligned(x_pitch, dtype == MOE_B200_TYPE_FP32 ? 4 : 2) || !aligned(q, 16) ||
+      !aligned(scale, 16))
+    return MOE_B200_ERR_MISALIGNED;
+  Device d;
+  const int st = open_device(&d);
+  if (st != MOE_B200_OK) return st;
+  return quantize(x, dtype, rows, cols, x_pitch, static_cast<uint8_t*>(q), static_cast<uint8_t*>(scale), true,
+                  static_cast<cudaStream_t>(stream));
+}
+
+int moe_b200_mxfp4_dequantize(const void* q, const void* scale, int64_t rows, int64_t cols, int dtype, void* out,
+                              void* stream) {
+  if (!tokens_ok(rows) || !dim_ok(cols, 32) || !any_type(dtype)) return MOE_B200_ERR_INVALID_ARGUMENT;
+  if (rows == 0) return MOE_B200_OK;
+  if (!q || !scale || !out) return MOE_B200_ERR_INVALID_ARGUMENT;
+  if (!aligned(q, 16) || !aligned(scale, 16) || !aligned(out, 16)) return MOE_B200_ERR_MISALIGNED;
+  Device d;
+  const int st = open_device(&d);
+  if (st != MOE_B200_OK) return st;
+  const int blocks = static_cast<int>(cols / 32);
+  const int64_t total = rows * blocks;
+  auto kern = dtype == MOE_B200_TYPE_BF16   ? mxfp4_dequantize_kernel<kTypeBf16>
+              : dtype == MOE_B200_TYPE_FP16 ? mxfp4_dequantize_kernel<kTypeFp16>
+                                            : mxfp4_dequantize_kernel<kTypeFp32>;
+  kern<<<static_cast<unsigned>(div_up(total, 256)), 256, 0, static_cast<cudaStream_t>(stream)>>>(
+      static_cast<const uint8_t*>(q), static_cast<const uint8_t*>(scale), total, blocks,
+      static_cast<int>(div_up(cols, 128)), aligned(out, 32), static_cast<uint8_t*>(out));
+  return cudaGetLastError() == cudaSuccess ? MOE_B200_OK : MOE_B200_ERR_CUDA;
+}
+
+int moe_b200_mxfp4_matmul(const void* a_q, const void* a_scale, const void* b_q, const void* b_scale, int64_t m,
+                          int64_t n, int64_t k, int dtype, void* out, void* stream) {
+  if (!tokens_ok(m) || n < 1 || n > MOE_B200_MAX_TOKENS || !dim_ok(k, 32) || !any_type(dtype))
+    return MOE_B200_ERR_INVALID_ARGUMENT;
+  if (m == 0) return MOE_B200_OK;
+  if (!a_q || !a_scale || !b_q || !b_scale || !out) return MOE_B200_ERR_INVALID_ARGUMENT;
+  if (!aligned(a_q, 16) || !aligned(a_scale, 16) || !aligned(b_q, 16) || !aligned(b_scale, 16) || !aligned(out, 16))
+    return MOE_B200_ERR_MISALIGNED;
+  Device d;
+  const int st = open_device(&d);
+  if (st != MOE_B200_OK) return st;
+  return mx_gemm(MxOperand{a_q, a_scale, m}, MxOperand{b_q, b_scale, n},
+                 params(d, m, n, k, MOE_B200_TYPE_BF16, 0, out, n, dtype), d, false, static_cast<cudaStream_t>(stream));
+}
+
+size_t moe_b200_mxfp4_linear_workspace_bytes(int64_t num_tokens, int64_t k) {
+  if (!tokens_ok(num_tokens) || !dim_ok(k, 32)) return 0;
+  return mx_bytes(num_tokens, k) + 256;
+}
+
+int moe_b200_mxfp4_linear(const void* x, int64_t x_pitch, int dtype, const void* w_q, const void* w_scale,
+                          int64_t num_tokens, int64_t n, int64_t k, void* out, void* workspace, size_t workspace_bytes,
+                          void* stream) {
+  const int64_t T = num_tokens;
+  if (!tokens_ok(T) || n < 1 || n > MOE_B200_MAX_TOKENS || !dim_ok(k, 32) || !any_type(dtype) || !pitch_ok(x_pitch, k))
+    return MOE_B200_ERR_INVALID_ARGUMENT;
+  if (T == 0) return MOE_B200_OK;
+  if (!x || !w_q || !w_scale || !out || !workspace) return MOE_B200_ERR_INVALID_ARGUMENT;
+  if (!aligned(x, 16) || !pitch_aligned(x_pitch, dtype == MOE_B200_TYPE_FP32 ? 4 : 2) || !aligned(w_q, 16) ||
+      !aligned(w_scale, 16) || !aligned(out, 16) || !aligned(workspace, 256))
+    return MOE_B200_ERR_MISALIGNED;
+  if (workspace_bytes < moe_b200_mxfp4_linear_workspace_bytes(T, k)) return MOE_B200_ERR_WORKSPACE_TOO_SMALL;
+  Device d;
+  int st = open_device(&d);
+  if (st != MOE_B200_OK) return st;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const MxBuffers xq = mx_place(static_cast<uint8_t*>(workspace), T, k);
+  st = quantize(x, dtype, T, k, x_pitch, xq.q, xq.scale, false, s);
+  if (st != MOE_B200_OK) return st;
+  return mx_gemm(MxOperand{xq.q, xq.scale, T}, MxOperand{w_q, w_scale, n}, params(d, T, n, k, dtype, 0, out, n, dtype),
+                 d, true, s);
+}
+
+size_t moe_b200_mxfp4_gated_ffn_workspace_bytes(int64_t num_tokens, int64_t hidden_size, int64_t inter_size) {
+  if (!tokens_ok(num_tokens) || !dim_ok(hidden_size, 32) || !dim_ok(inter_size, 32)) return 0;
+  return mx_ffn_bytes(num_tokens, hidden_size, inter_size) + 256;
+}
+
+int moe_b200_mxfp4_gated_ffn(const void* x, int64_t x_pitch, int dtype, const void* w13_q, const void* w13_scale,
+                             const void* w2_q, const void* w2_scale, int activation, int64_t num_tokens,
+                             int64_t hidden_size, int64_t inter_size, void* output, void* workspace,
+                             size_t workspace_bytes, void* stream) {
+  const int64_t T = num_tokens, H = hidden_size, I = inter_size;
+  if (!tokens_ok(T) || !dim_ok(H, 32) || !dim_ok(I, 32) || !any_type(dtype) || !valid_act(activation) ||
+      !pitch_ok(x_pitch, H))
+    return MOE_B200_ERR_INVALID_ARGUMENT;
+  if (T == 0) return MOE_B200_OK;
+  if (!x || !w13_q || !w13_scale || !w2_q || !w2_scale || !output || !workspace) return MOE_B200_ERR_INVALID_ARGUMENT;
+  if (!aligned(x, 16) || !pitch_aligned(x_pitch, dtype == MOE_B200_TYPE_FP32 ? 4 : 2) || !aligned(w13_q, 16) ||
+      !aligned(w13_scale, 16) || !aligned(w2_q, 16) || !aligned(w2_scale, 16) || !aligned(output, 16) ||
+      !aligned(workspace, 256))
+    return MOE_B200_ERR_MISALIGNED;
+  if (workspace_bytes < moe_b200_mxfp4_gated_ffn_workspace_bytes(T, H, I)) return MOE_B200_ERR_WORKSPACE_TOO_SMALL;
+  Device d;
+  int st = open_device(&d);
+  if (st != MOE_B200_OK) return st;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  const MxBuffers xq = mx_place(ws, T, H);
+  const MxBuffers hq = mx_place(ws + mx_bytes(T, H), T, I);
+  const MxOperand xo{xq.q, xq.scale, T}, ho{hq.q, hq.scale, T};
+  const MxOperand w13{w13_q, w13_scale, 2 * I}, w2{w2_q, w2_scale, H};
+  st = quantize(x, dtype, T, H, x_pitch, xq.q, xq.scale, false, s);
+  if (st != MOE_B200_OK) return st;
+  if (fused_gate_quant(T, I)) {
+    DenseParams p = params(d, T, I, H, dtype, activation, nullptr, 0, dtype);
+    p.q = hq.q;
+    p.q_scale = hq.scale;
+    st = launch_mx_pair(kEpiGatedQuant, xo, w13, p, d.sm_count, true, s);
+    if (st != MOE_B200_OK) return st;
+  } else {
+    float* sums = reinterpret_cast<float*>(ws + mx_bytes(T, H) + mx_bytes(T, I));
+    st = mx_gemm(xo, w13, params(d, T, 2 * I, H, dtype, activation, sums, 2 * I, MOE_B200_TYPE_FP32), d, true, s);
+    if (st != MOE_B200_OK) return st;
+    const int k_tiles = static_cast<int>(div_up(I, 128));
+    if (launch_kernel(mxfp4_gate_kernel, static_cast<unsigned>(div_up(T * 4 * k_tiles, 256)), 256, 0, s, true,
+                      static_cast<const float*>(sums), static_cast<int>(T), static_cast<int>(I / 32), k_tiles,
+                      activation, hq.q, hq.scale) != cudaSuccess)
+      return MOE_B200_ERR_CUDA;
+  }
+  return mx_gemm(ho, w2, params(d, T, H, I, dtype, activation, output, H, dtype), d, true, s);
+}
+
+int moe_b200_dense_read_status(uint32_t* status, void* stream) {
+  if (status == nullptr) return MOE_B200_ERR_INVALID_ARGUMENT;
+  Device d;
+  const int st = open_device(&d);
+  if (st != MOE_B200_OK) return st;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  uint32_t v = 0;
+  if (cudaMemcpyAsync(&v, d.status, sizeof(v), cudaMemcpyDeviceToHost, s) != cudaSuccess ||
+      cudaMemsetAsync(d.status, 0, sizeof(v), s) != cudaSuccess || cudaStreamSynchronize(s) != cudaSuccess)
+    return MOE_B200_ERR_CUDA;
+  *status = v;
+  return v == 0 ? MOE_B200_OK : MOE_B200_ERR_DEVICE_TIMEOUT;
+}
+
+}  // extern "C"

@@ -19,6 +19,7 @@
 
 #include "../../include/moe_b200.h"
 #include "gemm_sm100.h"
+#include "host_common.h"
 #include "moe_kernels.cuh"
 #include "moe_shapes.cuh"
 
@@ -191,31 +192,27 @@ EncodeTiledFn get_encode_fn() {
   return fn;
 }
 
-// 2-D byte matrix [rows, inner] with row pitch `inner`, 128-byte swizzle.
-bool encode_u8_2d(CUtensorMap* m, const void* base, uint64_t inner, uint64_t rows,
-                  uint32_t box_inner, uint32_t box_rows) {
-  EncodeTiledFn fn = get_encode_fn();
-  if (fn == nullptr) return false;
-  const cuuint64_t dims[2] = {inner, rows};
-  const cuuint64_t strides[1] = {inner};
-  const cuuint32_t box[2] = {box_inner, box_rows};
-  const cuuint32_t estr[2] = {1, 1};
-  return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
-// ---------------------------------------------------------------- device
-struct DeviceInfo {
-  int checked = 0;
-  int ok = 0;
-  int sm_count = 0;
-};
-
 constexpr int kMaxDevices = 64;
 DeviceInfo g_dev[kMaxDevices];
 std::mutex g_dev_mu;
 
+}  // namespace
+
+bool encode_2d(CUtensorMap* m, const void* base, int elem_bytes, uint64_t inner, uint64_t rows, uint64_t pitch,
+               uint32_t box_inner, uint32_t box_rows, bool swizzle) {
+  EncodeTiledFn fn = get_encode_fn();
+  if (fn == nullptr) return false;
+  const cuuint64_t dims[2] = {inner, rows};
+  const cuuint64_t strides[1] = {pitch};
+  const cuuint32_t box[2] = {box_inner, box_rows};
+  const cuuint32_t estr[2] = {1, 1};
+  return fn(m, elem_bytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2,
+            const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// ---------------------------------------------------------------- device
 int current_device_info(DeviceInfo* out) {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return MOE_B200_ERR_CUDA;
@@ -237,9 +234,13 @@ int current_device_info(DeviceInfo* out) {
   return d.ok ? MOE_B200_OK : MOE_B200_ERR_UNSUPPORTED_DEVICE;
 }
 
-bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
+namespace {
 
-int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
+// 2-D byte matrix [rows, inner] with row pitch `inner`, 128-byte swizzle.
+bool encode_u8_2d(CUtensorMap* m, const void* base, uint64_t inner, uint64_t rows,
+                  uint32_t box_inner, uint32_t box_rows) {
+  return encode_2d(m, base, 1, inner, rows, inner, box_inner, box_rows);
+}
 
 // Upper bound on the number of work units of a grouped GEMM, from T only.
 int grid_for(int64_t T, int bn, int row_blocks, int splits, int sm_count) {

@@ -1,0 +1,179 @@
+// 4-bit microscaled blocks (OCP MX, e2m1 elements): quantiser, dequantiser,
+// and the quantiser of gated sums.
+//
+// A block is 32 consecutive columns of a row. Its exponent is floor(log2 of
+// the largest magnitude) - 2, its elements the nearest e2m1 numbers (ties to
+// even, beyond 6 to 6) to x / 2^exponent; scaling by a power of two is exact,
+// so the only rounding is the 4-bit one. All three kernels give one thread
+// one block: it reads whole 32-byte sectors and holds the block in registers,
+// so the block maximum needs no exchange between threads, and a warp writes
+// 512 contiguous bytes of codes. Four neighbouring threads' exponent bytes
+// are one word of the tiled array. Bound by HBM: 2 (or 4) bytes in and 17/32
+// byte out per element.
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "dense_ptx.cuh"
+#include "ffn_math.cuh"
+#include "mxfp4.cuh"
+
+namespace moe {
+
+namespace {
+
+// 32 values of a block at `src` (16-byte aligned; whole sectors if vec32).
+template <int kType>
+__device__ __forceinline__ void load_block(const void* src, bool vec32, float* v) {
+  constexpr int kWords = kType == kTypeFp32 ? 32 : 16;
+  uint32_t r[kWords];
+  if (vec32) {
+#pragma unroll
+    for (int j = 0; j < kWords; j += 8) ld_global_32(r + j, static_cast<const uint32_t*>(src) + j);
+  } else {
+#pragma unroll
+    for (int j = 0; j < kWords; j += 4) {
+      const uint4 q = *reinterpret_cast<const uint4*>(static_cast<const uint32_t*>(src) + j);
+      r[j] = q.x, r[j + 1] = q.y, r[j + 2] = q.z, r[j + 3] = q.w;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < kWords; ++j) {
+    if (kType == kTypeFp32) {
+      v[j] = __uint_as_float(r[j]);
+    } else {
+      const float2 f = unpack_16(r[j], kType);
+      v[2 * j] = f.x;
+      v[2 * j + 1] = f.y;
+    }
+  }
+}
+
+// Codes of a block, and its exponent byte into the row's word of the tiled
+// array. Called by whole warps: the four threads of a word are neighbours,
+// of the same row. `live`: the block exists; `padded`: its exponent byte does
+// (zero where the block does not).
+__device__ __forceinline__ void store_block(const float* v, bool live, bool padded, int64_t row, int block,
+                                            int k_tiles, uint8_t* q_row, uint8_t* scale) {
+  uint32_t byte = 0;
+  if (live) {
+    uint32_t amax = 0;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) amax = max(amax, __float_as_uint(v[j]) & 0x7fffffffu);
+    byte = mx_exponent(amax);
+    uint4 c = make_uint4(0, 0, 0, 0);
+    if (byte != 255u) {
+      const float inv = mx_inverse(byte);
+      c = make_uint4(mx_pack8(v, inv), mx_pack8(v + 8, inv), mx_pack8(v + 16, inv), mx_pack8(v + 24, inv));
+    }
+    *reinterpret_cast<uint4*>(q_row + 16 * static_cast<int64_t>(block)) = c;
+  }
+  uint32_t word = byte << (8 * (block & 3));
+  word |= __shfl_xor_sync(0xffffffffu, word, 1);
+  word |= __shfl_xor_sync(0xffffffffu, word, 2);
+  if (padded && (block & 3) == 0)
+    *reinterpret_cast<uint32_t*>(scale + mx_scale_offset(row, block, k_tiles)) = word;
+}
+
+}  // namespace
+
+template <int kType>
+__global__ void __launch_bounds__(256)
+    mxfp4_quantize_kernel(const uint8_t* x, int64_t pitch, int rows, int blocks, int k_tiles, int pad_rows, int vec32,
+                          uint8_t* q, uint8_t* scale) {
+  pdl_launch_next();
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int per_row = 4 * k_tiles;
+  const int row = static_cast<int>(i / per_row);
+  const int block = static_cast<int>(i - static_cast<int64_t>(row) * per_row);
+  const bool live = row < rows && block < blocks;
+  float v[32];
+  if (live)
+    load_block<kType>(x + row * pitch + static_cast<int64_t>(block) * (kType == kTypeFp32 ? 128 : 64), vec32 != 0, v);
+  store_block(v, live, row < pad_rows, row, block, k_tiles, q + static_cast<int64_t>(row) * blocks * 16, scale);
+}
+
+// h = act(gate) * up of fp32 sums [rows, 2 n] (up, then gate), in 4 bits.
+__global__ void __launch_bounds__(256)
+    mxfp4_gate_kernel(const float* sums, int rows, int blocks, int k_tiles, int act, uint8_t* q, uint8_t* scale) {
+  pdl_launch_next();
+  pdl_wait();
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int per_row = 4 * k_tiles;
+  const int row = static_cast<int>(i / per_row);
+  const int block = static_cast<int>(i - static_cast<int64_t>(row) * per_row);
+  const bool live = row < rows && block < blocks;
+  float v[32];
+  if (live) {
+    const float* up = sums + static_cast<int64_t>(row) * 64 * blocks + 32 * block;
+    float g[32];
+    load_block<kTypeFp32>(up, true, v);
+    load_block<kTypeFp32>(up + 32 * blocks, true, g);
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] *= act_value(g[j], act);
+  }
+  store_block(v, live, row < rows, row, block, k_tiles, q + static_cast<int64_t>(row) * blocks * 16, scale);
+}
+
+template <int kType>
+__global__ void __launch_bounds__(256)
+    mxfp4_dequantize_kernel(const uint8_t* q, const uint8_t* scale, int64_t total, int blocks, int k_tiles, int vec32,
+                            uint8_t* out) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= total) return;
+  const int64_t row = i / blocks;
+  const int block = static_cast<int>(i - row * blocks);
+  const uint32_t byte = scale[mx_scale_offset(row, block, k_tiles)];
+  // 2^(byte - 127); byte 0 is a subnormal, 255 is NaN
+  const float f = __uint_as_float(byte == 0u ? 0x00400000u : byte == 255u ? 0x7fc00000u : byte << 23);
+  const uint4 c = *reinterpret_cast<const uint4*>(q + 16 * i);
+  const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+  float v[32];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    uint32_t h[4];
+    asm("{\n\t.reg .b8 t0, t1, t2, t3;\n\t"
+        "mov.b32 {t0, t1, t2, t3}, %4;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %0, t0;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %1, t1;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %2, t2;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %3, t3;\n\t}"
+        : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+        : "r"(w[j]));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 p = unpack_16(h[e], kTypeFp16);
+      v[8 * j + 2 * e] = p.x * f;
+      v[8 * j + 2 * e + 1] = p.y * f;
+    }
+  }
+  constexpr int kWords = kType == kTypeFp32 ? 32 : 16;
+  uint32_t r[kWords];
+#pragma unroll
+  for (int j = 0; j < kWords; ++j)
+    r[j] = kType == kTypeFp32 ? __float_as_uint(v[j]) : pack_16(v[(2 * j) & 31], v[(2 * j + 1) & 31], kType);
+  uint32_t* dst = reinterpret_cast<uint32_t*>(out) + i * kWords;
+  if (vec32) {
+#pragma unroll
+    for (int j = 0; j < kWords; j += 8) st_global_32(dst + j, r + j);
+  } else {
+#pragma unroll
+    for (int j = 0; j < kWords; j += 4)
+      *reinterpret_cast<uint4*>(dst + j) = make_uint4(r[j], r[j + 1], r[j + 2], r[j + 3]);
+  }
+}
+
+template __global__ void mxfp4_quantize_kernel<kTypeBf16>(const uint8_t*, int64_t, int, int, int, int, int, uint8_t*,
+                                                          uint8_t*);
+template __global__ void mxfp4_quantize_kernel<kTypeFp16>(const uint8_t*, int64_t, int, int, int, int, int, uint8_t*,
+                                                          uint8_t*);
+template __global__ void mxfp4_quantize_kernel<kTypeFp32>(const uint8_t*, int64_t, int, int, int, int, int, uint8_t*,
+                                                          uint8_t*);
+template __global__ void mxfp4_dequantize_kernel<kTypeBf16>(const uint8_t*, const uint8_t*, int64_t, int, int, int,
+                                                            uint8_t*);
+template __global__ void mxfp4_dequantize_kernel<kTypeFp16>(const uint8_t*, const uint8_t*, int64_t, int, int, int,
+                                                            uint8_t*);
+template __global__ void mxfp4_dequantize_kernel<kTypeFp32>(const uint8_t*, const uint8_t*, int64_t, int, int, int,
+                                                            uint8_t*);
+
+}  // namespace moe

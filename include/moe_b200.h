@@ -445,6 +445,120 @@ MOE_B200_API int moe_b200_a2a_combine(const int32_t* topk_idx, void* const* shar
                                       void* output, void* stream);
 MOE_B200_API int moe_b200_a2a_read_status(const void* area, uint32_t* status, int32_t* recv_rows, void* stream);
 
+/*
+ * Dense operators beside the routed experts: the gated feed-forward block
+ * that every token passes (the shared expert of a layer) with its gradients,
+ * and 4-bit microscaled matrices with the block's 4-bit serving form. The
+ * reference implements the routed experts only (solution/cuda/main.cpp:13-142),
+ * so none of them has a counterpart there.
+ *
+ * All are asynchronous on `stream`, allocate nothing and do no host
+ * synchronisation; they may be captured in a CUDA graph. Sizes are arguments:
+ * num_tokens up to MOE_B200_MAX_TOKENS, hidden_size and inter_size up to 65536.
+ * Matrices are row-major; `*_pitch` is the distance between rows in elements
+ * (rows may lie apart, each row contiguous and starting on 16 bytes). All
+ * pointers are 16-byte aligned, preact 32, workspaces 256. Workspaces are
+ * scratch: calls that may overlap need one each, and so do two captured
+ * graphs that may.
+ */
+#define MOE_B200_TYPE_BF16 0
+#define MOE_B200_TYPE_FP16 1
+#define MOE_B200_TYPE_FP32 2
+#define MOE_B200_ACT_SILU 0
+#define MOE_B200_ACT_GELU_TANH 1
+
+/*
+ * Gated feed-forward block: with [u | g] = x w13^T (rows [0, I) of w13 up,
+ * [I, 2I) gate, the order of gemm1_weights above), h = act(g) * u and
+ * output = h w2^T. fp32 sums; h is rounded once to `dtype`, the type (bf16 or
+ * fp16) of x, the weights and the output.
+ *   x [T, H], w13 [2I, H], w2 [H, I], output [T, H]; H and I multiples of 8
+ *   preact   fp32 [T, 2I] or NULL: receives u and g, for the gradients (kept
+ *            in 32 bits, because their rounding would enter du and dg)
+ *   hidden   [T, I] or NULL: receives h; NULL keeps it in the workspace
+ * workspace may be NULL when hidden is given.
+ */
+MOE_B200_API size_t moe_b200_gated_ffn_workspace_bytes(int64_t num_tokens, int64_t hidden_size, int64_t inter_size);
+MOE_B200_API int moe_b200_gated_ffn(const void* x, int64_t x_pitch, const void* w13, const void* w2, int dtype,
+                                    int activation, int64_t num_tokens, int64_t hidden_size, int64_t inter_size,
+                                    void* output, float* preact, void* hidden, void* workspace,
+                                    size_t workspace_bytes, void* stream);
+
+/*
+ * Gradients of the block for grad_output [T, H], from the preact and hidden
+ * that the forward call saved: with dh = grad_output w2, du = dh act(g) and
+ * dg = dh u act'(g) (rounded to dtype as operands of the products below),
+ *   grad_x   = [du | dg] w13          [T, H]
+ *   grad_w13 = [du | dg]^T x          [2I, H]
+ *   grad_w2  = grad_output^T hidden   [H, I]
+ * Any gradient may be NULL and is then not computed (with it the inputs that
+ * only it needs may be NULL). Written in full, not added to; no atomics, so
+ * repeated calls agree bit for bit. With no tokens the weights' gradients
+ * are set to zero.
+ */
+MOE_B200_API size_t moe_b200_gated_ffn_backward_workspace_bytes(int64_t num_tokens, int64_t hidden_size,
+                                                                int64_t inter_size);
+MOE_B200_API int moe_b200_gated_ffn_backward(const void* grad_output, int64_t grad_pitch, const void* x,
+                                             int64_t x_pitch, const void* w13, const void* w2, const float* preact,
+                                             const void* hidden, int dtype, int activation, int64_t num_tokens,
+                                             int64_t hidden_size, int64_t inter_size, void* grad_x, void* grad_w13,
+                                             void* grad_w2, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * 4-bit microscaled matrices (OCP MXFP4). A block is 32 consecutive columns
+ * of a row: its exponent is floor(log2 amax) - 2 (at least -127), its values
+ * are e2m1 numbers (0, .5, 1, 1.5, 2, 3, 4, 6 and their negatives), x divided
+ * by 2^exponent and rounded to nearest, ties to even, beyond 6 to 6. A block
+ * with an infinity or a NaN gets the NaN exponent 255: its values are NaN.
+ *   q      [R, K / 2] bytes, column 2j in the low nibble of byte j
+ *   scale  moe_b200_mxfp4_scale_bytes(R, K) bytes: the exponents + 127 in
+ *          tiles of 128 rows x 4 blocks, the order in which the tensor cores
+ *          take them: row r, block b at
+ *          ((r / 128) ceil(K / 128) + b / 4) 512 + (r % 32) 16 + (r % 128) / 32 * 4 + b % 4
+ *          Places of blocks and rows that do not exist hold 0.
+ * K is a multiple of 32. dtype: any of the three types.
+ */
+MOE_B200_API size_t moe_b200_mxfp4_scale_bytes(int64_t rows, int64_t cols);
+MOE_B200_API int moe_b200_mxfp4_quantize(const void* x, int64_t x_pitch, int dtype, int64_t rows, int64_t cols,
+                                         void* q, void* scale, void* stream);
+MOE_B200_API int moe_b200_mxfp4_dequantize(const void* q, const void* scale, int64_t rows, int64_t cols, int dtype,
+                                           void* out, void* stream);
+
+/*
+ * out [m, n] = A B^T of two 4-bit matrices A [m, k], B [n, k]: the products
+ * of values and exponents summed in fp32, rounded once to dtype. m up to
+ * MOE_B200_MAX_TOKENS, any n up to it.
+ */
+MOE_B200_API int moe_b200_mxfp4_matmul(const void* a_q, const void* a_scale, const void* b_q, const void* b_scale,
+                                       int64_t m, int64_t n, int64_t k, int dtype, void* out, void* stream);
+
+/* The same with A = the 4-bit form of x [T, k], made inside the call. */
+MOE_B200_API size_t moe_b200_mxfp4_linear_workspace_bytes(int64_t num_tokens, int64_t k);
+MOE_B200_API int moe_b200_mxfp4_linear(const void* x, int64_t x_pitch, int dtype, const void* w_q, const void* w_scale,
+                                       int64_t num_tokens, int64_t n, int64_t k, void* out, void* workspace,
+                                       size_t workspace_bytes, void* stream);
+
+/*
+ * The gated feed-forward block in 4 bits: with Q the quantiser above,
+ * [u | g] = Q(x) w13^T, output = Q(act(g) * u) w2^T; the hidden goes from its
+ * fp32 value to 4 bits without another rounding. H and I multiples of 32.
+ */
+MOE_B200_API size_t moe_b200_mxfp4_gated_ffn_workspace_bytes(int64_t num_tokens, int64_t hidden_size,
+                                                             int64_t inter_size);
+MOE_B200_API int moe_b200_mxfp4_gated_ffn(const void* x, int64_t x_pitch, int dtype, const void* w13_q,
+                                          const void* w13_scale, const void* w2_q, const void* w2_scale,
+                                          int activation, int64_t num_tokens, int64_t hidden_size,
+                                          int64_t inter_size, void* output, void* workspace,
+                                          size_t workspace_bytes, void* stream);
+
+/*
+ * Status word of the dense operators on the current device: bits 1 << 0..2
+ * (moe_b200_read_status) since the last read, set when a kernel gave up a
+ * bounded wait; outputs of calls since then are not valid. Synchronises
+ * `stream` and clears the word; MOE_B200_ERR_DEVICE_TIMEOUT when it was set.
+ */
+MOE_B200_API int moe_b200_dense_read_status(uint32_t* status, void* stream);
+
 /* ABI version of this header (bumped on any signature or struct layout change). */
 MOE_B200_API int moe_b200_abi_version(void);
 
