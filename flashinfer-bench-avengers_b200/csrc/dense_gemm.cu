@@ -211,10 +211,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       int stage = 0;
       uint32_t ph = 0;
       bool ok = true;
-      int it = 0;   // tiles done by this pair
-      int sfi = 0;  // stages done (exponent buffers alternate)
+      int it = 0;                 // tiles done by this pair
+      int old = kS - 2;           // 4-bit: the stage before last, and its phase
+      uint32_t old_ph = 1, sf = 0;
       const uint32_t idesc0 = kMx ? idesc_mxf4(256, 256, 0) : idesc_f16(256, p.bn, p.type == kTypeFp16, kAMn, kBMn);
       const uint32_t idesc1 = kMx ? idesc_mxf4(256, 256, 2) : idesc0;
+      const uint32_t base = smem_u32(smem);
+      const uint32_t lo_a0 = kAMn ? desc_lo_mnmajor(base) : desc_lo_kmajor(base);
+      const uint32_t lo_b0 = kBMn ? desc_lo_mnmajor(base + kTileBytes) : desc_lo_kmajor(base + kTileBytes);
+      const uint32_t lo_s0 = desc_lo_scale(base + 2 * kTileBytes);
       for (int t = pair; ok && t < tiles; t += pairs, ++it) {
         const int buf = it & 1;
         const uint32_t d = tmem + (buf ? Tr::kAcc1 : 0);
@@ -229,40 +234,42 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             ok = false;
             break;
           }
-          tc_fence_after();
-          const uint32_t sa = smem_u32(smem + stage * Tr::kStageBytes);
-          const uint32_t sb = sa + kTileBytes;
+          const uint32_t off = static_cast<uint32_t>(stage) * (Tr::kStageBytes >> 4);
+          const uint32_t lo_a = lo_a0 + off, lo_b = lo_b0 + off;
           if constexpr (kMx) {
-            // The exponent columns written now were last read two stages ago.
-            if (sfi >= 2) {
-              const int old = sfi - 2;
-              if (!mbar_wait(smem_u32(&empty_bar[old % kS]), static_cast<uint32_t>(old / kS) & 1u, s_abort, p.status,
-                             kStatusTimeoutMma)) {
-                ok = false;
-                break;
-              }
+            // The exponent columns written now were last read two stages ago
+            // (the first two waits pass at once).
+            if (!mbar_wait(smem_u32(&empty_bar[old]), old_ph, s_abort, p.status, kStatusTimeoutMma)) {
+              ok = false;
+              break;
             }
-            const uint32_t sfa = tmem + Tr::kScaleCol + (sfi & 1) * 24;
+            if (++old == kS) {
+              old = 0;
+              old_ph ^= 1u;
+            }
+            tc_fence_after();
+            const uint32_t lo_s = lo_s0 + off;
+            const uint32_t sfa = tmem + Tr::kScaleCol + sf;
             const uint32_t sfb = sfa + 8;
-            const uint32_t sc = sb + kTileBytes;
+            sf ^= 24u;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              tmem_copy_scales<2>(sfa + 4 * j, scale_copy_desc(sc + 512 * j));
-              tmem_copy_scales<2>(sfb + 8 * j, scale_copy_desc(sc + 1024 + 512 * j));
-              tmem_copy_scales<2>(sfb + 8 * j + 4, scale_copy_desc(sc + 2048 + 512 * j));
+              tmem_copy_scales<2>(sfa + 4 * j, desc_of(kDescHiPlain, lo_s + 32 * j));
+              tmem_copy_scales<2>(sfb + 8 * j, desc_of(kDescHiPlain, lo_s + 64 + 32 * j));
+              tmem_copy_scales<2>(sfb + 8 * j + 4, desc_of(kDescHiPlain, lo_s + 128 + 32 * j));
             }
-            const int steps = min(4, (p.k - kb * 256 + 63) >> 6);
-            for (int k = 0; k < steps; ++k)
-              umma_mxf4<2>(d, sw128_kmajor_desc(sa + k * 32), sw128_kmajor_desc(sb + k * 32), k & 1 ? idesc1 : idesc0,
-                           sfa + 4 * (k >> 1), sfb + 8 * (k >> 1), kb | k);
-            ++sfi;
-          } else {
+            const int left = p.k - kb * 256;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const uint64_t da = kAMn ? sw128_mnmajor_desc(sa + k * 2048, 8192) : sw128_kmajor_desc(sa + k * 32);
-              const uint64_t db = kBMn ? sw128_mnmajor_desc(sb + k * 2048, 8192) : sw128_kmajor_desc(sb + k * 32);
-              umma_f16<2>(d, da, db, idesc0, kb | k);
-            }
+            for (int k = 0; k < 4; ++k)
+              if (k == 0 || left > 64 * k)
+                umma_mxf4<2>(d, desc_of(kDescHiSw128, lo_a + 2 * k), desc_of(kDescHiSw128, lo_b + 2 * k),
+                             k & 1 ? idesc1 : idesc0, sfa + 4 * (k >> 1), sfb + 8 * (k >> 1), kb | k);
+          } else {
+            tc_fence_after();
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              umma_f16<2>(d, desc_of(kDescHiSw128, lo_a + (kAMn ? 128 : 2) * k),
+                          desc_of(kDescHiSw128, lo_b + (kBMn ? 128 : 2) * k), idesc0, kb | k);
           }
           umma_commit_pair(smem_u32(&empty_bar[stage]));
           if (++stage == kS) {

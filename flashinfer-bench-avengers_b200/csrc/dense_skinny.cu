@@ -138,44 +138,57 @@ __global__ void __launch_bounds__(kSkinnyThreads, 1)
       const uint32_t idesc0 =
           kMx ? idesc_mxf4(128, sh.bn, 0) : idesc_f16(128, sh.bn, p.type == kTypeFp16, false, false);
       const uint32_t idesc1 = kMx ? idesc_mxf4(128, sh.bn, 2) : idesc0;
+      const uint32_t lo_w0 = desc_lo_kmajor(smem_u32(smem));
+      const uint32_t lo_x0 = lo_w0 + (kWeightTile >> 4);
+      const uint32_t lo_s0 = desc_lo_scale(smem_u32(smem) + kWeightTile + sh.bn * 128);
       bool ok = true;
+      int stage = 0, old = sh.stages - 2;   // 4-bit: the stage before last, and its phase
+      uint32_t ph = 0, old_ph = 1, sf = 0;
       for (int i = 0; i < iters; ++i) {
-        const int stage = i % sh.stages;
-        if (!mbar_wait(smem_u32(&full_bar[stage]), static_cast<uint32_t>(i / sh.stages) & 1u, s_abort, p.status,
-                       kStatusTimeoutMma)) {
+        if (!mbar_wait(smem_u32(&full_bar[stage]), ph, s_abort, p.status, kStatusTimeoutMma)) {
           ok = false;
           break;
         }
-        tc_fence_after();
-        const uint32_t sw = smem_u32(smem + stage * sh.stage_bytes);
-        const uint32_t sx = sw + kWeightTile;
+        const uint32_t off = static_cast<uint32_t>(stage * (sh.stage_bytes >> 4));
+        const uint32_t lo_w = lo_w0 + off, lo_x = lo_x0 + off;
         if constexpr (kMx) {
-          if (i >= 2) {   // these exponent columns were last read two stages ago
-            const int old = i - 2;
-            if (!mbar_wait(smem_u32(&empty_bar[old % sh.stages]), static_cast<uint32_t>(old / sh.stages) & 1u, s_abort,
-                           p.status, kStatusTimeoutMma)) {
-              ok = false;
-              break;
-            }
+          // these exponent columns were last read two stages ago (the first
+          // two waits pass at once)
+          if (!mbar_wait(smem_u32(&empty_bar[old]), old_ph, s_abort, p.status, kStatusTimeoutMma)) {
+            ok = false;
+            break;
           }
-          const uint32_t sfw = tmem + 128 + (i & 1) * 16;
+          if (++old == sh.stages) {
+            old = 0;
+            old_ph ^= 1u;
+          }
+          tc_fence_after();
+          const uint32_t lo_s = lo_s0 + off;
+          const uint32_t sfw = tmem + 128 + sf;
           const uint32_t sfx = sfw + 8;
-          const uint32_t sc = sx + sh.bn * 128;
+          sf ^= 16u;
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            tmem_copy_scales<1>(sfw + 4 * j, scale_copy_desc(sc + 512 * j));
-            tmem_copy_scales<1>(sfx + 4 * j, scale_copy_desc(sc + 1024 + 512 * j));
+            tmem_copy_scales<1>(sfw + 4 * j, desc_of(kDescHiPlain, lo_s + 32 * j));
+            tmem_copy_scales<1>(sfx + 4 * j, desc_of(kDescHiPlain, lo_s + 64 + 32 * j));
           }
-          const int steps = min(4, (p.k - (kb0 + i) * 256 + 63) >> 6);
-          for (int k = 0; k < steps; ++k)
-            umma_mxf4<1>(tmem, sw128_kmajor_desc(sw + k * 32), sw128_kmajor_desc(sx + k * 32), k & 1 ? idesc1 : idesc0,
-                         sfw + 4 * (k >> 1), sfx + 4 * (k >> 1), i | k);
-        } else {
+          const int left = p.k - (kb0 + i) * 256;
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            umma_f16<1>(tmem, sw128_kmajor_desc(sw + k * 32), sw128_kmajor_desc(sx + k * 32), idesc0, i | k);
+            if (k == 0 || left > 64 * k)
+              umma_mxf4<1>(tmem, desc_of(kDescHiSw128, lo_w + 2 * k), desc_of(kDescHiSw128, lo_x + 2 * k),
+                           k & 1 ? idesc1 : idesc0, sfw + 4 * (k >> 1), sfx + 4 * (k >> 1), i | k);
+        } else {
+          tc_fence_after();
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma_f16<1>(tmem, desc_of(kDescHiSw128, lo_w + 2 * k), desc_of(kDescHiSw128, lo_x + 2 * k), idesc0, i | k);
         }
         umma_commit(smem_u32(&empty_bar[stage]));
+        if (++stage == sh.stages) {
+          stage = 0;
+          ph ^= 1u;
+        }
       }
       if (ok) umma_commit(smem_u32(done_bar));
     }
