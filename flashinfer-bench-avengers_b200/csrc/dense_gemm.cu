@@ -85,8 +85,8 @@ __device__ __forceinline__ Tile tile_at(int t, const DenseParams& p) {
   return o;
 }
 
-// Writes 16 consecutive 16-bit outputs (columns c .. c+15 of a row with n
-// columns, n and c multiples of 8).
+// Writes 16 consecutive 16-bit outputs: columns c .. c+15 of a row, those
+// below n (n and c multiples of 8).
 __device__ __forceinline__ void store_row16(uint16_t* row, int c, int n, const uint32_t* v, bool vec32) {
   if (vec32 && c + 16 <= n) {
     st_global_32(row + c, v);
@@ -298,6 +298,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       const uint32_t acc = lanes + (buf ? Tr::kAcc1 : 0);
       const int64_t row = static_cast<int64_t>(tl.m0) + rank * 128 + quarter * 32 + lane;
       const bool live = row < p.m;
+      const int end = min(p.n, tl.n0 + width);   // first column past this tile
       uint32_t scale_word = 0;
       for (int i = 0; i < chunks; ++i) {
         // 4-bit operands: the columns shared with the other accumulator first
@@ -314,13 +315,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&acce_bar[0]), 0));
             __syncwarp();
           }
-          if (live && tl.n0 + c < p.n) {
+          if (live && tl.n0 + c < end) {
             if constexpr (kEpi == kEpiGated) {
               if (p.preact != nullptr) {
                 float* pre = p.preact + row * (2 * static_cast<int64_t>(p.n)) + tl.n0 + c;
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                  if (tl.n0 + c + 8 * j < p.n) {
+                  if (tl.n0 + c + 8 * j < end) {
                     st_global_32(pre + 8 * j, r + 8 * j);
                     st_global_32(pre + p.n + 8 * j, g + 8 * j);
                   }
@@ -334,8 +335,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
               uint32_t v[16];
 #pragma unroll
               for (int j = 0; j < 16; ++j) v[j] = pack_16(h[2 * j], h[2 * j + 1], p.type);
-              store_row16(out, tl.n0 + c, p.n, v, vec32);
-              store_row16(out, tl.n0 + c + 16, p.n, v + 8, vec32);
+              store_row16(out, tl.n0 + c, end, v, vec32);
+              store_row16(out, tl.n0 + c + 16, end, v + 8, vec32);
             } else {
               uint32_t amax = 0;
 #pragma unroll
@@ -358,17 +359,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&acce_bar[0]), 0));
             __syncwarp();
           }
-          if (live && tl.n0 + c < p.n) {
+          if (live && tl.n0 + c < end) {
             if constexpr (kEpi == kEpiStore) {
               if (p.out_type == kTypeFp32) {
                 float* out = static_cast<float*>(p.out) + row * p.ldo + tl.n0 + c;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                  if (vec32 && tl.n0 + c + 8 * j + 8 <= p.n) {
+                  if (vec32 && tl.n0 + c + 8 * j + 8 <= end) {
                     st_global_32(out + 8 * j, r + 8 * j);
                   } else {
                     for (int e = 0; e < 8; ++e)
-                      if (tl.n0 + c + 8 * j + e < p.n) out[8 * j + e] = __uint_as_float(r[8 * j + e]);
+                      if (tl.n0 + c + 8 * j + e < end) out[8 * j + e] = __uint_as_float(r[8 * j + e]);
                   }
                 }
               } else {
@@ -380,10 +381,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                 if (kMx && !vec32) {
                   // any n: column by column
                   for (int j = 0; j < 32; ++j)
-                    if (tl.n0 + c + j < p.n) out[tl.n0 + c + j] = static_cast<uint16_t>(v[j >> 1] >> (16 * (j & 1)));
+                    if (tl.n0 + c + j < end) out[tl.n0 + c + j] = static_cast<uint16_t>(v[j >> 1] >> (16 * (j & 1)));
                 } else {
-                  store_row16(out, tl.n0 + c, p.n, v, vec32);
-                  store_row16(out, tl.n0 + c + 16, p.n, v + 8, vec32);
+                  store_row16(out, tl.n0 + c, end, v, vec32);
+                  store_row16(out, tl.n0 + c + 16, end, v + 8, vec32);
                 }
               }
             } else {   // kEpiDact
@@ -394,7 +395,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                 uint32_t u[16] = {}, g[16] = {};
 #pragma unroll
                 for (int e = 0; e < 2; ++e)
-                  if (tl.n0 + c + 16 * j + 8 * e < p.n) {
+                  if (tl.n0 + c + 16 * j + 8 * e < end) {
                     ld_global_32(u + 8 * e, pre + 16 * j + 8 * e);
                     ld_global_32(g + 8 * e, pre + p.n + 16 * j + 8 * e);
                   }
@@ -413,8 +414,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                   du[e] = pack_16(v[0], v[1], p.type);
                   dg[e] = pack_16(w[0], w[1], p.type);
                 }
-                store_row16(out, tl.n0 + c + 16 * j, p.n, du, vec32);
-                store_row16(out + p.n, tl.n0 + c + 16 * j, p.n, dg, vec32);
+                store_row16(out, tl.n0 + c + 16 * j, end, du, vec32);
+                store_row16(out + p.n, tl.n0 + c + 16 * j, end, dg, vec32);
               }
             }
           }
@@ -457,12 +458,37 @@ int launch_pair(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& s
              : MOE_B200_ERR_CUDA;
 }
 
+// Columns per tile (the MMA's N, 64 to 256): the fewest time units over all
+// waves of tiles. A K step costs an MMA 2 N cycles and the loads 256 + N (A's
+// 128 rows and N / 2 rows of B per CTA; at about 64 bytes a cycle from L2 the
+// two meet at N = 256); a tile's start and epilogue cost about 1500 more.
+// B stored along N is loaded in 64-column atoms whatever N is. Against 256
+// throughout: V_TEXT.
+int choose_bn(const DenseParams& p, bool gate, bool b_mn, int pairs) {
+  const int64_t m_tiles = div_up(p.m, 256), k = div_up(p.k, 64);
+  int best = 256;
+  int64_t best_cost = INT64_MAX;
+  // the columns of a tile come in whole 32-byte stores: 16 features
+  for (int bn = 256; bn >= 64; bn -= gate ? 32 : 16) {
+    const int step = gate ? bn / 2 : bn;
+    const int64_t waves = div_up(m_tiles * div_up(p.n, step), pairs);
+    const int64_t b_cols = b_mn ? div_up(bn / 2, 64) * 128 : bn;
+    const int64_t load = 256 + b_cols, mma = 2 * bn;
+    const int64_t cost = waves * (k * (load > mma ? load : mma) + 1500);
+    if (cost < best_cost) {
+      best_cost = cost;
+      best = bn;
+    }
+  }
+  return best;
+}
+
 }  // namespace
 
 int launch_dense_pair(DenseEpi epi, const DenseOperand& a, bool a_mn, const DenseOperand& b, bool b_mn, DenseParams p,
                       int sm_count, bool dependent, cudaStream_t s) {
   const bool gate = epi == kEpiGated;
-  p.bn = 256;
+  p.bn = choose_bn(p, gate, b_mn, sm_count / 2);
   p.n_step = gate ? p.bn / 2 : p.bn;
   p.b_half = gate ? p.n : p.bn / 2;
   p.m_tiles = static_cast<int>(div_up(p.m, 256));

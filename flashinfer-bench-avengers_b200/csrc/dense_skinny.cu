@@ -13,9 +13,12 @@
 // Gated form: the tile's 128 rows are 64 up rows and the 64 gate rows of the
 // same features, and the adding thread applies the activation.
 //
-// The first ring of weight tiles is requested before the kernel waits for
-// its predecessor (programmatic dependent launch): weights are inputs of the
-// whole call, only the token operand comes from the kernel before.
+// Two GEMMs of a call overlap (programmatic dependent launch): weights are
+// inputs of the whole call, so a kernel requests its first ring of weight
+// tiles before it waits for its predecessor; only the token operand comes
+// from the kernel before. It is let go when its predecessor requests its own
+// last ring, so HBM does not idle under the first one's tail. (Asking for the
+// rest of the K range into L2 as well was no faster.)
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -36,15 +39,18 @@ namespace {
 constexpr int kSkinnyThreads = 128;
 constexpr int kMaxStages = 12;
 constexpr int kWeightTile = 16384;             // 128 rows of 128 bytes
-constexpr int kRingBytes = 212 * 1024;
-constexpr int kSkinnySmem = kRingBytes + (2 * kMaxStages + 1) * 8 + 16 + 1024;
-static_assert(kSkinnySmem <= 227 * 1024, "shared memory");
+constexpr int kRingSmall = 108 * 1024;          // two CTAs per SM
+constexpr int kRingLarge = 212 * 1024;
+constexpr int kSkinnyExtra = (2 * kMaxStages + 1) * 8 + 16 + 1024;
+static_assert(kRingLarge + kSkinnyExtra <= 227 * 1024, "shared memory");
+static_assert(2 * (kRingSmall + kSkinnyExtra + 1024) <= 228 * 1024, "two CTAs per SM");
 
 struct SkinnyShape {
   int bn;            // tokens per tile (multiple of 16)
   int splits;        // CTAs per cluster
   int stages;
   int stage_bytes;
+  int ring_bytes;
 };
 
 }  // namespace
@@ -57,7 +63,7 @@ __global__ void __launch_bounds__(kSkinnyThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kRingBytes);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + sh.ring_bytes);
   uint64_t* full_bar = bars;
   uint64_t* empty_bar = bars + kMaxStages;
   uint64_t* done_bar = bars + 2 * kMaxStages;
@@ -90,7 +96,6 @@ __global__ void __launch_bounds__(kSkinnyThreads, 1)
     tmem_alloc(smem_u32(s_tmem), kCols);
     tmem_relinquish();
   }
-  pdl_launch_next();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -119,6 +124,10 @@ __global__ void __launch_bounds__(kSkinnyThreads, 1)
       };
       const int first = min(sh.stages, iters);
       for (int i = 0; i < first; ++i) load_w(i, i);
+      // The next kernel of the call may start once this CTA requests its last
+      // ring (25.5 us for the block at one token; 26.3 released at the start).
+      const int release = max(iters - sh.stages, 0);
+      if (release < first) pdl_launch_next();
       pdl_wait();
       for (int i = 0; i < first; ++i) load_x(i, i);
       for (int i = first; i < iters; ++i) {
@@ -130,6 +139,7 @@ __global__ void __launch_bounds__(kSkinnyThreads, 1)
         }
         load_w(i, stage);
         load_x(i, stage);
+        if (i == release) pdl_launch_next();
       }
     }
     __syncwarp();
@@ -214,45 +224,66 @@ __global__ void __launch_bounds__(kSkinnyThreads, 1)
   // --------------------------- this CTA's share of the columns, all parts
   if (all_ready) {
     const int share = (kGate ? 64 : 128) / sh.splits;
-    const int f = rank * share + static_cast<int>(threadIdx.x) % share;   // feature within the tile
-    const int per = kSkinnyThreads / share;                               // tokens per pass
+    const int quads = share / 4;                                          // threads per token
+    const int f = rank * share + static_cast<int>(threadIdx.x) % quads * 4;   // first of four features in the tile
+    const int per = kSkinnyThreads / quads;                               // tokens per pass
     const uint32_t red_addr = smem_u32(red);
     uint32_t part[8];
 #pragma unroll
     for (int q = 0; q < 8; ++q) part[q] = q < sh.splits ? map_to_cta(red_addr, q) : 0u;
+    const int live = static_cast<int>(p.m - t0 < sh.bn ? p.m - t0 : sh.bn);
     if (n0 + f < p.n) {
-      const int live = static_cast<int>(p.m - t0 < sh.bn ? p.m - t0 : sh.bn);
-      for (int t = static_cast<int>(threadIdx.x) / share; t < live; t += per) {
-        float a[8], b[8];
+#pragma unroll 2
+      for (int t = static_cast<int>(threadIdx.x) / quads; t < live; t += per) {
+        float4 a[8], b[8];
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
           if (q < sh.splits) {
-            a[q] = ld_cluster_f32(part[q] + (t * 128 + f) * 4);
-            if (kGate) b[q] = ld_cluster_f32(part[q] + (t * 128 + 64 + f) * 4);
+            a[q] = ld_cluster_f32x4(part[q] + (t * 128 + f) * 4);
+            if (kGate) b[q] = ld_cluster_f32x4(part[q] + (t * 128 + 64 + f) * 4);
           }
         }
-        float sum = a[0], gate = kGate ? b[0] : 0.0f;
+        float4 sum = a[0], gate = b[0];
 #pragma unroll
         for (int q = 1; q < 8; ++q) {
           if (q < sh.splits) {
-            sum += a[q];
-            if (kGate) gate += b[q];
+            sum.x += a[q].x, sum.y += a[q].y, sum.z += a[q].z, sum.w += a[q].w;
+            if (kGate) gate.x += b[q].x, gate.y += b[q].y, gate.z += b[q].z, gate.w += b[q].w;
           }
         }
         const int64_t row = static_cast<int64_t>(t0) + t;
         if (kGate) {
           if (p.preact != nullptr) {
             float* pre = p.preact + row * (2 * static_cast<int64_t>(p.n)) + n0 + f;
-            pre[0] = sum;
-            pre[p.n] = gate;
+            *reinterpret_cast<float4*>(pre) = sum;
+            *reinterpret_cast<float4*>(pre + p.n) = gate;
           }
-          sum *= act_value(gate, p.act);
+          sum.x *= act_value(gate.x, p.act), sum.y *= act_value(gate.y, p.act);
+          sum.z *= act_value(gate.z, p.act), sum.w *= act_value(gate.w, p.act);
         }
         const int64_t at = row * p.ldo + n0 + f;
-        if (p.out_type == kTypeFp32)
-          static_cast<float*>(p.out)[at] = sum;
-        else
-          static_cast<uint16_t*>(p.out)[at] = round_16(sum, p.out_type);
+        if (p.out_type == kTypeFp32) {
+          float* out = static_cast<float*>(p.out) + at;
+          if (p.vec32) {
+            *reinterpret_cast<float4*>(out) = sum;
+          } else {
+            out[0] = sum.x;
+            if (n0 + f + 1 < p.n) out[1] = sum.y;
+            if (n0 + f + 2 < p.n) out[2] = sum.z;
+            if (n0 + f + 3 < p.n) out[3] = sum.w;
+          }
+        } else {
+          const uint2 v = make_uint2(pack_16(sum.x, sum.y, p.out_type), pack_16(sum.z, sum.w, p.out_type));
+          uint16_t* out = static_cast<uint16_t*>(p.out) + at;
+          if (p.vec32) {
+            *reinterpret_cast<uint2*>(out) = v;
+          } else {
+            out[0] = static_cast<uint16_t>(v.x);
+            if (n0 + f + 1 < p.n) out[1] = static_cast<uint16_t>(v.x >> 16);
+            if (n0 + f + 2 < p.n) out[2] = static_cast<uint16_t>(v.y);
+            if (n0 + f + 3 < p.n) out[3] = static_cast<uint16_t>(v.y >> 16);
+          }
+        }
       }
     }
   }
@@ -268,12 +299,13 @@ template <bool kMx, bool kGate>
 int launch_skinny(const CUtensorMap& w, const CUtensorMap& x, const CUtensorMap& sfw, const CUtensorMap& sfx,
                   const DenseParams& p, SkinnyShape sh, int units, int token_tiles, bool dependent, cudaStream_t s) {
   auto kern = dense_skinny_kernel<kMx, kGate>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSkinnySmem) != cudaSuccess)
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingLarge + kSkinnyExtra) !=
+      cudaSuccess)
     return MOE_B200_ERR_CUDA;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(units * sh.splits), static_cast<unsigned>(token_tiles));
   cfg.blockDim = dim3(kSkinnyThreads);
-  cfg.dynamicSmemBytes = kSkinnySmem;
+  cfg.dynamicSmemBytes = sh.ring_bytes + kSkinnyExtra;
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -296,7 +328,10 @@ SkinnyShape choose_shape(const DenseParams& p, int units, int token_tiles, int b
   while (sh.splits < 8 && 2 * sh.splits * units * token_tiles <= sm_count && 2 * sh.splits <= p.k_iters)
     sh.splits *= 2;
   sh.stage_bytes = kWeightTile + bn * 128 + extra;
-  sh.stages = kRingBytes / sh.stage_bytes;
+  // Up to 64 tokens a ring of 108 KB: the next GEMM of the call fits on the
+  // SM beside this one and streams its first weights under this one's tail.
+  sh.ring_bytes = bn <= 64 ? kRingSmall : kRingLarge;
+  sh.stages = sh.ring_bytes / sh.stage_bytes;
   if (sh.stages > kMaxStages) sh.stages = kMaxStages;
   return sh;
 }
@@ -309,6 +344,7 @@ int launch_dense_skinny(DenseEpi epi, const DenseOperand& a, const DenseOperand&
                         bool dependent, cudaStream_t s) {
   const bool gate = epi == kEpiGated;
   p.k_iters = static_cast<int>(div_up(p.k, 64));
+  p.vec32 = 1;   // four columns at a time: n and ldo are multiples of 8
   const int units = static_cast<int>(div_up(p.n, gate ? 64 : 128));
   const int bn = token_tile(p.m);
   const int token_tiles = static_cast<int>(div_up(p.m, bn));
@@ -324,6 +360,7 @@ int launch_dense_skinny(DenseEpi epi, const DenseOperand& a, const DenseOperand&
 int launch_mx_skinny(const MxOperand& a, const MxOperand& b, DenseParams p, int sm_count, bool dependent,
                      cudaStream_t s) {
   p.k_iters = static_cast<int>(div_up(p.k, 256));
+  p.vec32 = p.n % 4 == 0 && p.ldo % 4 == 0;   // four columns at a time
   const int units = static_cast<int>(div_up(p.n, 128));
   const int bn = token_tile(p.m);
   const int token_tiles = static_cast<int>(div_up(p.m, bn));
