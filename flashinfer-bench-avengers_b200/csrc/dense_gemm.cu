@@ -47,24 +47,24 @@ namespace {
 
 constexpr int kTileBytes = 16384;   // 128 rows (or 128 MN elements x 64 K) of 128 bytes
 
+constexpr int kMaxStages = 12;
+constexpr int kRingBytes = 224 * 1024;
+constexpr int kNumBars = 2 * kMaxStages + 4;
+constexpr int kPairSmem = kRingBytes + kNumBars * 8 + 16 + 1024;
+static_assert(kPairSmem <= 227 * 1024, "shared memory");
+
 template <bool kMx>
 struct PairTraits {
-  static constexpr int kStages = 6;
   static constexpr int kScaleBytes = kMx ? 3072 : 0;   // A: 2 K tiles, B: 2 row tiles x 2 K tiles of 512 bytes
-  static constexpr int kStageBytes = 2 * kTileBytes + kScaleBytes;
   // Tensor memory: two accumulators of up to 256 columns. With 4-bit
   // operands 48 columns hold the staged exponents (2 x 24), and the
   // accumulators overlap in 48 columns, which the epilogue drains first.
   static constexpr int kAcc1 = kMx ? 208 : 256;
   static constexpr int kScaleCol = 464;
-  static constexpr int kOffBars = kStages * kStageBytes;
-  static constexpr int kNumBars = 2 * kStages + 4;
-  static constexpr int kSmemBytes = kOffBars + kNumBars * 8 + 16 + 1024;
-  static_assert(kSmemBytes <= 227 * 1024, "shared memory");
 };
 
-constexpr int kPairThreads = 256;
-constexpr int kEpiWarps = 4;
+constexpr int kEpiWarps = 8;
+constexpr int kPairThreads = (4 + kEpiWarps) * 32;
 
 struct Tile {
   int m0, n0;   // first output row of the pair, first output column
@@ -105,16 +105,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                       const DenseParams p) {
   using Tr = PairTraits<kMx>;
   constexpr bool kGate = kEpi == kEpiGated || kEpi == kEpiGatedQuant;
-  constexpr int kS = Tr::kStages;
+  const int kS = p.stages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Tr::kOffBars);
-  uint64_t* full_bar = bars;             // first CTA: both CTAs' copies of a stage have landed
-  uint64_t* empty_bar = bars + kS;       // the stage's MMAs are done
-  uint64_t* accf_bar = bars + 2 * kS;    // accumulator complete
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kRingBytes);
+  uint64_t* full_bar = bars;                 // first CTA: both CTAs' copies of a stage have landed
+  uint64_t* empty_bar = bars + kMaxStages;   // the stage's MMAs are done
+  uint64_t* accf_bar = bars + 2 * kMaxStages;   // accumulator complete
   uint64_t* acce_bar = accf_bar + 2;     // first CTA: both CTAs' epilogues are through with an accumulator
-  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bars + Tr::kNumBars);
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bars + kNumBars);
   volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
 
   const int warp = threadIdx.x >> 5;
@@ -149,65 +149,89 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   cluster_sync();
   tc_fence_after();
   const uint32_t tmem = *s_tmem;
-  // Everything above overlaps the previous kernel's tail.
-  pdl_wait();
+  // Everything above overlaps the previous kernel's tail. (The producer waits
+  // for that kernel below; no bounded wait of the others starts before.)
+  if (warp != 0) pdl_wait();
 
   if (warp == 0) {
     // ---------------------------------------------------------- producer
-    if (lane == 0) {
-      const int b_rows = p.bn >> 1;                          // B rows this CTA stages
-      const int b_atoms = kBMn ? (b_rows + 63) >> 6 : 0;
-      const uint32_t bytes =
-          kTileBytes + (kBMn ? static_cast<uint32_t>(b_atoms) * 8192u : static_cast<uint32_t>(b_rows) * 128u) +
-          Tr::kScaleBytes;
-      int stage = 0;
-      uint32_t ph = 0;
-      bool ok = true;
-      for (int t = pair; ok && t < tiles; t += pairs) {
-        const Tile tl = tile_at(t, p);
-        const int am = tl.m0 + static_cast<int>(rank) * 128;
-        const int bnr = tl.n0 + static_cast<int>(rank) * p.b_half;
-        for (int kb = 0; kb < p.k_iters; ++kb) {
-          if (!mbar_wait(smem_u32(&empty_bar[stage]), ph ^ 1u, s_abort, p.status, kStatusTimeoutProducer)) {
-            ok = false;
-            break;
-          }
-          const uint32_t bar = map_to_cta(smem_u32(&full_bar[stage]), 0);
-          if (rank == 0) mbar_arrive_expect_tx(smem_u32(&full_bar[stage]), 2u * bytes);
-          const uint32_t sa = smem_u32(smem + stage * Tr::kStageBytes);
-          const uint32_t sb = sa + kTileBytes;
-          if constexpr (kMx) {
-            tma_load_2d_pair(sa, &tm_a, bar, kb * 128, am);
-            tma_load_2d_pair(sb, &tm_b, bar, kb * 128, bnr);
-            const int kt = (p.k + 127) >> 7;                 // exponent tiles along K
-            const uint32_t sc = sb + kTileBytes;
-            tma_load_2d_pair(sc, &tm_sfa, bar, 0, (am >> 7) * kt + 2 * kb);
-            tma_load_2d_pair(sc + 1024, &tm_sfb, bar, 0, (tl.n0 >> 7) * kt + 2 * kb);
-            tma_load_2d_pair(sc + 2048, &tm_sfb, bar, 0, ((tl.n0 + p.b_half) >> 7) * kt + 2 * kb);
-          } else {
-            if constexpr (kAMn) {
-              tma_load_2d_pair(sa, &tm_a, bar, am, kb * 64);
-              tma_load_2d_pair(sa + 8192, &tm_a, bar, am + 64, kb * 64);
-            } else {
-              tma_load_2d_pair(sa, &tm_a, bar, kb * 64, am);
-            }
-            if constexpr (kBMn) {
-              for (int j = 0; j < b_atoms; ++j) tma_load_2d_pair(sb + j * 8192, &tm_b, bar, bnr + 64 * j, kb * 64);
-            } else {
-              tma_load_2d_pair(sb, &tm_b, bar, kb * 64, bnr);
-            }
-          }
-          if (++stage == kS) {
-            stage = 0;
-            ph ^= 1u;
-          }
+    const bool issue = elect_lane();
+    const int b_rows = p.bn >> 1;                          // B rows this CTA stages
+    const int b_atoms = kBMn ? (b_rows + 63) >> 6 : 0;
+    const uint32_t bytes =
+        kTileBytes + (kBMn ? static_cast<uint32_t>(b_atoms) * 8192u : static_cast<uint32_t>(b_rows) * 128u) +
+        Tr::kScaleBytes;
+    const int kt = kMx ? (p.k + 127) >> 7 : 0;             // exponent tiles along K
+    const uint32_t base = smem_u32(smem);
+    const uint32_t full0 = smem_u32(full_bar);
+    const uint32_t full0_pair = map_to_cta(full0, 0);
+    auto load_b = [&](int n0, int kb, int stage) {
+      const uint32_t bar = full0_pair + 8u * stage;
+      const uint32_t sb = base + stage * p.stage_bytes + kTileBytes;
+      const int bnr = n0 + static_cast<int>(rank) * p.b_half;
+      if (rank == 0) mbar_arrive_expect_tx(full0 + 8u * stage, 2u * bytes);
+      if constexpr (kMx) {
+        tma_load_2d_pair(sb, &tm_b, bar, kb * 128, bnr);
+        tma_load_2d_pair(sb + kTileBytes + 1024, &tm_sfb, bar, 0, (n0 >> 7) * kt + 2 * kb);
+        tma_load_2d_pair(sb + kTileBytes + 2048, &tm_sfb, bar, 0, ((n0 + p.b_half) >> 7) * kt + 2 * kb);
+      } else if constexpr (kBMn) {
+        tma_load_2d_pair(sb, &tm_b, bar, bnr, kb * 64);
+        if (b_atoms > 1) tma_load_2d_pair(sb + 8192, &tm_b, bar, bnr + 64, kb * 64);
+      } else {
+        tma_load_2d_pair(sb, &tm_b, bar, kb * 64, bnr);
+      }
+    };
+    auto load_a = [&](int m0, int kb, int stage) {
+      const uint32_t bar = full0_pair + 8u * stage;
+      const uint32_t sa = base + stage * p.stage_bytes;
+      const int am = m0 + static_cast<int>(rank) * 128;
+      if constexpr (kMx) {
+        tma_load_2d_pair(sa, &tm_a, bar, kb * 128, am);
+        tma_load_2d_pair(sa + 2 * kTileBytes, &tm_sfa, bar, 0, (am >> 7) * kt + 2 * kb);
+      } else if constexpr (kAMn) {
+        tma_load_2d_pair(sa, &tm_a, bar, am, kb * 64);
+        tma_load_2d_pair(sa + 8192, &tm_a, bar, am + 64, kb * 64);
+      } else {
+        tma_load_2d_pair(sa, &tm_a, bar, kb * 64, am);
+      }
+    };
+    // B is an input of the whole call (weights, or saved by another call):
+    // its part of the first ring does not wait for the predecessor.
+    const int early = min(kS, p.k_iters);
+    if (issue) {
+      const int n0 = tile_at(pair, p).n0;
+      for (int kb = 0; kb < early; ++kb) load_b(n0, kb, kb);
+    }
+    __syncwarp();
+    pdl_wait();
+    int stage = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    for (int t = pair; ok && t < tiles; t += pairs) {
+      const Tile tl = tile_at(t, p);
+      const int skip = t == pair ? early : 0;   // K steps whose B is on its way already
+      for (int kb = 0; kb < p.k_iters; ++kb) {
+        if (kb >= skip && !warp_wait(smem_u32(empty_bar) + 8u * stage, ph ^ 1u, s_abort, p.status,
+                                     kStatusTimeoutProducer)) {
+          ok = false;
+          break;
+        }
+        if (issue) {
+          if (kb >= skip) load_b(tl.n0, kb, stage);
+          load_a(tl.m0, kb, stage);
+        }
+        __syncwarp();
+        if (++stage == kS) {
+          stage = 0;
+          ph ^= 1u;
         }
       }
-      if (!ok) drain_copies();
     }
+    if (!ok) drain_copies();
   } else if (warp == 1) {
     // --------------------------------------------------------------- MMA
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
+      const bool issue = elect_lane();
       int stage = 0;
       uint32_t ph = 0;
       bool ok = true;
@@ -226,20 +250,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         if (kMx ? it >= 1 : it >= 2) {
           const uint32_t bar = smem_u32(&acce_bar[kMx ? 0 : buf]);
           const uint32_t par = kMx ? static_cast<uint32_t>(it - 1) & 1u : (static_cast<uint32_t>(it >> 1) - 1u) & 1u;
-          if (!mbar_wait_cluster(bar, par, s_abort, p.status, kStatusTimeoutMma)) break;
+          if (!__all_sync(0xffffffffu, mbar_wait_cluster(bar, par, s_abort, p.status, kStatusTimeoutMma))) break;
           tc_fence_after();
         }
         for (int kb = 0; kb < p.k_iters; ++kb) {
-          if (!mbar_wait(smem_u32(&full_bar[stage]), ph, s_abort, p.status, kStatusTimeoutMma)) {
+          if (!warp_wait(smem_u32(full_bar) + 8u * stage, ph, s_abort, p.status, kStatusTimeoutMma)) {
             ok = false;
             break;
           }
-          const uint32_t off = static_cast<uint32_t>(stage) * (Tr::kStageBytes >> 4);
+          const uint32_t off = static_cast<uint32_t>(stage * (p.stage_bytes >> 4));
           const uint32_t lo_a = lo_a0 + off, lo_b = lo_b0 + off;
           if constexpr (kMx) {
             // The exponent columns written now were last read two stages ago
             // (the first two waits pass at once).
-            if (!mbar_wait(smem_u32(&empty_bar[old]), old_ph, s_abort, p.status, kStatusTimeoutMma)) {
+            if (!warp_wait(smem_u32(empty_bar) + 8u * old, old_ph, s_abort, p.status, kStatusTimeoutMma)) {
               ok = false;
               break;
             }
@@ -247,42 +271,47 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
               old = 0;
               old_ph ^= 1u;
             }
-            tc_fence_after();
-            const uint32_t lo_s = lo_s0 + off;
-            const uint32_t sfa = tmem + Tr::kScaleCol + sf;
-            const uint32_t sfb = sfa + 8;
-            sf ^= 24u;
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              tmem_copy_scales<2>(sfa + 4 * j, desc_of(kDescHiPlain, lo_s + 32 * j));
-              tmem_copy_scales<2>(sfb + 8 * j, desc_of(kDescHiPlain, lo_s + 64 + 32 * j));
-              tmem_copy_scales<2>(sfb + 8 * j + 4, desc_of(kDescHiPlain, lo_s + 128 + 32 * j));
-            }
-            const int left = p.k - kb * 256;
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              if (k == 0 || left > 64 * k)
-                umma_mxf4<2>(d, desc_of(kDescHiSw128, lo_a + 2 * k), desc_of(kDescHiSw128, lo_b + 2 * k),
-                             k & 1 ? idesc1 : idesc0, sfa + 4 * (k >> 1), sfb + 8 * (k >> 1), kb | k);
-          } else {
-            tc_fence_after();
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              umma_f16<2>(d, desc_of(kDescHiSw128, lo_a + (kAMn ? 128 : 2) * k),
-                          desc_of(kDescHiSw128, lo_b + (kBMn ? 128 : 2) * k), idesc0, kb | k);
           }
-          umma_commit_pair(smem_u32(&empty_bar[stage]));
+          tc_fence_after();
+          if (issue) {
+            if constexpr (kMx) {
+              const uint32_t lo_s = lo_s0 + off;
+              const uint32_t sfa = tmem + Tr::kScaleCol + sf;
+              const uint32_t sfb = sfa + 8;
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                tmem_copy_scales<2>(sfa + 4 * j, desc_of(kDescHiPlain, lo_s + 32 * j));
+                tmem_copy_scales<2>(sfb + 8 * j, desc_of(kDescHiPlain, lo_s + 64 + 32 * j));
+                tmem_copy_scales<2>(sfb + 8 * j + 4, desc_of(kDescHiPlain, lo_s + 128 + 32 * j));
+              }
+              const int left = p.k - kb * 256;
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                if (k == 0 || left > 64 * k)
+                  umma_mxf4<2>(d, desc_of(kDescHiSw128, lo_a + 2 * k), desc_of(kDescHiSw128, lo_b + 2 * k),
+                               k & 1 ? idesc1 : idesc0, sfa + 4 * (k >> 1), sfb + 8 * (k >> 1), kb | k);
+            } else {
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                umma_f16<2>(d, desc_of(kDescHiSw128, lo_a + (kAMn ? 128 : 2) * k),
+                            desc_of(kDescHiSw128, lo_b + (kBMn ? 128 : 2) * k), idesc0, kb | k);
+            }
+            umma_commit_pair(smem_u32(empty_bar) + 8u * stage);
+            if (kb == p.k_iters - 1) umma_commit_pair(smem_u32(&accf_bar[buf]));
+          }
+          __syncwarp();
+          sf ^= 24u;
           if (++stage == kS) {
             stage = 0;
             ph ^= 1u;
           }
         }
-        if (ok) umma_commit_pair(smem_u32(&accf_bar[buf]));
       }
     }
   } else if (warp >= 4) {
     // ---------------------------------------------------------- epilogue
     const int quarter = warp & 3;
+    const int half = (warp - 4) >> 2;   // two warps per quarter, taking turns at 32-column chunks
     const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
     const int width = kGate ? p.n_step : p.bn;   // output columns of a tile
     const int chunks = (width + 31) >> 5;
@@ -299,8 +328,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       const int64_t row = static_cast<int64_t>(tl.m0) + rank * 128 + quarter * 32 + lane;
       const bool live = row < p.m;
       const int end = min(p.n, tl.n0 + width);   // first column past this tile
-      uint32_t scale_word = 0;
-      for (int i = 0; i < chunks; ++i) {
+      for (int i = half; i < chunks; i += 2) {
         // 4-bit operands: the columns shared with the other accumulator first
         const int c = 32 * (kMx && buf == 0 ? chunks - 1 - i : i);
         uint32_t r[32];
@@ -310,7 +338,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           tmem_ld32(acc + c, r);
           tmem_ld32(acc + p.n_step + c, g);
           tmem_wait_ld();
-          if (kMx && i == (chunks > 1 ? 1 : 0)) {
+          if (kMx && i == half) {
             tc_fence_before();
             if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&acce_bar[0]), 0));
             __syncwarp();
@@ -348,13 +376,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                 v = make_uint4(mx_pack8(h, inv), mx_pack8(h + 8, inv), mx_pack8(h + 16, inv), mx_pack8(h + 24, inv));
               }
               *reinterpret_cast<uint4*>(p.q + (row * p.n + tl.n0 + c) / 2) = v;
-              scale_word |= byte << ((c >> 5) * 8);
+              p.q_scale[mx_scale_offset(row, (tl.n0 + c) >> 5, (p.n + 127) >> 7)] = static_cast<uint8_t>(byte);
             }
           }
         } else {
           tmem_ld32(acc + c, r);
           tmem_wait_ld();
-          if (kMx && i == (chunks > 1 ? 1 : 0)) {
+          if (kMx && i == half) {
             tc_fence_before();
             if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&acce_bar[0]), 0));
             __syncwarp();
@@ -421,10 +449,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           }
         }
       }
-      if constexpr (kEpi == kEpiGatedQuant) {
-        if (live)
-          *reinterpret_cast<uint32_t*>(p.q_scale + mx_scale_offset(row, tl.n0 >> 5, (p.n + 127) >> 7)) = scale_word;
-      }
       if (!kMx) {
         tc_fence_before();
         __syncwarp();
@@ -437,7 +461,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   __syncwarp();
   tc_fence_before();
   __syncthreads();
-  cluster_sync();
+  cluster_sync_relaxed();
   tc_fence_after();
   if (warp == 2) tmem_dealloc_pair(tmem, 512);
 }
@@ -448,7 +472,7 @@ template <bool kMx, bool kAMn, bool kBMn, int kEpi>
 int launch_pair(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& sfa, const CUtensorMap& sfb,
                 const DenseParams& p, int sm_count, bool dependent, cudaStream_t s) {
   auto kern = dense_pair_kernel<kMx, kAMn, kBMn, kEpi>;
-  constexpr int smem = PairTraits<kMx>::kSmemBytes;
+  constexpr int smem = kPairSmem;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return MOE_B200_ERR_CUDA;
   const int64_t tiles = static_cast<int64_t>(p.m_tiles) * p.n_tiles;
@@ -456,6 +480,13 @@ int launch_pair(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& s
   return launch_kernel(kern, 2 * pairs, kPairThreads, smem, s, dependent, a, b, sfa, sfb, p) == cudaSuccess
              ? MOE_B200_OK
              : MOE_B200_ERR_CUDA;
+}
+
+// As many stages as the ring holds: a K step's loads take about 1.8 us to
+// come back, so with six stages a step takes 300 ns however narrow the tile.
+void set_ring(DenseParams* p, int stage_bytes) {
+  p->stage_bytes = stage_bytes;
+  p->stages = kRingBytes / stage_bytes < kMaxStages ? kRingBytes / stage_bytes : kMaxStages;
 }
 
 // Columns per tile (the MMA's N, 64 to 256): the fewest time units over all
@@ -494,6 +525,7 @@ int launch_dense_pair(DenseEpi epi, const DenseOperand& a, bool a_mn, const Dens
   p.m_tiles = static_cast<int>(div_up(p.m, 256));
   p.n_tiles = static_cast<int>(div_up(p.n, p.n_step));
   p.k_iters = static_cast<int>(div_up(p.k, 64));
+  set_ring(&p, kTileBytes + (b_mn ? static_cast<int>(div_up(p.bn / 2, 64)) * 8192 : p.bn / 2 * 128));
   const int64_t dact_half = epi == kEpiDact ? static_cast<int64_t>(p.n) * 2 : 0;
   p.vec32 = aligned(p.out, 32) && (p.ldo * 2) % 32 == 0 && dact_half % 32 == 0;
   CUtensorMap ta, tb;
@@ -522,6 +554,7 @@ int launch_mx_pair(DenseEpi epi, const MxOperand& a, const MxOperand& b, DensePa
   p.m_tiles = static_cast<int>(div_up(p.m, 256));
   p.n_tiles = static_cast<int>(div_up(p.n, p.n_step));
   p.k_iters = static_cast<int>(div_up(p.k, 256));
+  set_ring(&p, 2 * kTileBytes + PairTraits<true>::kScaleBytes);
   const int esz = p.out_type == kTypeFp32 ? 4 : 2;
   p.vec32 = aligned(p.out, 32) && (p.ldo * esz) % 32 == 0 && p.n % 8 == 0;
   const int64_t kt = div_up(p.k, 128);

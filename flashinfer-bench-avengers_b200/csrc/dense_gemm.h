@@ -40,7 +40,7 @@ struct DenseParams {
   uint8_t* q_scale;    //   and tiled exponents
   uint32_t* status;    // sticky device status word
   // derived by the launcher
-  int bn, n_step, b_half, m_tiles, n_tiles, k_iters, vec32;
+  int bn, n_step, b_half, m_tiles, n_tiles, k_iters, vec32, stages, stage_bytes;
 };
 
 struct MxOperand {
@@ -49,6 +49,9 @@ struct MxOperand {
   int64_t rows;
 };
 
+// B of every GEMM must be complete before the call's first kernel starts: it
+// is read before the previous kernel has finished. A may be its result.
+//
 // D = A B^T over CTA pairs; a_mn / b_mn: the operand is stored K x M (K x N).
 // kEpiGated: B has 2 n rows, up then gate. Returns a MOE_B200 status code.
 int launch_dense_pair(DenseEpi epi, const DenseOperand& a, bool a_mn, const DenseOperand& b, bool b_mn, DenseParams p,

@@ -22,6 +22,12 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+// Only keeps the CTAs together (before one leaves that others may still
+// reach): orders no memory, so it does not wait for the CTA's stores.
+__device__ __forceinline__ void cluster_sync_relaxed() {
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+
 // The address, in the cluster's shared window, of `addr` in CTA `rank`.
 __device__ __forceinline__ uint32_t map_to_cta(uint32_t addr, uint32_t rank) {
   uint32_t r;
@@ -67,6 +73,27 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity,
       }
     }
   }
+}
+
+// One lane of a converged warp, the same one every time.
+__device__ __forceinline__ bool elect_lane() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r != 0;
+}
+
+// mbar_wait by a whole warp, with one answer for all lanes. The producer and
+// MMA warps run their loops with all lanes and let one lane issue, so loop
+// counters, addresses and descriptors stay in uniform registers, from which
+// the instructions take them: with one lane in the loop an iteration cost
+// 540 cycles of issue whatever the tile.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort, uint32_t* status,
+                                          uint32_t why) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, status, why));
 }
 
 // After a wait that gave up: let this thread's own copies land before the

@@ -103,80 +103,85 @@ __global__ void __launch_bounds__(kSkinnyThreads, 1)
   if (warp != 0) pdl_wait();   // no bounded wait starts before the predecessor is done
 
   if (warp == 0) {
-    if (lane == 0) {
-      const uint32_t bytes = kWeightTile + sh.bn * 128 + (kMx ? 2048 : 0);
-      const int kt = kMx ? (p.k + 127) >> 7 : 0;
-      // Stage i of this CTA: weights (and their exponents), and tokens.
-      auto load_w = [&](int i, int stage) {
-        const uint32_t bar = smem_u32(&full_bar[stage]);
-        const uint32_t sw = smem_u32(smem + stage * sh.stage_bytes);
-        const int x = (kb0 + i) * (kMx ? 128 : 64);
-        mbar_arrive_expect_tx(bar, bytes);
-        tma_load_2d(sw, &tm_w, bar, x, n0);
-        tma_load_2d(sw + kWeightTile / 2, &tm_w, bar, x, n0 + (kGate ? p.n : 64));
-        if (kMx) tma_load_2d(sw + kWeightTile + sh.bn * 128, &tm_sfw, bar, 0, (n0 >> 7) * kt + 2 * (kb0 + i));
-      };
-      auto load_x = [&](int i, int stage) {
-        const uint32_t bar = smem_u32(&full_bar[stage]);
-        const uint32_t sx = smem_u32(smem + stage * sh.stage_bytes) + kWeightTile;
-        tma_load_2d(sx, &tm_x, bar, (kb0 + i) * (kMx ? 128 : 64), t0);
-        if (kMx) tma_load_2d(sx + sh.bn * 128 + 1024, &tm_sfx, bar, 0, (t0 >> 7) * kt + 2 * (kb0 + i));
-      };
-      const int first = min(sh.stages, iters);
+    const bool issue = elect_lane();
+    const uint32_t bytes = kWeightTile + sh.bn * 128 + (kMx ? 2048 : 0);
+    const int kt = kMx ? (p.k + 127) >> 7 : 0;
+    const uint32_t base = smem_u32(smem);
+    const uint32_t full0 = smem_u32(full_bar);
+    // Stage i of this CTA: weights (and their exponents), and tokens.
+    auto load_w = [&](int i, int stage) {
+      const uint32_t bar = full0 + 8u * stage;
+      const uint32_t sw = base + stage * sh.stage_bytes;
+      const int x = (kb0 + i) * (kMx ? 128 : 64);
+      mbar_arrive_expect_tx(bar, bytes);
+      tma_load_2d(sw, &tm_w, bar, x, n0);
+      tma_load_2d(sw + kWeightTile / 2, &tm_w, bar, x, n0 + (kGate ? p.n : 64));
+      if (kMx) tma_load_2d(sw + kWeightTile + sh.bn * 128, &tm_sfw, bar, 0, (n0 >> 7) * kt + 2 * (kb0 + i));
+    };
+    auto load_x = [&](int i, int stage) {
+      const uint32_t bar = full0 + 8u * stage;
+      const uint32_t sx = base + stage * sh.stage_bytes + kWeightTile;
+      tma_load_2d(sx, &tm_x, bar, (kb0 + i) * (kMx ? 128 : 64), t0);
+      if (kMx) tma_load_2d(sx + sh.bn * 128 + 1024, &tm_sfx, bar, 0, (t0 >> 7) * kt + 2 * (kb0 + i));
+    };
+    const int first = min(sh.stages, iters);
+    // The next kernel of the call may start once this CTA requests its last
+    // ring (25.5 us for the block at one token; 26.3 released at the start).
+    const int release = max(iters - sh.stages, 0);
+    if (issue)
       for (int i = 0; i < first; ++i) load_w(i, i);
-      // The next kernel of the call may start once this CTA requests its last
-      // ring (25.5 us for the block at one token; 26.3 released at the start).
-      const int release = max(iters - sh.stages, 0);
-      if (release < first) pdl_launch_next();
-      pdl_wait();
+    if (release < first) pdl_launch_next();
+    __syncwarp();
+    pdl_wait();
+    if (issue)
       for (int i = 0; i < first; ++i) load_x(i, i);
-      for (int i = first; i < iters; ++i) {
-        const int stage = i % sh.stages;
-        if (!mbar_wait(smem_u32(&empty_bar[stage]), static_cast<uint32_t>(i / sh.stages - 1) & 1u, s_abort, p.status,
-                       kStatusTimeoutProducer)) {
-          drain_copies();
-          break;
-        }
+    __syncwarp();
+    int stage = first == sh.stages ? 0 : first;
+    uint32_t ph = 0;
+    for (int i = first; i < iters; ++i) {
+      if (!warp_wait(smem_u32(empty_bar) + 8u * stage, ph, s_abort, p.status, kStatusTimeoutProducer)) {
+        drain_copies();
+        break;
+      }
+      if (issue) {
         load_w(i, stage);
         load_x(i, stage);
-        if (i == release) pdl_launch_next();
+      }
+      if (i == release) pdl_launch_next();
+      __syncwarp();
+      if (++stage == sh.stages) {
+        stage = 0;
+        ph ^= 1u;
       }
     }
-    __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0) {
-      const uint32_t idesc0 =
-          kMx ? idesc_mxf4(128, sh.bn, 0) : idesc_f16(128, sh.bn, p.type == kTypeFp16, false, false);
-      const uint32_t idesc1 = kMx ? idesc_mxf4(128, sh.bn, 2) : idesc0;
-      const uint32_t lo_w0 = desc_lo_kmajor(smem_u32(smem));
-      const uint32_t lo_x0 = lo_w0 + (kWeightTile >> 4);
-      const uint32_t lo_s0 = desc_lo_scale(smem_u32(smem) + kWeightTile + sh.bn * 128);
-      bool ok = true;
-      int stage = 0, old = sh.stages - 2;   // 4-bit: the stage before last, and its phase
-      uint32_t ph = 0, old_ph = 1, sf = 0;
-      for (int i = 0; i < iters; ++i) {
-        if (!mbar_wait(smem_u32(&full_bar[stage]), ph, s_abort, p.status, kStatusTimeoutMma)) {
-          ok = false;
-          break;
+    const bool issue = elect_lane();
+    const uint32_t idesc0 = kMx ? idesc_mxf4(128, sh.bn, 0) : idesc_f16(128, sh.bn, p.type == kTypeFp16, false, false);
+    const uint32_t idesc1 = kMx ? idesc_mxf4(128, sh.bn, 2) : idesc0;
+    const uint32_t lo_w0 = desc_lo_kmajor(smem_u32(smem));
+    const uint32_t lo_x0 = lo_w0 + (kWeightTile >> 4);
+    const uint32_t lo_s0 = desc_lo_scale(smem_u32(smem) + kWeightTile + sh.bn * 128);
+    int stage = 0, old = sh.stages - 2;   // 4-bit: the stage before last, and its phase
+    uint32_t ph = 0, old_ph = 1, sf = 0;
+    for (int i = 0; i < iters; ++i) {
+      if (!warp_wait(smem_u32(full_bar) + 8u * stage, ph, s_abort, p.status, kStatusTimeoutMma)) break;
+      const uint32_t off = static_cast<uint32_t>(stage * (sh.stage_bytes >> 4));
+      const uint32_t lo_w = lo_w0 + off, lo_x = lo_x0 + off;
+      if constexpr (kMx) {
+        // these exponent columns were last read two stages ago (the first
+        // two waits pass at once)
+        if (!warp_wait(smem_u32(empty_bar) + 8u * old, old_ph, s_abort, p.status, kStatusTimeoutMma)) break;
+        if (++old == sh.stages) {
+          old = 0;
+          old_ph ^= 1u;
         }
-        const uint32_t off = static_cast<uint32_t>(stage * (sh.stage_bytes >> 4));
-        const uint32_t lo_w = lo_w0 + off, lo_x = lo_x0 + off;
+      }
+      tc_fence_after();
+      if (issue) {
         if constexpr (kMx) {
-          // these exponent columns were last read two stages ago (the first
-          // two waits pass at once)
-          if (!mbar_wait(smem_u32(&empty_bar[old]), old_ph, s_abort, p.status, kStatusTimeoutMma)) {
-            ok = false;
-            break;
-          }
-          if (++old == sh.stages) {
-            old = 0;
-            old_ph ^= 1u;
-          }
-          tc_fence_after();
           const uint32_t lo_s = lo_s0 + off;
           const uint32_t sfw = tmem + 128 + sf;
           const uint32_t sfx = sfw + 8;
-          sf ^= 16u;
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             tmem_copy_scales<1>(sfw + 4 * j, desc_of(kDescHiPlain, lo_s + 32 * j));
@@ -189,20 +194,20 @@ __global__ void __launch_bounds__(kSkinnyThreads, 1)
               umma_mxf4<1>(tmem, desc_of(kDescHiSw128, lo_w + 2 * k), desc_of(kDescHiSw128, lo_x + 2 * k),
                            k & 1 ? idesc1 : idesc0, sfw + 4 * (k >> 1), sfx + 4 * (k >> 1), i | k);
         } else {
-          tc_fence_after();
 #pragma unroll
           for (int k = 0; k < 4; ++k)
             umma_f16<1>(tmem, desc_of(kDescHiSw128, lo_w + 2 * k), desc_of(kDescHiSw128, lo_x + 2 * k), idesc0, i | k);
         }
-        umma_commit(smem_u32(&empty_bar[stage]));
-        if (++stage == sh.stages) {
-          stage = 0;
-          ph ^= 1u;
-        }
+        umma_commit(smem_u32(empty_bar) + 8u * stage);
+        if (i == iters - 1) umma_commit(smem_u32(done_bar));
       }
-      if (ok) umma_commit(smem_u32(done_bar));
+      __syncwarp();
+      sf ^= 16u;
+      if (++stage == sh.stages) {
+        stage = 0;
+        ph ^= 1u;
+      }
     }
-    __syncwarp();
   }
 
   // ------------------------------------- partial sums into shared memory
@@ -288,7 +293,7 @@ __global__ void __launch_bounds__(kSkinnyThreads, 1)
     }
   }
   tc_fence_before();
-  cluster_sync();   // the others have read this CTA's part
+  cluster_sync_relaxed();   // the others have read this CTA's part
   tc_fence_after();
   if (warp == 2) tmem_dealloc(tmem, kCols);
 }
