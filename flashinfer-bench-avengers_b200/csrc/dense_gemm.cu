@@ -24,6 +24,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 #include <cstring>
 
@@ -39,8 +40,17 @@ namespace moe {
 __device__ uint32_t g_dense_status;
 
 uint32_t* dense_status_word() {
-  void* p = nullptr;
-  return cudaGetSymbolAddress(&p, g_dense_status) == cudaSuccess ? static_cast<uint32_t*>(p) : nullptr;
+  static std::atomic<uint32_t*> words[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
+  uint32_t* word = words[dev].load(std::memory_order_acquire);
+  if (word == nullptr) {
+    void* p = nullptr;
+    if (cudaGetSymbolAddress(&p, g_dense_status) != cudaSuccess) return nullptr;
+    word = static_cast<uint32_t*>(p);
+    words[dev].store(word, std::memory_order_release);
+  }
+  return word;
 }
 
 namespace {
@@ -473,7 +483,10 @@ int launch_pair(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& s
                 const DenseParams& p, int sm_count, bool dependent, cudaStream_t s) {
   auto kern = dense_pair_kernel<kMx, kAMn, kBMn, kEpi>;
   constexpr int smem = kPairSmem;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+  static OncePerDevice ready;
+  if (!ready([&] {
+        return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) == cudaSuccess;
+      }))
     return MOE_B200_ERR_CUDA;
   const int64_t tiles = static_cast<int64_t>(p.m_tiles) * p.n_tiles;
   const int pairs = static_cast<int>(tiles < sm_count / 2 ? tiles : sm_count / 2);

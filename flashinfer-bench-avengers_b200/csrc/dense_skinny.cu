@@ -304,8 +304,11 @@ template <bool kMx, bool kGate>
 int launch_skinny(const CUtensorMap& w, const CUtensorMap& x, const CUtensorMap& sfw, const CUtensorMap& sfx,
                   const DenseParams& p, SkinnyShape sh, int units, int token_tiles, bool dependent, cudaStream_t s) {
   auto kern = dense_skinny_kernel<kMx, kGate>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingLarge + kSkinnyExtra) !=
-      cudaSuccess)
+  static OncePerDevice ready;
+  if (!ready([&] {
+        return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingLarge + kSkinnyExtra) ==
+               cudaSuccess;
+      }))
     return MOE_B200_ERR_CUDA;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(units * sh.splits), static_cast<unsigned>(token_tiles));

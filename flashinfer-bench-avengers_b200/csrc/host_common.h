@@ -5,6 +5,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstddef>
 #include <cstdint>
 
@@ -25,6 +26,25 @@ int current_device_info(DeviceInfo* out);
 // `swizzle` false. Elements outside the matrix read as zero.
 bool encode_2d(CUtensorMap* m, const void* base, int elem_bytes, uint64_t inner, uint64_t rows, uint64_t pitch,
                uint32_t box_inner, uint32_t box_rows, bool swizzle = true);
+
+// Devices a per-device setting has been made on (a kernel's shared-memory
+// limit): made once, remembered per device.
+class OncePerDevice {
+ public:
+  template <typename F>
+  bool operator()(F&& set) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
+    const uint64_t bit = uint64_t(1) << dev;
+    if (done_.load(std::memory_order_acquire) & bit) return true;
+    if (!set()) return false;
+    done_.fetch_or(bit, std::memory_order_release);
+    return true;
+  }
+
+ private:
+  std::atomic<uint64_t> done_{0};
+};
 
 inline bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 

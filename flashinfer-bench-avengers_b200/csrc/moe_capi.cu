@@ -202,6 +202,15 @@ bool encode_2d(CUtensorMap* m, const void* base, int elem_bytes, uint64_t inner,
                uint32_t box_inner, uint32_t box_rows, bool swizzle) {
   EncodeTiledFn fn = get_encode_fn();
   if (fn == nullptr) return false;
+  // The driver call needs a context on this thread. Reading the current
+  // device does not make one current on a thread new to CUDA (autograd's
+  // backward threads are); setting it does.
+  thread_local bool context = false;
+  if (!context) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) return false;
+    context = true;
+  }
   const cuuint64_t dims[2] = {inner, rows};
   const cuuint64_t strides[1] = {pitch};
   const cuuint32_t box[2] = {box_inner, box_rows};

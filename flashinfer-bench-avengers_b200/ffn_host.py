@@ -65,6 +65,10 @@ def _library() -> ctypes.CDLL:
 
 
 # ------------------------------------------------------------------ checks
+# Every entry point first tests all its conditions in one expression, a
+# microsecond or two; only where one fails does it go through them one by one
+# for the message. (Building the messages on every call cost more than the
+# launches: 33 us a call of the block at one token, now 17.)
 def _check_cuda(name: str, t, dev=None) -> None:
     _check(isinstance(t, torch.Tensor), f"{name} must be a torch.Tensor")
     _check(t.is_cuda, f"{name} must be CUDA")
@@ -78,17 +82,42 @@ def _check_dim(name: str, d: int, multiple: int) -> None:
 
 def _check_rows(name: str, t: torch.Tensor, cols: int | None = None) -> int:
     """Rows that may lie apart, each contiguous; returns their pitch in elements."""
+    pitch = _pitch(t)
+    if pitch >= 0 and (cols is None or t.size(1) == cols):
+        return pitch
     _check(t.dim() == 2 and (cols is None or t.size(1) == cols),
            f"{name} must be [T, {cols if cols is not None else 'K'}]")
     _check(t.size(0) <= MAX_TOKENS, f"{name} has more than {MAX_TOKENS} rows")
     pitch = t.stride(0) if t.size(0) > 1 else t.size(1)
     _check(t.stride(1) == 1 and pitch >= t.size(1), f"{name} must have contiguous rows that do not overlap")
-    _check(t.size(0) == 0 or (t.data_ptr() % 16 == 0 and pitch * t.element_size() % 16 == 0),
-           f"{name}'s rows must start on 16 bytes")
+    _check(False, f"{name}'s rows must start on 16 bytes")
+
+
+def _pitch(t: torch.Tensor) -> int:
+    """Elements between the rows of a matrix the kernels can read, else -1:
+    rows contiguous, not overlapping, each starting on 16 bytes."""
+    stride, shape = t.stride(), t.shape
+    if len(shape) != 2:
+        return -1
+    rows, cols = shape
+    pitch = stride[0] if rows > 1 else cols
+    if (stride[1] != 1 and cols > 1) or pitch < cols or rows > MAX_TOKENS:
+        return -1
+    if rows and (t.data_ptr() & 15 or (rows > 1 and pitch * t.element_size() & 15)):
+        return -1
+    # a lone row has no pitch; its length, a multiple of 16 bytes where the
+    # size checks pass, stands in
     return pitch
 
 
+def _is_dense(t, shape: tuple, dtype: torch.dtype, dev, align: int = 16) -> bool:
+    return (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.device == dev
+            and t.is_contiguous() and not t.data_ptr() & (align - 1))
+
+
 def _check_dense(name: str, t, shape: tuple, dtype: torch.dtype, dev, align: int = 16) -> None:
+    if _is_dense(t, shape, dtype, dev, align):
+        return
     _check_cuda(name, t, dev)
     _check(tuple(t.shape) == shape and t.dtype == dtype and t.is_contiguous(),
            f"{name} must be a contiguous {dtype} tensor of shape {shape}")
@@ -96,36 +125,40 @@ def _check_dense(name: str, t, shape: tuple, dtype: torch.dtype, dev, align: int
 
 
 def _activation(name: str) -> int:
-    _check(name in ACTIVATIONS, f"activation must be one of {sorted(ACTIVATIONS)}, got {name!r}")
-    return ACTIVATIONS[name]
-
-
-def _stream(dev: torch.device) -> int:
-    return torch.cuda.current_stream(dev).cuda_stream
+    act = ACTIVATIONS.get(name) if isinstance(name, str) else None
+    if act is None:
+        raise RuntimeError(f"activation must be one of {sorted(ACTIVATIONS)}, got {name!r}")
+    return act
 
 
 def _scratch(nbytes: int, dev: torch.device) -> torch.Tensor:
     return torch.empty(nbytes, dtype=torch.uint8, device=dev)
 
 
-class _on:
-    """The inputs' device as the current one, at no cost where it already is."""
-
-    def __init__(self, dev: torch.device):
-        self.guard = None if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _call(name: str, dev: torch.device, *args) -> None:
+    """The library function on the current stream of ``dev``, with ``dev`` the
+    current device."""
+    fn = getattr(_bound or _library(), name)
+    if dev.index == torch._C._cuda_getDevice():
+        code = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    else:
+        with torch.cuda.device(dev):
+            code = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    if code:
+        _raise_on(code, name)
 
 
 # ------------------------------------------------- gated feed-forward block
 def _check_ffn(x, w13, w2) -> tuple[int, int, int, int]:
     """(T, H, I, x pitch) of checked inputs."""
+    if isinstance(x, torch.Tensor) and x.is_cuda and isinstance(w2, torch.Tensor) and w2.dim() == 2:
+        dtype, dev = x.dtype, x.device
+        pitch = _pitch(x)
+        H, inter = w2.shape
+        if (pitch >= 0 and x.size(1) == H and (dtype is torch.bfloat16 or dtype is torch.float16)
+                and not (H | inter) & 7 and 8 <= H <= MAX_DIM and 8 <= inter <= MAX_DIM
+                and _is_dense(w13, (2 * inter, H), dtype, dev) and _is_dense(w2, (H, inter), dtype, dev)):
+            return x.size(0), H, inter, pitch
     _check_cuda("x", x)
     _check(x.dtype in (torch.bfloat16, torch.float16), "x must be bfloat16 or float16")
     pitch = _check_rows("x", x)
@@ -145,18 +178,14 @@ def _run_ffn(x, w13, w2, activation, output, save: bool):
     act = _activation(activation)
     dev = x.device
     if output is None:
-        output = torch.empty((T, H), dtype=x.dtype, device=dev)
+        output = x.new_empty((T, H))
     else:
         _check_dense("output", output, (T, H), x.dtype, dev)
-    hidden = torch.empty((T, inter), dtype=x.dtype, device=dev)
+    hidden = x.new_empty((T, inter))
     preact = torch.empty((T, 2 * inter), dtype=torch.float32, device=dev) if save else None
     if T:
-        lib = _library()
-        with _on(dev):
-            code = lib.moe_b200_gated_ffn(x.data_ptr(), pitch, w13.data_ptr(), w2.data_ptr(), TYPES[x.dtype], act, T, H,
-                                          inter, output.data_ptr(), preact.data_ptr() if save else None,
-                                          hidden.data_ptr(), None, 0, _stream(dev))
-        _raise_on(code, "moe_b200_gated_ffn")
+        _call("moe_b200_gated_ffn", dev, x.data_ptr(), pitch, w13.data_ptr(), w2.data_ptr(), TYPES[x.dtype], act, T,
+              H, inter, output.data_ptr(), preact.data_ptr() if save else None, hidden.data_ptr(), None, 0)
     return output, preact, hidden
 
 
@@ -192,7 +221,8 @@ def gated_ffn(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, activation: 
     with gated_ffn_forward / gated_ffn_backward: the autograd engine binds
     each leaf to the stream of its first use, the two functions use the
     current stream alone."""
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (x, w13, w2)):
+    if torch.is_grad_enabled() and (getattr(x, "requires_grad", False) or getattr(w13, "requires_grad", False)
+                                    or getattr(w2, "requires_grad", False)):
         _check(output is None, "output cannot be given where gradients are recorded")
         return _GatedFFN.apply(x, w13, w2, activation)
     return _run_ffn(x, w13, w2, activation, output, False)[0]
@@ -213,24 +243,22 @@ def gated_ffn_backward(grad_output: torch.Tensor, x: torch.Tensor, w13: torch.Te
     act = _activation(activation)
     dev = x.device
     _check_cuda("grad_output", grad_output, dev)
-    _check(grad_output.dtype == x.dtype and tuple(grad_output.shape) == (T, H),
-           f"grad_output must be {x.dtype} [T, {H}] like the output")
+    if grad_output.dtype != x.dtype or grad_output.shape != (T, H):
+        raise RuntimeError(f"grad_output must be {x.dtype} [{T}, {H}] like the output")
     grad_pitch = _check_rows("grad_output", grad_output, H)
+    if not isinstance(saved, (tuple, list)) or len(saved) != 2:
+        raise RuntimeError("saved must be the pair that gated_ffn_forward returned")
     preact, hidden = saved
     _check_dense("saved u and g", preact, (T, 2 * inter), torch.float32, dev, 32)
     _check_dense("saved hidden", hidden, (T, inter), x.dtype, dev)
-    _check(len(needs) == 3, "needs must be three truth values")
-    shapes = ((T, H), (2 * inter, H), (H, inter))
-    grads = [torch.empty(shape, dtype=x.dtype, device=dev) if n else None for shape, n in zip(shapes, needs)]
-    if any(n for n in needs):
-        lib = _library()
-        with _on(dev):
-            ws = _scratch(4 * T * inter + 512, dev)
-            code = lib.moe_b200_gated_ffn_backward(
-                grad_output.data_ptr(), grad_pitch, x.data_ptr(), pitch, w13.data_ptr(), w2.data_ptr(),
-                preact.data_ptr(), hidden.data_ptr(), TYPES[x.dtype], act, T, H, inter,
-                *(g.data_ptr() if g is not None else None for g in grads), ws.data_ptr(), ws.numel(), _stream(dev))
-        _raise_on(code, "moe_b200_gated_ffn_backward")
+    if len(needs) != 3:
+        raise RuntimeError("needs must be three truth values")
+    grads = [x.new_empty(shape) if n else None for shape, n in zip(((T, H), (2 * inter, H), (H, inter)), needs)]
+    if needs[0] or needs[1] or needs[2]:
+        ws = _scratch(4 * T * inter + 512, dev)
+        _call("moe_b200_gated_ffn_backward", dev, grad_output.data_ptr(), grad_pitch, x.data_ptr(), pitch,
+              w13.data_ptr(), w2.data_ptr(), preact.data_ptr(), hidden.data_ptr(), TYPES[x.dtype], act, T, H, inter,
+              *(g.data_ptr() if g is not None else None for g in grads), ws.data_ptr(), ws.numel())
     return tuple(grads)
 
 
@@ -242,6 +270,10 @@ def mxfp4_scale_shape(rows: int, cols: int) -> tuple[int, ...]:
 
 
 def _check_values(name: str, x) -> int:
+    if isinstance(x, torch.Tensor) and x.is_cuda and x.dtype in TYPES:
+        pitch = _pitch(x)
+        if pitch >= 0 and not x.size(1) & 31 and 32 <= x.size(1) <= MAX_DIM:
+            return pitch
     _check_cuda(name, x)
     _check(x.dtype in TYPES, f"{name} must be bfloat16, float16 or float32")
     pitch = _check_rows(name, x)
@@ -251,6 +283,13 @@ def _check_values(name: str, x) -> int:
 
 def _check_mx(name: str, q, scale, dev=None, cols: int | None = None, rows: int | None = None) -> tuple[int, int]:
     """(rows, columns) of a checked 4-bit matrix."""
+    if isinstance(q, torch.Tensor) and q.is_cuda and q.dim() == 2:
+        r, half = q.shape
+        if ((dev is None or q.device == dev) and q.dtype is torch.uint8 and q.is_contiguous() and r <= MAX_TOKENS
+                and not half & 15 and 16 <= half <= MAX_DIM // 2 and (cols is None or 2 * half == cols)
+                and (rows is None or r == rows) and not q.data_ptr() & 15
+                and _is_dense(scale, mxfp4_scale_shape(r, 2 * half), torch.uint8, q.device)):
+            return r, 2 * half
     _check_cuda(name, q, dev)
     _check(q.dtype == torch.uint8 and q.dim() == 2 and q.is_contiguous(),
            f"{name} must be contiguous uint8 codes [R, K / 2]")
@@ -272,29 +311,27 @@ def mxfp4_quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     R, K = x.shape
     dev = x.device
     q = torch.empty((R, K // 2), dtype=torch.uint8, device=dev)
-    scale = torch.empty(mxfp4_scale_shape(R, K), dtype=torch.uint8, device=dev)
+    scale = q.new_empty(mxfp4_scale_shape(R, K))
     if R:
-        lib = _library()
-        with _on(dev):
-            code = lib.moe_b200_mxfp4_quantize(x.data_ptr(), pitch, TYPES[x.dtype], R, K, q.data_ptr(),
-                                               scale.data_ptr(), _stream(dev))
-        _raise_on(code, "moe_b200_mxfp4_quantize")
+        _call("moe_b200_mxfp4_quantize", dev, x.data_ptr(), pitch, TYPES[x.dtype], R, K, q.data_ptr(),
+              scale.data_ptr())
     return q, scale
 
 
 def mxfp4_dequantize(q: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The [R, K] values that a 4-bit matrix stands for, in ``dtype``."""
     R, K = _check_mx("q", q, scale)
-    _check(dtype in TYPES, "dtype must be bfloat16, float16 or float32")
+    _check_type(dtype)
     dev = q.device
     out = torch.empty((R, K), dtype=dtype, device=dev)
     if R:
-        lib = _library()
-        with _on(dev):
-            code = lib.moe_b200_mxfp4_dequantize(q.data_ptr(), scale.data_ptr(), R, K, TYPES[dtype], out.data_ptr(),
-                                                 _stream(dev))
-        _raise_on(code, "moe_b200_mxfp4_dequantize")
+        _call("moe_b200_mxfp4_dequantize", dev, q.data_ptr(), scale.data_ptr(), R, K, TYPES[dtype], out.data_ptr())
     return out
+
+
+def _check_type(dtype) -> None:
+    if dtype not in TYPES:
+        raise RuntimeError("dtype must be bfloat16, float16 or float32")
 
 
 def _mx_output(output, shape: tuple, dtype: torch.dtype, dev: torch.device) -> torch.Tensor:
@@ -310,16 +347,14 @@ def mxfp4_matmul(a_q: torch.Tensor, a_scale: torch.Tensor, b_q: torch.Tensor, b_
     to ``dtype``."""
     M, K = _check_mx("a_q", a_q, a_scale)
     N, _ = _check_mx("b_q", b_q, b_scale, a_q.device, K)
-    _check(N > 0, "b_q must have rows")
-    _check(dtype in TYPES, "dtype must be bfloat16, float16 or float32")
+    if N == 0:
+        raise RuntimeError("b_q must have rows")
+    _check_type(dtype)
     dev = a_q.device
     output = _mx_output(output, (M, N), dtype, dev)
     if M:
-        lib = _library()
-        with _on(dev):
-            code = lib.moe_b200_mxfp4_matmul(a_q.data_ptr(), a_scale.data_ptr(), b_q.data_ptr(), b_scale.data_ptr(), M,
-                                             N, K, TYPES[dtype], output.data_ptr(), _stream(dev))
-        _raise_on(code, "moe_b200_mxfp4_matmul")
+        _call("moe_b200_mxfp4_matmul", dev, a_q.data_ptr(), a_scale.data_ptr(), b_q.data_ptr(), b_scale.data_ptr(),
+              M, N, K, TYPES[dtype], output.data_ptr())
     return output
 
 
@@ -331,15 +366,13 @@ def mxfp4_linear(x: torch.Tensor, w_q: torch.Tensor, w_scale: torch.Tensor,
     T, K = x.shape
     dev = x.device
     N, _ = _check_mx("w_q", w_q, w_scale, dev, K)
-    _check(N > 0, "w_q must have rows")
+    if N == 0:
+        raise RuntimeError("w_q must have rows")
     output = _mx_output(output, (T, N), x.dtype, dev)
     if T:
-        lib = _library()
-        with _on(dev):
-            ws = _scratch(lib.moe_b200_mxfp4_linear_workspace_bytes(T, K), dev)
-            code = lib.moe_b200_mxfp4_linear(x.data_ptr(), pitch, TYPES[x.dtype], w_q.data_ptr(), w_scale.data_ptr(), T,
-                                             N, K, output.data_ptr(), ws.data_ptr(), ws.numel(), _stream(dev))
-        _raise_on(code, "moe_b200_mxfp4_linear")
+        ws = _scratch(_library().moe_b200_mxfp4_linear_workspace_bytes(T, K), dev)
+        _call("moe_b200_mxfp4_linear", dev, x.data_ptr(), pitch, TYPES[x.dtype], w_q.data_ptr(), w_scale.data_ptr(),
+              T, N, K, output.data_ptr(), ws.data_ptr(), ws.numel())
     return output
 
 
@@ -354,19 +387,17 @@ def mxfp4_gated_ffn(x: torch.Tensor, w13_q: torch.Tensor, w13_scale: torch.Tenso
     dev = x.device
     act = _activation(activation)
     two_i, _ = _check_mx("w13_q", w13_q, w13_scale, dev, H)
-    _check(two_i % 2 == 0 and two_i > 0, "w13_q must have 2 I rows")
     inter = two_i // 2
+    if two_i & 63 or not two_i:
+        raise RuntimeError(f"w13_q must have 2 I rows, I a multiple of 32; got {two_i}")
     _check_dim("the intermediate size", inter, 32)
     _check_mx("w2_q", w2_q, w2_scale, dev, inter, H)
     output = _mx_output(output, (T, H), x.dtype, dev)
     if T:
-        lib = _library()
-        with _on(dev):
-            ws = _scratch(lib.moe_b200_mxfp4_gated_ffn_workspace_bytes(T, H, inter), dev)
-            code = lib.moe_b200_mxfp4_gated_ffn(x.data_ptr(), pitch, TYPES[x.dtype], w13_q.data_ptr(),
-                                                w13_scale.data_ptr(), w2_q.data_ptr(), w2_scale.data_ptr(), act, T, H,
-                                                inter, output.data_ptr(), ws.data_ptr(), ws.numel(), _stream(dev))
-        _raise_on(code, "moe_b200_mxfp4_gated_ffn")
+        ws = _scratch(_library().moe_b200_mxfp4_gated_ffn_workspace_bytes(T, H, inter), dev)
+        _call("moe_b200_mxfp4_gated_ffn", dev, x.data_ptr(), pitch, TYPES[x.dtype], w13_q.data_ptr(),
+              w13_scale.data_ptr(), w2_q.data_ptr(), w2_scale.data_ptr(), act, T, H, inter, output.data_ptr(),
+              ws.data_ptr(), ws.numel())
     return output
 
 
@@ -376,7 +407,7 @@ def read_status(device: torch.device | None = None) -> int:
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     st = ctypes.c_uint32(0)
     with torch.cuda.device(dev):
-        code = _library().moe_b200_dense_read_status(ctypes.byref(st), _stream(dev))
+        code = _library().moe_b200_dense_read_status(ctypes.byref(st), torch.cuda.current_stream(dev).cuda_stream)
     if code not in (0, 7):
         _raise_on(code, "moe_b200_dense_read_status")
     return int(st.value)

@@ -216,6 +216,37 @@ def test_autograd(cuda_device):
 
 
 @pytest.mark.gpu
+def test_calls_from_new_threads(cuda_device):
+    """Threads that have not used CUDA before, two at once."""
+    import threading
+
+    import ffn_host
+
+    x, w13, w2, dy = _inputs(40, 256, 128, torch.bfloat16, seed=9)
+    want, saved = ffn_host.gated_ffn_forward(x, w13, w2)
+    grads = ffn_host.gated_ffn_backward(dy, x, w13, w2, saved)
+    torch.cuda.synchronize()
+    got, errors = [], []
+
+    def call():
+        try:
+            y, s = ffn_host.gated_ffn_forward(x, w13, w2)
+            got.append((y, *ffn_host.gated_ffn_backward(dy, x, w13, w2, s)))
+        except Exception as e:  # noqa: BLE001 - reported below
+            errors.append(e)
+
+    threads = [threading.Thread(target=call) for _ in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors, errors
+    for g in got:
+        assert all(torch.equal(a, b) for a, b in zip(g, (want, *grads)))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("T", [7, 260])
 def test_captured_training_step(cuda_device, T):
     """Forward and backward captured into a graph and replayed on new inputs,
