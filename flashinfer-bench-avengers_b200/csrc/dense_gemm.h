@@ -17,6 +17,13 @@ enum DenseEpi : int {
   kEpiDact = 3,        // sums are dh: [du | dg] from the saved up and gate sums
 };
 
+// Where the streaming form's token operand comes from.
+enum TokenSource : int {
+  kFromMatrix = 0,     // A, a 16-bit or 4-bit matrix
+  kFromRows = 1,       // 4-bit: unquantised rows (DenseParams x, of type `type`)
+  kFromSums = 2,       // 4-bit: act(gate) * up of fp32 sums [m, 2 k] (DenseParams x)
+};
+
 // Operands of the 16-bit GEMMs: K-contiguous ("K-major") or contiguous along
 // the output dimension ("MN-major").
 struct DenseOperand {
@@ -39,6 +46,9 @@ struct DenseParams {
   uint8_t* q;          // kEpiGatedQuant: codes [m, n / 2]
   uint8_t* q_scale;    //   and tiled exponents
   uint32_t* status;    // sticky device status word
+  int x_source;        // TokenSource (4-bit streaming form)
+  const void* x;       // its rows, x_pitch bytes apart
+  int64_t x_pitch;
   // derived by the launcher
   int bn, n_step, b_half, m_tiles, n_tiles, k_iters, vec32, stages, stage_bytes;
 };
@@ -62,11 +72,14 @@ int launch_mx_pair(DenseEpi epi, const MxOperand& a, const MxOperand& b, DensePa
                    cudaStream_t s);
 
 // Few rows of A: out = A B^T streaming B, K split over a cluster
-// (kEpiStore, kEpiGated).
+// (kEpiStore and kEpiGated; 4-bit: kEpiStore).
 int launch_dense_skinny(DenseEpi epi, const DenseOperand& a, const DenseOperand& b, DenseParams p, int sm_count,
                         bool dependent, cudaStream_t s);
 int launch_mx_skinny(const MxOperand& a, const MxOperand& b, DenseParams p, int sm_count, bool dependent,
                      cudaStream_t s);
+
+// Whether launch_mx_skinny takes sources other than kFromMatrix at this size.
+bool mx_skinny_quantizes(int64_t m, int64_t n, int64_t k, int sm_count);
 
 // The current device's sticky status word of the dense kernels (a library
 // global), or null when its address cannot be had.

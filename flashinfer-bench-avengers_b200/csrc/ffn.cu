@@ -92,6 +92,16 @@ int quantize(const void* x, int type, int64_t rows, int64_t cols, int64_t pitch,
   return cudaGetLastError() == cudaSuccess ? MOE_B200_OK : MOE_B200_ERR_CUDA;
 }
 
+// x [p->m, p->k] to 4 bits, in `to` or (`inside`) by the GEMM itself.
+int rows_to_4_bits(const void* x, int type, int64_t pitch, const MxBuffers& to, bool inside, DenseParams* p,
+                   cudaStream_t s) {
+  if (!inside) return quantize(x, type, p->m, p->k, pitch, to.q, to.scale, false, s);
+  p->x_source = kFromRows;
+  p->x = x;
+  p->x_pitch = pitch * (type == MOE_B200_TYPE_FP32 ? 4 : 2);
+  return MOE_B200_OK;
+}
+
 int mx_gemm(const MxOperand& a, const MxOperand& b, const DenseParams& p, const Device& d, bool dependent,
             cudaStream_t s) {
   if (p.m <= kSkinnyMaxTokens) return launch_mx_skinny(a, b, p, d.sm_count, dependent, s);
@@ -114,8 +124,10 @@ DenseParams params(const Device& d, int64_t m, int64_t n, int64_t k, int type, i
   return p;
 }
 
-// The 4-bit block with its hidden quantised in the GEMM's epilogue needs the
-// gate rows to start on an exponent tile.
+// The 4-bit block over CTA pairs quantises the hidden in the first GEMM's
+// epilogue, where the gate rows start on an exponent tile. Otherwise the sums
+// go through memory in fp32. (The streaming form with its up and gate tiles
+// in one cluster was slower than that: 32 against 24 us at 128 tokens.)
 bool fused_gate_quant(int64_t T, int64_t I) { return T > kSkinnyMaxTokens && I % 128 == 0; }
 
 size_t mx_ffn_bytes(int64_t T, int64_t H, int64_t I) {
@@ -304,10 +316,11 @@ int moe_b200_mxfp4_linear(const void* x, int64_t x_pitch, int dtype, const void*
   if (st != MOE_B200_OK) return st;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const MxBuffers xq = mx_place(static_cast<uint8_t*>(workspace), T, k);
-  st = quantize(x, dtype, T, k, x_pitch, xq.q, xq.scale, false, s);
+  DenseParams p = params(d, T, n, k, dtype, 0, out, n, dtype);
+  const bool inside = mx_skinny_quantizes(T, n, k, d.sm_count);
+  st = rows_to_4_bits(x, dtype, x_pitch, xq, inside, &p, s);
   if (st != MOE_B200_OK) return st;
-  return mx_gemm(MxOperand{xq.q, xq.scale, T}, MxOperand{w_q, w_scale, n}, params(d, T, n, k, dtype, 0, out, n, dtype),
-                 d, true, s);
+  return mx_gemm(MxOperand{xq.q, xq.scale, T}, MxOperand{w_q, w_scale, n}, p, d, !inside, s);
 }
 
 size_t moe_b200_mxfp4_gated_ffn_workspace_bytes(int64_t num_tokens, int64_t hidden_size, int64_t inter_size) {
@@ -339,25 +352,36 @@ int moe_b200_mxfp4_gated_ffn(const void* x, int64_t x_pitch, int dtype, const vo
   const MxBuffers hq = mx_place(ws + mx_bytes(T, H), T, I);
   const MxOperand xo{xq.q, xq.scale, T}, ho{hq.q, hq.scale, T};
   const MxOperand w13{w13_q, w13_scale, 2 * I}, w2{w2_q, w2_scale, H};
-  st = quantize(x, dtype, T, H, x_pitch, xq.q, xq.scale, false, s);
-  if (st != MOE_B200_OK) return st;
   if (fused_gate_quant(T, I)) {
     DenseParams p = params(d, T, I, H, dtype, activation, nullptr, 0, dtype);
     p.q = hq.q;
     p.q_scale = hq.scale;
+    st = quantize(x, dtype, T, H, x_pitch, xq.q, xq.scale, false, s);
+    if (st != MOE_B200_OK) return st;
     st = launch_mx_pair(kEpiGatedQuant, xo, w13, p, d.sm_count, true, s);
     if (st != MOE_B200_OK) return st;
+    return mx_gemm(ho, w2, params(d, T, H, I, dtype, activation, output, H, dtype), d, true, s);
+  }
+  float* sums = reinterpret_cast<float*>(ws + mx_bytes(T, H) + mx_bytes(T, I));
+  DenseParams p = params(d, T, 2 * I, H, dtype, activation, sums, 2 * I, MOE_B200_TYPE_FP32);
+  const bool x_inside = mx_skinny_quantizes(T, 2 * I, H, d.sm_count);
+  st = rows_to_4_bits(x, dtype, x_pitch, xq, x_inside, &p, s);
+  if (st != MOE_B200_OK) return st;
+  st = mx_gemm(xo, w13, p, d, !x_inside, s);
+  if (st != MOE_B200_OK) return st;
+  DenseParams p2 = params(d, T, H, I, dtype, activation, output, H, dtype);
+  if (mx_skinny_quantizes(T, H, I, d.sm_count)) {
+    p2.x_source = kFromSums;
+    p2.x = sums;
+    p2.x_pitch = 8 * I;
   } else {
-    float* sums = reinterpret_cast<float*>(ws + mx_bytes(T, H) + mx_bytes(T, I));
-    st = mx_gemm(xo, w13, params(d, T, 2 * I, H, dtype, activation, sums, 2 * I, MOE_B200_TYPE_FP32), d, true, s);
-    if (st != MOE_B200_OK) return st;
     const int k_tiles = static_cast<int>(div_up(I, 128));
     if (launch_kernel(mxfp4_gate_kernel, static_cast<unsigned>(div_up(T * 4 * k_tiles, 256)), 256, 0, s, true,
                       static_cast<const float*>(sums), static_cast<int>(T), static_cast<int>(I / 32), k_tiles,
                       activation, hq.q, hq.scale) != cudaSuccess)
       return MOE_B200_ERR_CUDA;
   }
-  return mx_gemm(ho, w2, params(d, T, H, I, dtype, activation, output, H, dtype), d, true, s);
+  return mx_gemm(ho, w2, p2, d, true, s);
 }
 
 int moe_b200_dense_read_status(uint32_t* status, void* stream) {

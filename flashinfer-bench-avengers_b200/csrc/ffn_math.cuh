@@ -84,6 +84,18 @@ __device__ __forceinline__ uint32_t mx_pack8(const float* v, float inv) {
   return r;
 }
 
+// Four values, into the low 16 bits.
+__device__ __forceinline__ uint32_t mx_pack4(const float* v, float inv) {
+  uint16_t r;
+  asm("{\n\t.reg .b8 t0, t1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 t0, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 t1, %4, %3;\n\t"
+      "mov.b16 %0, {t0, t1};\n\t}"
+      : "=h"(r)
+      : "f"(v[0] * inv), "f"(v[1] * inv), "f"(v[2] * inv), "f"(v[3] * inv));
+  return r;
+}
+
 // Byte of row r, 32-column block b in the tiled exponent array of a matrix
 // with `k_tiles` = ceil(K / 128) tiles per 128 rows.
 __host__ __device__ __forceinline__ int64_t mx_scale_offset(int64_t r, int64_t b, int64_t k_tiles) {

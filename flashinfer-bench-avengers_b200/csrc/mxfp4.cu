@@ -22,33 +22,6 @@ namespace moe {
 
 namespace {
 
-// 32 values of a block at `src` (16-byte aligned; whole sectors if vec32).
-template <int kType>
-__device__ __forceinline__ void load_block(const void* src, bool vec32, float* v) {
-  constexpr int kWords = kType == kTypeFp32 ? 32 : 16;
-  uint32_t r[kWords];
-  if (vec32) {
-#pragma unroll
-    for (int j = 0; j < kWords; j += 8) ld_global_32(r + j, static_cast<const uint32_t*>(src) + j);
-  } else {
-#pragma unroll
-    for (int j = 0; j < kWords; j += 4) {
-      const uint4 q = *reinterpret_cast<const uint4*>(static_cast<const uint32_t*>(src) + j);
-      r[j] = q.x, r[j + 1] = q.y, r[j + 2] = q.z, r[j + 3] = q.w;
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < kWords; ++j) {
-    if (kType == kTypeFp32) {
-      v[j] = __uint_as_float(r[j]);
-    } else {
-      const float2 f = unpack_16(r[j], kType);
-      v[2 * j] = f.x;
-      v[2 * j + 1] = f.y;
-    }
-  }
-}
-
 // Codes of a block, and its exponent byte into the row's word of the tiled
 // array. Called by whole warps: the four threads of a word are neighbours,
 // of the same row. `live`: the block exists; `padded`: its exponent byte does
@@ -57,15 +30,8 @@ __device__ __forceinline__ void store_block(const float* v, bool live, bool padd
                                             int k_tiles, uint8_t* q_row, uint8_t* scale) {
   uint32_t byte = 0;
   if (live) {
-    uint32_t amax = 0;
-#pragma unroll
-    for (int j = 0; j < 32; ++j) amax = max(amax, __float_as_uint(v[j]) & 0x7fffffffu);
-    byte = mx_exponent(amax);
-    uint4 c = make_uint4(0, 0, 0, 0);
-    if (byte != 255u) {
-      const float inv = mx_inverse(byte);
-      c = make_uint4(mx_pack8(v, inv), mx_pack8(v + 8, inv), mx_pack8(v + 16, inv), mx_pack8(v + 24, inv));
-    }
+    uint4 c;
+    byte = mx_block(v, &c);
     *reinterpret_cast<uint4*>(q_row + 16 * static_cast<int64_t>(block)) = c;
   }
   uint32_t word = byte << (8 * (block & 3));

@@ -1,11 +1,56 @@
-// Kernels of the 4-bit microscaled format (mxfp4.cu).
+// 4-bit microscaled blocks: what a thread does with one block, and the
+// kernels (mxfp4.cu).
 #pragma once
 
 #include <cuda_runtime.h>
 
 #include <cstdint>
 
+#include "dense_ptx.cuh"
+#include "ffn_math.cuh"
+
 namespace moe {
+
+// 32 values of a block at `src` (16-byte aligned; whole sectors if vec32).
+template <int kType>
+__device__ __forceinline__ void load_block(const void* src, bool vec32, float* v) {
+  constexpr int kWords = kType == kTypeFp32 ? 32 : 16;
+  uint32_t r[kWords];
+  if (vec32) {
+#pragma unroll
+    for (int j = 0; j < kWords; j += 8) ld_global_32(r + j, static_cast<const uint32_t*>(src) + j);
+  } else {
+#pragma unroll
+    for (int j = 0; j < kWords; j += 4) {
+      const uint4 q = *reinterpret_cast<const uint4*>(static_cast<const uint32_t*>(src) + j);
+      r[j] = q.x, r[j + 1] = q.y, r[j + 2] = q.z, r[j + 3] = q.w;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < kWords; ++j) {
+    if (kType == kTypeFp32) {
+      v[j] = __uint_as_float(r[j]);
+    } else {
+      const float2 f = unpack_16(r[j], kType);
+      v[2 * j] = f.x;
+      v[2 * j + 1] = f.y;
+    }
+  }
+}
+
+// The exponent byte and the 16 bytes of codes of 32 values.
+__device__ __forceinline__ uint32_t mx_block(const float* v, uint4* codes) {
+  uint32_t amax = 0;
+#pragma unroll
+  for (int j = 0; j < 32; ++j) amax = max(amax, __float_as_uint(v[j]) & 0x7fffffffu);
+  const uint32_t byte = mx_exponent(amax);
+  *codes = make_uint4(0, 0, 0, 0);
+  if (byte != 255u) {
+    const float inv = mx_inverse(byte);
+    *codes = make_uint4(mx_pack8(v, inv), mx_pack8(v + 8, inv), mx_pack8(v + 16, inv), mx_pack8(v + 24, inv));
+  }
+  return byte;
+}
 
 // rows x (32 * blocks) values, `pitch` bytes between rows, to codes and tiled
 // exponents. Exponents of rows up to pad_rows and of blocks up to
