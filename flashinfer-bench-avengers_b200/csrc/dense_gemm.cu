@@ -21,6 +21,12 @@
 // The operands may be stored along K or along the output dimension (the
 // gradients need W^T and X^T): the shared-memory descriptors take both, so
 // nothing is transposed in memory.
+//
+// One launch takes up to two products whose tiles follow one another in the
+// walk. The backward pass has two pairs of products that do not depend on
+// each other (dh with dW2, dx with dW13): together they fill their last waves
+// and save a kernel's start and end each (training step at 4096 tokens 824 ->
+// 796 us, 333 x 1032 x 520 48 -> 39 us).
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -77,20 +83,39 @@ constexpr int kScaleCol = 464;   // 4-bit: the first of those 48 columns
 constexpr int kEpiWarps = 8;
 constexpr int kPairThreads = (4 + kEpiWarps) * 32;
 
-struct Tile {
-  int m0, n0;   // first output row of the pair, first output column
+// One launch: up to two products, their tiles numbered one after the other.
+struct DenseGroup {
+  DenseParams p[2];
+  int tiles0;        // tiles of the first
+  int tiles;         // of both
+  int stages, stage_bytes;
+};
+
+// Tensor maps: A, B of the first product, then of the second; 4-bit: A, B and
+// their exponents.
+struct PairMaps {
+  CUtensorMap m[4];
+};
+
+struct Work {
+  int g;             // which product
+  int m0, n0;        // first output row of the pair, first output column
 };
 
 // Tiles in bands of 8 row tiles, rows fastest: the pairs running at one time
 // cover a near-square block of the output, so A and B slices are re-read
 // from L2.
-__device__ __forceinline__ Tile tile_at(int t, const DenseParams& p) {
+template <bool kGrouped>
+__device__ __forceinline__ Work work_at(int t, const DenseGroup& grp) {
   constexpr int kBand = 8;
+  Work o;
+  o.g = kGrouped && t >= grp.tiles0 ? 1 : 0;
+  if (o.g) t -= grp.tiles0;
+  const DenseParams& p = grp.p[o.g];
   const int per_band = kBand * p.n_tiles;
   const int band = t / per_band;
   const int r = t - band * per_band;
   const int rows = min(kBand, p.m_tiles - band * kBand);
-  Tile o;
   o.n0 = (r / rows) * p.n_step;
   o.m0 = (band * kBand + r % rows) * 256;
   return o;
@@ -107,16 +132,126 @@ __device__ __forceinline__ void store_row16(uint16_t* row, int c, int n, const u
   }
 }
 
+// ---- epilogues: 32 (or 16) columns of one row, those below `end` -----------
+
+// act(gate) * up, rounded to 16 bits (with the sums, where they are saved) or
+// to one 4-bit block.
+template <int kEpi>
+__device__ __forceinline__ void store_gated(const DenseParams& p, int64_t row, int col, int end, const uint32_t* up,
+                                            const uint32_t* gate) {
+  if constexpr (kEpi == kEpiGated) {
+    if (p.preact != nullptr) {
+      float* pre = p.preact + row * (2 * static_cast<int64_t>(p.n)) + col;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (col + 8 * j < end) {
+          st_global_32(pre + 8 * j, up + 8 * j);
+          st_global_32(pre + p.n + 8 * j, gate + 8 * j);
+        }
+    }
+  }
+  float h[32];
+#pragma unroll
+  for (int j = 0; j < 32; ++j) h[j] = act_value(__uint_as_float(gate[j]), p.act) * __uint_as_float(up[j]);
+  if constexpr (kEpi == kEpiGated) {
+    uint16_t* out = static_cast<uint16_t*>(p.out) + row * p.ldo;
+    uint32_t v[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] = pack_16(h[2 * j], h[2 * j + 1], p.type);
+    store_row16(out, col, end, v, p.vec32);
+    store_row16(out, col + 16, end, v + 8, p.vec32);
+  } else {
+    uint4 v;
+    const uint32_t byte = mx_block(h, &v);
+    *reinterpret_cast<uint4*>(p.q + (row * p.n + col) / 2) = v;
+    p.q_scale[mx_scale_offset(row, col >> 5, (p.n + 127) >> 7)] = static_cast<uint8_t>(byte);
+  }
+}
+
+// The sums themselves, rounded to the output's type.
+template <bool kMx>
+__device__ __forceinline__ void store_plain(const DenseParams& p, int64_t row, int col, int end, const uint32_t* r) {
+  if (kMx && p.out_type == kTypeFp32) {
+    float* out = static_cast<float*>(p.out) + row * p.ldo + col;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (p.vec32 && col + 8 * j + 8 <= end) {
+        st_global_32(out + 8 * j, r + 8 * j);
+      } else {
+        for (int e = 0; e < 8; ++e)
+          if (col + 8 * j + e < end) out[8 * j + e] = __uint_as_float(r[8 * j + e]);
+      }
+    }
+    return;
+  }
+  uint16_t* out = static_cast<uint16_t*>(p.out) + row * p.ldo;
+  uint32_t v[16];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) v[j] = pack_16(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]), p.out_type);
+  if (kMx && !p.vec32) {
+    // any n: column by column
+    for (int j = 0; j < 32; ++j)
+      if (col + j < end) out[col + j] = static_cast<uint16_t>(v[j >> 1] >> (16 * (j & 1)));
+  } else {
+    store_row16(out, col, end, v, p.vec32);
+    store_row16(out, col + 16, end, v + 8, p.vec32);
+  }
+}
+
+// Saved up and gate sums of 16 columns.
+struct Saved {
+  uint32_t u[16], g[16];
+};
+
+__device__ __forceinline__ void load_saved(const DenseParams& p, int64_t row, int col, int end, Saved& s) {
+  const float* pre = p.preact + row * (2 * static_cast<int64_t>(p.n)) + col;
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+    if (col + 8 * e < end) {
+      ld_global_32(s.u + 8 * e, pre + 8 * e);
+      ld_global_32(s.g + 8 * e, pre + p.n + 8 * e);
+    }
+}
+
+// [du | dg] = [dh act(g) | dh u act'(g)] of 16 columns.
+__device__ __forceinline__ void store_dact(const DenseParams& p, int64_t row, int col, int end, const uint32_t* dh,
+                                           const Saved& s) {
+  uint32_t du[8], dg[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    float v[2], w[2];
+#pragma unroll
+    for (int l = 0; l < 2; ++l) {
+      float value, slope;
+      act_value_slope(__uint_as_float(s.g[2 * e + l]), p.act, value, slope);
+      const float d = __uint_as_float(dh[2 * e + l]);
+      v[l] = d * value;
+      w[l] = d * __uint_as_float(s.u[2 * e + l]) * slope;
+    }
+    du[e] = pack_16(v[0], v[1], p.type);
+    dg[e] = pack_16(w[0], w[1], p.type);
+  }
+  uint16_t* out = static_cast<uint16_t*>(p.out) + row * p.ldo;
+  store_row16(out, col, end, du, p.vec32);
+  store_row16(out + p.n, col, end, dg, p.vec32);
+}
+
+// 4-bit: the columns the next accumulator needs are in registers.
+__device__ __forceinline__ void release_early(uint64_t* acce_bar, int lane) {
+  tc_fence_before();
+  if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&acce_bar[0]), 0));
+  __syncwarp();
+}
+
 }  // namespace
 
-template <bool kMx, bool kAMn, bool kBMn, int kEpi>
+template <bool kMx, bool kBMn, int kEpi>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
-    dense_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
-                      const __grid_constant__ CUtensorMap tm_sfa, const __grid_constant__ CUtensorMap tm_sfb,
-                      const DenseParams p) {
+    dense_pair_kernel(const __grid_constant__ PairMaps maps, const __grid_constant__ DenseGroup grp) {
   using Tr = PairTraits<kMx>;
   constexpr bool kGate = kEpi == kEpiGated || kEpi == kEpiGatedQuant;
-  const int kS = p.stages;
+  constexpr bool kGrouped = kEpi == kEpiBackward;   // two products, A stored either way
+  const int kS = grp.stages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
@@ -133,11 +268,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   const uint32_t rank = cluster_cta_rank();
   const int pair = blockIdx.x >> 1;
   const int pairs = gridDim.x >> 1;
-  const int tiles = p.m_tiles * p.n_tiles;
+  const int tiles = grp.tiles;
+  uint32_t* const status = grp.p[0].status;
 
   if (warp == 0 && lane == 0) {
-    prefetch_tmap(&tm_a);
-    prefetch_tmap(&tm_b);
+    prefetch_tmap(&maps.m[0]);
+    prefetch_tmap(&maps.m[1]);
     for (int s = 0; s < kS; ++s) {
       mbar_init(smem_u32(&full_bar[s]), 1);
       mbar_init(smem_u32(&empty_bar[s]), 1);
@@ -167,69 +303,71 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   if (warp == 0) {
     // ---------------------------------------------------------- producer
     const bool issue = elect_lane();
-    const int b_rows = p.bn >> 1;                          // B rows this CTA stages
-    const int b_atoms = kBMn ? (b_rows + 63) >> 6 : 0;
-    const uint32_t bytes =
-        kTileBytes + (kBMn ? static_cast<uint32_t>(b_atoms) * 8192u : static_cast<uint32_t>(b_rows) * 128u) +
-        Tr::kScaleBytes;
-    const int kt = kMx ? (p.k + 127) >> 7 : 0;             // exponent tiles along K
     const uint32_t base = smem_u32(smem);
     const uint32_t full0 = smem_u32(full_bar);
     const uint32_t full0_pair = map_to_cta(full0, 0);
-    auto load_b = [&](int n0, int kb, int stage) {
+    // B's part of a stage, and the count of bytes both CTAs' parts bring.
+    auto load_b = [&](const Work& w, int kb, int stage) {
+      const DenseParams& p = grp.p[w.g];
       const uint32_t bar = full0_pair + 8u * stage;
-      const uint32_t sb = base + stage * p.stage_bytes + kTileBytes;
-      const int bnr = n0 + static_cast<int>(rank) * p.b_half;
-      if (rank == 0) mbar_arrive_expect_tx(full0 + 8u * stage, 2u * bytes);
+      const uint32_t sb = base + stage * grp.stage_bytes + kTileBytes;
+      const int bnr = w.n0 + static_cast<int>(rank) * p.b_half;
+      if (rank == 0) mbar_arrive_expect_tx(full0 + 8u * stage, 2u * p.copy_bytes);
       if constexpr (kMx) {
-        tma_load_2d_pair(sb, &tm_b, bar, kb * 128, bnr);
-        tma_load_2d_pair(sb + kTileBytes + 1024, &tm_sfb, bar, 0, (n0 >> 7) * kt + 2 * kb);
-        tma_load_2d_pair(sb + kTileBytes + 2048, &tm_sfb, bar, 0, ((n0 + p.b_half) >> 7) * kt + 2 * kb);
+        const int kt = (p.k + 127) >> 7;   // exponent tiles along K
+        tma_load_2d_pair(sb, &maps.m[1], bar, kb * 128, bnr);
+        tma_load_2d_pair(sb + kTileBytes + 1024, &maps.m[3], bar, 0, (w.n0 >> 7) * kt + 2 * kb);
+        tma_load_2d_pair(sb + kTileBytes + 2048, &maps.m[3], bar, 0, ((w.n0 + p.b_half) >> 7) * kt + 2 * kb);
       } else if constexpr (kBMn) {
-        tma_load_2d_pair(sb, &tm_b, bar, bnr, kb * 64);
-        if (b_atoms > 1) tma_load_2d_pair(sb + 8192, &tm_b, bar, bnr + 64, kb * 64);
+        const CUtensorMap* map = &maps.m[2 * w.g + 1];
+        tma_load_2d_pair(sb, map, bar, bnr, kb * 64);
+        if (p.bn > 128) tma_load_2d_pair(sb + 8192, map, bar, bnr + 64, kb * 64);
       } else {
-        tma_load_2d_pair(sb, &tm_b, bar, kb * 64, bnr);
+        tma_load_2d_pair(sb, &maps.m[1], bar, kb * 64, bnr);
       }
     };
-    auto load_a = [&](int m0, int kb, int stage) {
+    auto load_a = [&](const Work& w, int kb, int stage) {
+      const DenseParams& p = grp.p[w.g];
       const uint32_t bar = full0_pair + 8u * stage;
-      const uint32_t sa = base + stage * p.stage_bytes;
-      const int am = m0 + static_cast<int>(rank) * 128;
+      const uint32_t sa = base + stage * grp.stage_bytes;
+      const int am = w.m0 + static_cast<int>(rank) * 128;
       if constexpr (kMx) {
-        tma_load_2d_pair(sa, &tm_a, bar, kb * 128, am);
-        tma_load_2d_pair(sa + 2 * kTileBytes, &tm_sfa, bar, 0, (am >> 7) * kt + 2 * kb);
-      } else if constexpr (kAMn) {
-        tma_load_2d_pair(sa, &tm_a, bar, am, kb * 64);
-        tma_load_2d_pair(sa + 8192, &tm_a, bar, am + 64, kb * 64);
+        tma_load_2d_pair(sa, &maps.m[0], bar, kb * 128, am);
+        tma_load_2d_pair(sa + 2 * kTileBytes, &maps.m[2], bar, 0, (am >> 7) * ((p.k + 127) >> 7) + 2 * kb);
       } else {
-        tma_load_2d_pair(sa, &tm_a, bar, kb * 64, am);
+        const CUtensorMap* map = &maps.m[2 * w.g];
+        if (kGrouped && p.a_mn) {
+          tma_load_2d_pair(sa, map, bar, am, kb * 64);
+          tma_load_2d_pair(sa + 8192, map, bar, am + 64, kb * 64);
+        } else {
+          tma_load_2d_pair(sa, map, bar, kb * 64, am);
+        }
       }
     };
     // B is an input of the whole call (weights, or saved by another call):
     // its part of the first ring does not wait for the predecessor.
-    const int early = min(kS, p.k_iters);
-    if (issue) {
-      const int n0 = tile_at(pair, p).n0;
-      for (int kb = 0; kb < early; ++kb) load_b(n0, kb, kb);
-    }
+    const Work w0 = work_at<kGrouped>(pair, grp);
+    const int early = min(kS, grp.p[w0.g].k_iters);
+    if (issue)
+      for (int kb = 0; kb < early; ++kb) load_b(w0, kb, kb);
     __syncwarp();
     pdl_wait();
     int stage = 0;
     uint32_t ph = 0;
     bool ok = true;
     for (int t = pair; ok && t < tiles; t += pairs) {
-      const Tile tl = tile_at(t, p);
+      const Work w = work_at<kGrouped>(t, grp);
+      const int k_iters = grp.p[w.g].k_iters;
       const int skip = t == pair ? early : 0;   // K steps whose B is on its way already
-      for (int kb = 0; kb < p.k_iters; ++kb) {
-        if (kb >= skip && !warp_wait(smem_u32(empty_bar) + 8u * stage, ph ^ 1u, s_abort, p.status,
-                                     kStatusTimeoutProducer)) {
+      for (int kb = 0; kb < k_iters; ++kb) {
+        if (kb >= skip &&
+            !warp_wait(smem_u32(empty_bar) + 8u * stage, ph ^ 1u, s_abort, status, kStatusTimeoutProducer)) {
           ok = false;
           break;
         }
         if (issue) {
-          if (kb >= skip) load_b(tl.n0, kb, stage);
-          load_a(tl.m0, kb, stage);
+          if (kb >= skip) load_b(w, kb, stage);
+          load_a(w, kb, stage);
         }
         __syncwarp();
         if (++stage == kS) {
@@ -249,32 +387,36 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       int it = 0;                 // tiles done by this pair
       int old = kS - 2;           // 4-bit: the stage before last, and its phase
       uint32_t old_ph = 1, sf = 0;
-      const uint32_t idesc0 = kMx ? idesc_mxf4(256, 256, 0) : idesc_f16(256, p.bn, p.type == kTypeFp16, kAMn, kBMn);
-      const uint32_t idesc1 = kMx ? idesc_mxf4(256, 256, 2) : idesc0;
       const uint32_t base = smem_u32(smem);
-      const uint32_t lo_a0 = kAMn ? desc_lo_mnmajor(base) : desc_lo_kmajor(base);
       const uint32_t lo_b0 = kBMn ? desc_lo_mnmajor(base + kTileBytes) : desc_lo_kmajor(base + kTileBytes);
       const uint32_t lo_s0 = desc_lo_scale(base + 2 * kTileBytes);
       for (int t = pair; ok && t < tiles; t += pairs, ++it) {
+        const DenseParams& p = grp.p[work_at<kGrouped>(t, grp).g];
+        const bool a_mn = kGrouped && p.a_mn;
+        const uint32_t idesc0 = kMx ? idesc_mxf4(256, 256, 0) : idesc_f16(256, p.bn, p.type == kTypeFp16, a_mn, kBMn);
+        const uint32_t idesc1 = kMx ? idesc_mxf4(256, 256, 2) : idesc0;
+        const uint32_t lo_a0 = a_mn ? desc_lo_mnmajor(base) : desc_lo_kmajor(base);
+        const uint32_t a_step = a_mn ? 128 : 2;
+        const int k_iters = p.k_iters;
         const int buf = it & 1;
         const uint32_t d = tmem + (buf ? Tr::kAcc1 : 0);
         if (kMx ? it >= 1 : it >= 2) {
           const uint32_t bar = smem_u32(&acce_bar[kMx ? 0 : buf]);
           const uint32_t par = kMx ? static_cast<uint32_t>(it - 1) & 1u : (static_cast<uint32_t>(it >> 1) - 1u) & 1u;
-          if (!__all_sync(0xffffffffu, mbar_wait_cluster(bar, par, s_abort, p.status, kStatusTimeoutMma))) break;
+          if (!__all_sync(0xffffffffu, mbar_wait_cluster(bar, par, s_abort, status, kStatusTimeoutMma))) break;
           tc_fence_after();
         }
-        for (int kb = 0; kb < p.k_iters; ++kb) {
-          if (!warp_wait(smem_u32(full_bar) + 8u * stage, ph, s_abort, p.status, kStatusTimeoutMma)) {
+        for (int kb = 0; kb < k_iters; ++kb) {
+          if (!warp_wait(smem_u32(full_bar) + 8u * stage, ph, s_abort, status, kStatusTimeoutMma)) {
             ok = false;
             break;
           }
-          const uint32_t off = static_cast<uint32_t>(stage * (p.stage_bytes >> 4));
+          const uint32_t off = static_cast<uint32_t>(stage * (grp.stage_bytes >> 4));
           const uint32_t lo_a = lo_a0 + off, lo_b = lo_b0 + off;
           if constexpr (kMx) {
             // The exponent columns written now were last read two stages ago
             // (the first two waits pass at once).
-            if (!warp_wait(smem_u32(empty_bar) + 8u * old, old_ph, s_abort, p.status, kStatusTimeoutMma)) {
+            if (!warp_wait(smem_u32(empty_bar) + 8u * old, old_ph, s_abort, status, kStatusTimeoutMma)) {
               ok = false;
               break;
             }
@@ -304,11 +446,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             } else {
 #pragma unroll
               for (int k = 0; k < 4; ++k)
-                umma_f16<2>(d, desc_of(kDescHiSw128, lo_a + (kAMn ? 128 : 2) * k),
+                umma_f16<2>(d, desc_of(kDescHiSw128, lo_a + a_step * k),
                             desc_of(kDescHiSw128, lo_b + (kBMn ? 128 : 2) * k), idesc0, kb | k);
             }
             umma_commit_pair(smem_u32(empty_bar) + 8u * stage);
-            if (kb == p.k_iters - 1) umma_commit_pair(smem_u32(&accf_bar[buf]));
+            if (kb == k_iters - 1) umma_commit_pair(smem_u32(&accf_bar[buf]));
           }
           __syncwarp();
           sf ^= 24u;
@@ -324,24 +466,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     const int quarter = warp & 3;
     const int half = (warp - 4) >> 2;   // two warps per quarter, taking turns at 32-column chunks
     const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
-    const int width = kGate ? p.n_step : p.bn;   // output columns of a tile
-    const int chunks = (width + 31) >> 5;
-    const bool vec32 = p.vec32 != 0;
     int it = 0;
     for (int t = pair; t < tiles; t += pairs, ++it) {
-      const Tile tl = tile_at(t, p);
+      const Work w = work_at<kGrouped>(t, grp);
+      const DenseParams& p = grp.p[w.g];
+      const int width = kGate ? p.n_step : p.bn;   // output columns of a tile
+      const int chunks = (width + 31) >> 5;
       const int buf = it & 1;
-      const bool ready = mbar_wait(smem_u32(&accf_bar[buf]), static_cast<uint32_t>(it >> 1) & 1u, s_abort, p.status,
+      const int64_t row = static_cast<int64_t>(w.m0) + rank * 128 + quarter * 32 + lane;
+      const bool live = row < p.m;
+      const int end = min(p.n, w.n0 + width);      // first column past this tile
+      // dh: the saved sums of the first two 16-column pieces are on their way
+      // while the accumulator is still being computed.
+      const bool dact = kEpi == kEpiBackward && p.preact != nullptr;
+      Saved saved[2];
+      if (dact) {
+        load_saved(p, row, w.n0 + 32 * half, live ? end : 0, saved[0]);
+        load_saved(p, row, w.n0 + 32 * half + 16, live ? end : 0, saved[1]);
+      }
+      const bool ready = mbar_wait(smem_u32(&accf_bar[buf]), static_cast<uint32_t>(it >> 1) & 1u, s_abort, status,
                                    kStatusTimeoutEpilogue);
       if (!__all_sync(0xffffffffu, ready)) break;
       tc_fence_after();
       const uint32_t acc = lanes + (buf ? Tr::kAcc1 : 0);
-      const int64_t row = static_cast<int64_t>(tl.m0) + rank * 128 + quarter * 32 + lane;
-      const bool live = row < p.m;
-      const int end = min(p.n, tl.n0 + width);   // first column past this tile
       for (int i = half; i < chunks; i += 2) {
         // 4-bit operands: the columns shared with the other accumulator first
         const int c = 32 * (kMx && buf == 0 ? chunks - 1 - i : i);
+        const int col = w.n0 + c;
         uint32_t r[32];
         __syncwarp();
         if constexpr (kGate) {
@@ -349,107 +500,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           tmem_ld32(acc + c, r);
           tmem_ld32(acc + p.n_step + c, g);
           tmem_wait_ld();
-          if (kMx && i == half) {
-            tc_fence_before();
-            if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&acce_bar[0]), 0));
-            __syncwarp();
-          }
-          if (live && tl.n0 + c < end) {
-            if constexpr (kEpi == kEpiGated) {
-              if (p.preact != nullptr) {
-                float* pre = p.preact + row * (2 * static_cast<int64_t>(p.n)) + tl.n0 + c;
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                  if (tl.n0 + c + 8 * j < end) {
-                    st_global_32(pre + 8 * j, r + 8 * j);
-                    st_global_32(pre + p.n + 8 * j, g + 8 * j);
-                  }
-              }
-            }
-            float h[32];
-#pragma unroll
-            for (int j = 0; j < 32; ++j) h[j] = act_value(__uint_as_float(g[j]), p.act) * __uint_as_float(r[j]);
-            if constexpr (kEpi == kEpiGated) {
-              uint16_t* out = static_cast<uint16_t*>(p.out) + row * p.ldo;
-              uint32_t v[16];
-#pragma unroll
-              for (int j = 0; j < 16; ++j) v[j] = pack_16(h[2 * j], h[2 * j + 1], p.type);
-              store_row16(out, tl.n0 + c, end, v, vec32);
-              store_row16(out, tl.n0 + c + 16, end, v + 8, vec32);
-            } else {
-              uint4 v;
-              const uint32_t byte = mx_block(h, &v);
-              *reinterpret_cast<uint4*>(p.q + (row * p.n + tl.n0 + c) / 2) = v;
-              p.q_scale[mx_scale_offset(row, (tl.n0 + c) >> 5, (p.n + 127) >> 7)] = static_cast<uint8_t>(byte);
-            }
-          }
+          if (kMx && i == half) release_early(acce_bar, lane);
+          if (live && col < end) store_gated<kEpi>(p, row, col, end, r, g);
         } else {
           tmem_ld32(acc + c, r);
           tmem_wait_ld();
-          if (kMx && i == half) {
-            tc_fence_before();
-            if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&acce_bar[0]), 0));
-            __syncwarp();
-          }
-          if (live && tl.n0 + c < end) {
-            if constexpr (kEpi == kEpiStore) {
-              if (p.out_type == kTypeFp32) {
-                float* out = static_cast<float*>(p.out) + row * p.ldo + tl.n0 + c;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                  if (vec32 && tl.n0 + c + 8 * j + 8 <= end) {
-                    st_global_32(out + 8 * j, r + 8 * j);
-                  } else {
-                    for (int e = 0; e < 8; ++e)
-                      if (tl.n0 + c + 8 * j + e < end) out[8 * j + e] = __uint_as_float(r[8 * j + e]);
-                  }
-                }
-              } else {
-                uint16_t* out = static_cast<uint16_t*>(p.out) + row * p.ldo;
-                uint32_t v[16];
-#pragma unroll
-                for (int j = 0; j < 16; ++j)
-                  v[j] = pack_16(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]), p.out_type);
-                if (kMx && !vec32) {
-                  // any n: column by column
-                  for (int j = 0; j < 32; ++j)
-                    if (tl.n0 + c + j < end) out[tl.n0 + c + j] = static_cast<uint16_t>(v[j >> 1] >> (16 * (j & 1)));
-                } else {
-                  store_row16(out, tl.n0 + c, end, v, vec32);
-                  store_row16(out, tl.n0 + c + 16, end, v + 8, vec32);
-                }
-              }
-            } else {   // kEpiDact
-              const float* pre = p.preact + row * (2 * static_cast<int64_t>(p.n)) + tl.n0 + c;
-              uint16_t* out = static_cast<uint16_t*>(p.out) + row * p.ldo;
-#pragma unroll
-              for (int j = 0; j < 2; ++j) {
-                uint32_t u[16] = {}, g[16] = {};
-#pragma unroll
-                for (int e = 0; e < 2; ++e)
-                  if (tl.n0 + c + 16 * j + 8 * e < end) {
-                    ld_global_32(u + 8 * e, pre + 16 * j + 8 * e);
-                    ld_global_32(g + 8 * e, pre + p.n + 16 * j + 8 * e);
-                  }
-                uint32_t du[8], dg[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                  float v[2], w[2];
-#pragma unroll
-                  for (int l = 0; l < 2; ++l) {
-                    float value, slope;
-                    act_value_slope(__uint_as_float(g[2 * e + l]), p.act, value, slope);
-                    const float dh = __uint_as_float(r[16 * j + 2 * e + l]);
-                    v[l] = dh * value;
-                    w[l] = dh * __uint_as_float(u[2 * e + l]) * slope;
-                  }
-                  du[e] = pack_16(v[0], v[1], p.type);
-                  dg[e] = pack_16(w[0], w[1], p.type);
-                }
-                store_row16(out, tl.n0 + c + 16 * j, end, du, vec32);
-                store_row16(out + p.n, tl.n0 + c + 16 * j, end, dg, vec32);
-              }
-            }
+          if (kMx && i == half) release_early(acce_bar, lane);
+          if (dact) {
+            const int next = i + 2 < chunks && live ? end : 0;
+            if (live && col < end) store_dact(p, row, col, end, r, saved[0]);
+            load_saved(p, row, col + 64, next, saved[0]);
+            if (live && col + 16 < end) store_dact(p, row, col + 16, end, r + 16, saved[1]);
+            load_saved(p, row, col + 80, next, saved[1]);
+          } else if (live && col < end) {
+            store_plain<kMx>(p, row, col, end, r);
           }
         }
       }
@@ -472,48 +536,47 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 
 namespace {
 
-template <bool kMx, bool kAMn, bool kBMn, int kEpi>
-int launch_pair(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& sfa, const CUtensorMap& sfb,
-                const DenseParams& p, int sm_count, bool dependent, cudaStream_t s) {
-  auto kern = dense_pair_kernel<kMx, kAMn, kBMn, kEpi>;
+// As many stages as the ring holds.
+void set_ring(DenseGroup* grp, int stage_bytes) {
+  grp->stage_bytes = stage_bytes;
+  grp->stages = kRingBytes / stage_bytes < kMaxStages ? kRingBytes / stage_bytes : kMaxStages;
+}
+
+template <bool kMx, bool kBMn, int kEpi>
+int launch_pair(const PairMaps& maps, const DenseGroup& grp, int sm_count, bool dependent, cudaStream_t s) {
+  auto kern = dense_pair_kernel<kMx, kBMn, kEpi>;
   constexpr int smem = kPairSmem;
   static OncePerDevice ready;
   if (!ready([&] {
         return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) == cudaSuccess;
       }))
     return MOE_B200_ERR_CUDA;
-  const int64_t tiles = static_cast<int64_t>(p.m_tiles) * p.n_tiles;
-  const int pairs = static_cast<int>(tiles < sm_count / 2 ? tiles : sm_count / 2);
-  return launch_kernel(kern, 2 * pairs, kPairThreads, smem, s, dependent, a, b, sfa, sfb, p) == cudaSuccess
+  const int pairs = grp.tiles < sm_count / 2 ? grp.tiles : sm_count / 2;
+  return launch_kernel(kern, 2 * pairs, kPairThreads, smem, s, dependent, maps, grp) == cudaSuccess
              ? MOE_B200_OK
              : MOE_B200_ERR_CUDA;
 }
 
-// As many stages as the ring holds: a K step's loads take about 1.8 us to
-// come back, so with six stages a step takes 300 ns however narrow the tile.
-void set_ring(DenseParams* p, int stage_bytes) {
-  p->stage_bytes = stage_bytes;
-  p->stages = kRingBytes / stage_bytes < kMaxStages ? kRingBytes / stage_bytes : kMaxStages;
+// Time units of a tile of bn columns: a K step costs an MMA 2 N cycles and the
+// loads 256 + N (A's 128 rows and N / 2 rows of B per CTA; at about 64 bytes a
+// cycle from L2 the two meet at N = 256; B stored along N comes in 64-column
+// atoms whatever N is); a tile's start and epilogue cost about 1500 more.
+int64_t tile_cost(const DenseParams& p, int bn, bool b_mn) {
+  const int64_t load = 256 + (b_mn ? (bn > 128 ? 256 : 128) : bn), mma = 2 * bn;
+  return div_up(p.k, 64) * (load > mma ? load : mma) + 1500;
 }
 
-// Columns per tile (the MMA's N, 64 to 256): the fewest time units over all
-// waves of tiles. A K step costs an MMA 2 N cycles and the loads 256 + N (A's
-// 128 rows and N / 2 rows of B per CTA; at about 64 bytes a cycle from L2 the
-// two meet at N = 256); a tile's start and epilogue cost about 1500 more.
-// B stored along N is loaded in 64-column atoms whatever N is. Against 256
-// throughout: training step at 4096 tokens 813 -> 786 us, at 333 x 1032 x 520
-// 75 -> 55 us.
-int choose_bn(const DenseParams& p, bool gate, bool b_mn, int pairs) {
-  const int64_t m_tiles = div_up(p.m, 256), k = div_up(p.k, 64);
+int64_t tile_count(const DenseParams& p, int step) { return div_up(p.m, 256) * div_up(p.n, step); }
+
+// Columns per tile (the MMA's N) of one product: the fewest time units over
+// all waves of tiles. Against 256 throughout: training step at 4096 tokens
+// 813 -> 786 us, at 333 x 1032 x 520 75 -> 55 us. The columns of a tile come
+// in whole 32-byte stores, so 16 features.
+int choose_bn(const DenseParams& p, bool gate, int pairs) {
   int best = 256;
   int64_t best_cost = INT64_MAX;
-  // the columns of a tile come in whole 32-byte stores: 16 features
   for (int bn = 256; bn >= 64; bn -= gate ? 32 : 16) {
-    const int step = gate ? bn / 2 : bn;
-    const int64_t waves = div_up(m_tiles * div_up(p.n, step), pairs);
-    const int64_t b_cols = b_mn ? div_up(bn / 2, 64) * 128 : bn;
-    const int64_t load = 256 + b_cols, mma = 2 * bn;
-    const int64_t cost = waves * (k * (load > mma ? load : mma) + 1500);
+    const int64_t cost = div_up(tile_count(p, gate ? bn / 2 : bn), pairs) * tile_cost(p, bn, false);
     if (cost < best_cost) {
       best_cost = cost;
       best = bn;
@@ -522,58 +585,127 @@ int choose_bn(const DenseParams& p, bool gate, bool b_mn, int pairs) {
   return best;
 }
 
-}  // namespace
-
-int launch_dense_pair(DenseEpi epi, const DenseOperand& a, bool a_mn, const DenseOperand& b, bool b_mn, DenseParams p,
-                      int sm_count, bool dependent, cudaStream_t s) {
-  const bool gate = epi == kEpiGated;
-  p.bn = choose_bn(p, gate, b_mn, sm_count / 2);
-  p.n_step = gate ? p.bn / 2 : p.bn;
-  p.b_half = gate ? p.n : p.bn / 2;
-  p.m_tiles = static_cast<int>(div_up(p.m, 256));
-  p.n_tiles = static_cast<int>(div_up(p.n, p.n_step));
-  p.k_iters = static_cast<int>(div_up(p.k, 64));
-  set_ring(&p, kTileBytes + (b_mn ? static_cast<int>(div_up(p.bn / 2, 64)) * 8192 : p.bn / 2 * 128));
-  const int64_t dact_half = epi == kEpiDact ? static_cast<int64_t>(p.n) * 2 : 0;
-  p.vec32 = aligned(p.out, 32) && (p.ldo * 2) % 32 == 0 && dact_half % 32 == 0;
-  CUtensorMap ta, tb;
-  if (!encode_2d(&ta, a.base, 2, a.cols, a.rows, a.pitch, 64, a_mn ? 64 : 128) ||
-      !encode_2d(&tb, b.base, 2, b.cols, b.rows, b.pitch, 64, b_mn ? 64 : p.bn / 2))
-    return MOE_B200_ERR_DRIVER;
-  if (epi == kEpiGated && !a_mn && !b_mn)
-    return launch_pair<false, false, false, kEpiGated>(ta, tb, ta, tb, p, sm_count, dependent, s);
-  if (epi == kEpiDact && !a_mn && b_mn)
-    return launch_pair<false, false, true, kEpiDact>(ta, tb, ta, tb, p, sm_count, dependent, s);
-  if (epi == kEpiStore && !a_mn && !b_mn)
-    return launch_pair<false, false, false, kEpiStore>(ta, tb, ta, tb, p, sm_count, dependent, s);
-  if (epi == kEpiStore && !a_mn && b_mn)
-    return launch_pair<false, false, true, kEpiStore>(ta, tb, ta, tb, p, sm_count, dependent, s);
-  if (epi == kEpiStore && a_mn && b_mn)
-    return launch_pair<false, true, true, kEpiStore>(ta, tb, ta, tb, p, sm_count, dependent, s);
-  return MOE_B200_ERR_INVALID_ARGUMENT;
+// The same for two products walked one after the other: the busiest pair is
+// the first one (the most tiles of the first product) or the last to take one
+// of the second's.
+void choose_bn_two(DenseParams* p, int pairs) {
+  int64_t best_cost = INT64_MAX;
+  for (int b0 = 256; b0 >= 64; b0 -= 32)
+    for (int b1 = 256; b1 >= 64; b1 -= 32) {
+      const int64_t t0 = tile_count(p[0], b0), t1 = tile_count(p[1], b1);
+      const int64_t c0 = tile_cost(p[0], b0, true), c1 = tile_cost(p[1], b1, true);
+      const int64_t all = div_up(t0 + t1, pairs), most0 = div_up(t0, pairs), least0 = t0 / pairs;
+      int64_t cost = most0 * c0 + (all - most0) * c1;
+      const int64_t other = least0 * c0 + (all - least0) * c1;
+      if ((t0 + t1) % pairs == 0 || (t0 + t1) % pairs > t0 % pairs)   // a pair has one tile of the first less
+        cost = cost > other ? cost : other;
+      if (cost < best_cost) {
+        best_cost = cost;
+        p[0].bn = b0;
+        p[1].bn = b1;
+      }
+    }
 }
 
-int launch_mx_pair(DenseEpi epi, const MxOperand& a, const MxOperand& b, DenseParams p, int sm_count, bool dependent,
-                   cudaStream_t s) {
+// Derived fields of a 16-bit product with its bn chosen.
+void finish(DenseParams* p, bool gate, bool b_mn) {
+  p->n_step = gate ? p->bn / 2 : p->bn;
+  p->b_half = gate ? p->n : p->bn / 2;
+  p->m_tiles = static_cast<int>(div_up(p->m, 256));
+  p->n_tiles = static_cast<int>(div_up(p->n, p->n_step));
+  p->k_iters = static_cast<int>(div_up(p->k, 64));
+  p->copy_bytes = kTileBytes + (b_mn ? (p->bn > 128 ? 16384 : 8192) : p->bn / 2 * 128);
+}
+
+}  // namespace
+
+int launch_dense_pair(DenseEpi epi, const DenseOperand& a, const DenseOperand& b, const DenseParams& params,
+                      int sm_count, bool dependent, cudaStream_t s) {
+  const bool gate = epi == kEpiGated;
+  DenseGroup grp;
+  std::memset(&grp, 0, sizeof(grp));
+  DenseParams& p = grp.p[0];
+  p = params;
+  p.bn = choose_bn(p, gate, sm_count / 2);
+  finish(&p, gate, false);
+  p.vec32 = aligned(p.out, 32) && (p.ldo * 2) % 32 == 0;
+  grp.tiles0 = grp.tiles = p.m_tiles * p.n_tiles;
+  set_ring(&grp, p.copy_bytes);
+  PairMaps maps;
+  if (!encode_2d(&maps.m[0], a.base, 2, a.cols, a.rows, a.pitch, 64, 128) ||
+      !encode_2d(&maps.m[1], b.base, 2, b.cols, b.rows, b.pitch, 64, p.bn / 2))
+    return MOE_B200_ERR_DRIVER;
+  maps.m[2] = maps.m[3] = maps.m[0];
+  return gate ? launch_pair<false, false, kEpiGated>(maps, grp, sm_count, dependent, s)
+              : launch_pair<false, false, kEpiStore>(maps, grp, sm_count, dependent, s);
+}
+
+int launch_dense_backward(const DenseProduct* products, int count, int sm_count, bool dependent, cudaStream_t s) {
+  DenseGroup grp;
+  std::memset(&grp, 0, sizeof(grp));
+  for (int i = 0; i < count; ++i) grp.p[i] = products[i].p;
+  if (count == 1) {
+    // with no second product its cost and tiles are zero
+    DenseParams* p = grp.p;
+    int64_t best = INT64_MAX;
+    for (int bn = 256; bn >= 64; bn -= 32) {
+      const int64_t cost = div_up(tile_count(*p, bn), sm_count / 2) * tile_cost(*p, bn, true);
+      if (cost < best) {
+        best = cost;
+        p->bn = bn;
+      }
+    }
+  } else {
+    choose_bn_two(grp.p, sm_count / 2);
+  }
+  PairMaps maps;
+  int stage = 0;
+  for (int i = 0; i < count; ++i) {
+    const DenseOperand &a = products[i].a, &b = products[i].b;
+    DenseParams& p = grp.p[i];
+    p.a_mn = products[i].a_mn;
+    finish(&p, false, true);
+    // kEpiDact writes du and, n columns on, dg
+    p.vec32 = aligned(p.out, 32) && (p.ldo * 2) % 32 == 0 && (p.preact == nullptr || p.n % 16 == 0);
+    grp.tiles += p.m_tiles * p.n_tiles;
+    if (i == 0) grp.tiles0 = grp.tiles;
+    stage = stage > p.copy_bytes ? stage : p.copy_bytes;
+    if (!encode_2d(&maps.m[2 * i], a.base, 2, a.cols, a.rows, a.pitch, 64, p.a_mn ? 64 : 128) ||
+        !encode_2d(&maps.m[2 * i + 1], b.base, 2, b.cols, b.rows, b.pitch, 64, 64))
+      return MOE_B200_ERR_DRIVER;
+  }
+  if (count == 1) maps.m[2] = maps.m[3] = maps.m[0];
+  set_ring(&grp, stage);
+  return launch_pair<false, true, kEpiBackward>(maps, grp, sm_count, dependent, s);
+}
+
+int launch_mx_pair(DenseEpi epi, const MxOperand& a, const MxOperand& b, const DenseParams& params, int sm_count,
+                   bool dependent, cudaStream_t s) {
   const bool gate = epi == kEpiGatedQuant;
+  DenseGroup grp;
+  std::memset(&grp, 0, sizeof(grp));
+  DenseParams& p = grp.p[0];
+  p = params;
   p.bn = 256;
   p.n_step = gate ? 128 : 256;
   p.b_half = gate ? p.n : 128;
   p.m_tiles = static_cast<int>(div_up(p.m, 256));
   p.n_tiles = static_cast<int>(div_up(p.n, p.n_step));
   p.k_iters = static_cast<int>(div_up(p.k, 256));
-  set_ring(&p, 2 * kTileBytes + PairTraits<true>::kScaleBytes);
+  p.copy_bytes = 2 * kTileBytes + PairTraits<true>::kScaleBytes;
   const int esz = p.out_type == kTypeFp32 ? 4 : 2;
   p.vec32 = aligned(p.out, 32) && (p.ldo * esz) % 32 == 0 && p.n % 8 == 0;
+  grp.tiles0 = grp.tiles = p.m_tiles * p.n_tiles;
+  set_ring(&grp, p.copy_bytes);
   const int64_t kt = div_up(p.k, 128);
-  CUtensorMap ta, tb, tsa, tsb;
-  if (!encode_2d(&ta, a.q, 1, p.k / 2, a.rows, p.k / 2, 128, 128) ||
-      !encode_2d(&tb, b.q, 1, p.k / 2, b.rows, p.k / 2, 128, 128) ||
-      !encode_2d(&tsa, a.scale, 2, 256, div_up(a.rows, 128) * kt, 512, 256, 2, false) ||
-      !encode_2d(&tsb, b.scale, 2, 256, div_up(b.rows, 128) * kt, 512, 256, 2, false))
+  PairMaps maps;
+  if (!encode_2d(&maps.m[0], a.q, 1, p.k / 2, a.rows, p.k / 2, 128, 128) ||
+      !encode_2d(&maps.m[1], b.q, 1, p.k / 2, b.rows, p.k / 2, 128, 128) ||
+      !encode_2d(&maps.m[2], a.scale, 2, 256, div_up(a.rows, 128) * kt, 512, 256, 2, false) ||
+      !encode_2d(&maps.m[3], b.scale, 2, 256, div_up(b.rows, 128) * kt, 512, 256, 2, false))
     return MOE_B200_ERR_DRIVER;
-  if (gate) return launch_pair<true, false, false, kEpiGatedQuant>(ta, tb, tsa, tsb, p, sm_count, dependent, s);
-  return launch_pair<true, false, false, kEpiStore>(ta, tb, tsa, tsb, p, sm_count, dependent, s);
+  return gate ? launch_pair<true, false, kEpiGatedQuant>(maps, grp, sm_count, dependent, s)
+              : launch_pair<true, false, kEpiStore>(maps, grp, sm_count, dependent, s);
 }
 
 }  // namespace moe

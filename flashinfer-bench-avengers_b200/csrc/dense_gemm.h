@@ -14,7 +14,8 @@ enum DenseEpi : int {
   kEpiStore = 0,       // out[r, c] = sum, rounded to out_type
   kEpiGated = 1,       // h = act(gate) * up from the up and gate sums; optionally the sums in fp32
   kEpiGatedQuant = 2,  // the same h, in 4 bits with block exponents
-  kEpiDact = 3,        // sums are dh: [du | dg] from the saved up and gate sums
+  kEpiBackward = 3,    // preact set: the sums are dh, out = [du | dg] with the saved up and gate sums;
+                       // otherwise out[r, c] = sum
 };
 
 // Where the streaming form's token operand comes from.
@@ -24,8 +25,7 @@ enum TokenSource : int {
   kFromSums = 2,       // 4-bit: act(gate) * up of fp32 sums [m, 2 k] (DenseParams x)
 };
 
-// Operands of the 16-bit GEMMs: K-contiguous ("K-major") or contiguous along
-// the output dimension ("MN-major").
+// A stored matrix of 16-bit elements.
 struct DenseOperand {
   const void* base;
   int64_t rows;      // rows of the stored matrix
@@ -40,9 +40,9 @@ struct DenseParams {
   int act;             // activation code
   int type;            // operand type code (bf16 / fp16)
   int out_type;        // type code of `out`
-  void* out;           // [m, n], row pitch ldo elements; kEpiDact: [m, 2 n]
+  void* out;           // [m, n], row pitch ldo elements; [du | dg]: [m, 2 n]
   int64_t ldo;
-  float* preact;       // fp32 [m, 2 n]: written by kEpiGated when set, read by kEpiDact
+  float* preact;       // fp32 [m, 2 n]: written by kEpiGated when set, read by kEpiBackward
   uint8_t* q;          // kEpiGatedQuant: codes [m, n / 2]
   uint8_t* q_scale;    //   and tiled exponents
   uint32_t* status;    // sticky device status word
@@ -50,7 +50,14 @@ struct DenseParams {
   const void* x;       // its rows, x_pitch bytes apart
   int64_t x_pitch;
   // derived by the launcher
-  int bn, n_step, b_half, m_tiles, n_tiles, k_iters, vec32, stages, stage_bytes;
+  int bn, n_step, b_half, m_tiles, n_tiles, k_iters, vec32, a_mn, copy_bytes;
+};
+
+// D = A B^T with B stored K x N, and A stored M x K or (a_mn) K x M.
+struct DenseProduct {
+  DenseOperand a, b;
+  bool a_mn;
+  DenseParams p;
 };
 
 struct MxOperand {
@@ -62,14 +69,18 @@ struct MxOperand {
 // B of every GEMM must be complete before the call's first kernel starts: it
 // is read before the previous kernel has finished. A may be its result.
 //
-// D = A B^T over CTA pairs; a_mn / b_mn: the operand is stored K x M (K x N).
-// kEpiGated: B has 2 n rows, up then gate. Returns a MOE_B200 status code.
-int launch_dense_pair(DenseEpi epi, const DenseOperand& a, bool a_mn, const DenseOperand& b, bool b_mn, DenseParams p,
-                      int sm_count, bool dependent, cudaStream_t s);
+// D = A B^T over CTA pairs, both operands stored along K (kEpiStore,
+// kEpiGated: B has 2 n rows, up then gate). Returns a MOE_B200 status code.
+int launch_dense_pair(DenseEpi epi, const DenseOperand& a, const DenseOperand& b, const DenseParams& p, int sm_count,
+                      bool dependent, cudaStream_t s);
 
-// The same for 4-bit operands (kEpiStore, kEpiGatedQuant).
-int launch_mx_pair(DenseEpi epi, const MxOperand& a, const MxOperand& b, DenseParams p, int sm_count, bool dependent,
-                   cudaStream_t s);
+// One or two products of the backward pass that do not depend on each other,
+// in one launch.
+int launch_dense_backward(const DenseProduct* products, int count, int sm_count, bool dependent, cudaStream_t s);
+
+// 4-bit operands over CTA pairs (kEpiStore, kEpiGatedQuant).
+int launch_mx_pair(DenseEpi epi, const MxOperand& a, const MxOperand& b, const DenseParams& p, int sm_count,
+                   bool dependent, cudaStream_t s);
 
 // Few rows of A: out = A B^T streaming B, K split over a cluster
 // (kEpiStore and kEpiGated; 4-bit: kEpiStore).

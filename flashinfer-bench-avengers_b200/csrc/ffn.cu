@@ -55,7 +55,7 @@ DenseOperand rows_of(const void* base, int64_t rows, int64_t cols, int64_t pitch
 int forward_gemm(DenseEpi epi, const DenseOperand& x, const DenseOperand& w, const DenseParams& p, const Device& d,
                  bool dependent, cudaStream_t s) {
   if (p.m <= kSkinnyMaxTokens) return launch_dense_skinny(epi, x, w, p, d.sm_count, dependent, s);
-  return launch_dense_pair(epi, x, false, w, false, p, d.sm_count, dependent, s);
+  return launch_dense_pair(epi, x, w, p, d.sm_count, dependent, s);
 }
 
 // ---- 4-bit matrices ---------------------------------------------------------
@@ -210,32 +210,26 @@ int moe_b200_gated_ffn_backward(const void* grad_output, int64_t grad_pitch, con
   if (st != MOE_B200_OK) return st;
   const DenseOperand dy = rows_of(grad_output, T, H, grad_pitch);
   const DenseOperand dact = rows_of(workspace, T, 2 * I, 2 * I);
-  bool dependent = false;
+  // dh = dy W2, in its epilogue [du | dg], together with dW2 = dy^T h; then
+  // dx = [du | dg] W13 together with dW13 = [du | dg]^T x.
+  DenseProduct first[2], second[2];
+  int n1 = 0, n2 = 0;
   if (need_dact) {
-    // dh = dy W2, and in its epilogue [du | dg]
-    DenseParams p = params(d, T, I, H, dtype, activation, workspace, 2 * I, dtype);
-    p.preact = const_cast<float*>(preact);
-    st = launch_dense_pair(kEpiDact, dy, false, rows_of(w2, H, I, I), true, p, d.sm_count, dependent, s);
-    if (st != MOE_B200_OK) return st;
-    dependent = true;
+    first[n1] = {dy, rows_of(w2, H, I, I), false, params(d, T, I, H, dtype, activation, workspace, 2 * I, dtype)};
+    first[n1++].p.preact = const_cast<float*>(preact);
   }
-  if (grad_w2) {
-    st = launch_dense_pair(kEpiStore, dy, true, rows_of(hidden, T, I, I), true,
-                           params(d, H, I, T, dtype, activation, grad_w2, I, dtype), d.sm_count, dependent, s);
-    if (st != MOE_B200_OK) return st;
-    dependent = true;
-  }
-  if (grad_x) {
-    st = launch_dense_pair(kEpiStore, dact, false, rows_of(w13, 2 * I, H, H), true,
-                           params(d, T, H, 2 * I, dtype, activation, grad_x, H, dtype), d.sm_count, dependent, s);
+  if (grad_w2)
+    first[n1++] = {dy, rows_of(hidden, T, I, I), true, params(d, H, I, T, dtype, activation, grad_w2, I, dtype)};
+  if (grad_x)
+    second[n2++] = {dact, rows_of(w13, 2 * I, H, H), false, params(d, T, H, 2 * I, dtype, activation, grad_x, H, dtype)};
+  if (grad_w13)
+    second[n2++] = {dact, rows_of(x, T, H, x_pitch), true,
+                    params(d, 2 * I, H, T, dtype, activation, grad_w13, H, dtype)};
+  if (n1 > 0) {
+    st = launch_dense_backward(first, n1, d.sm_count, false, s);
     if (st != MOE_B200_OK) return st;
   }
-  if (grad_w13) {
-    st = launch_dense_pair(kEpiStore, dact, true, rows_of(x, T, H, x_pitch), true,
-                           params(d, 2 * I, H, T, dtype, activation, grad_w13, H, dtype), d.sm_count, dependent, s);
-    if (st != MOE_B200_OK) return st;
-  }
-  return MOE_B200_OK;
+  return n2 > 0 ? launch_dense_backward(second, n2, d.sm_count, true, s) : MOE_B200_OK;
 }
 
 size_t moe_b200_mxfp4_scale_bytes(int64_t rows, int64_t cols) {
