@@ -77,25 +77,23 @@ MxBuffers mx_place(uint8_t* at, int64_t rows, int64_t cols) {
 }
 
 int quantize(const void* x, int type, int64_t rows, int64_t cols, int64_t pitch, uint8_t* q, uint8_t* scale,
-             bool pad, cudaStream_t s) {
-  const int k_tiles = static_cast<int>(div_up(cols, 128));
-  const int64_t pad_rows = pad ? div_up(rows, 128) * 128 : rows;
-  const unsigned grid = static_cast<unsigned>(div_up(pad_rows * 4 * k_tiles, 256));
+             cudaStream_t s) {
   const int64_t pitch_bytes = pitch * (type == MOE_B200_TYPE_FP32 ? 4 : 2);
   const int vec32 = aligned(x, 32) && pitch_bytes % 32 == 0;
-  const uint8_t* src = static_cast<const uint8_t*>(x);
+  const int k_tiles = static_cast<int>(div_up(cols, 128));
+  const dim3 grid(static_cast<unsigned>(k_tiles), static_cast<unsigned>(div_up(rows, 128)));
   auto kern = type == MOE_B200_TYPE_BF16   ? mxfp4_quantize_kernel<kTypeBf16>
               : type == MOE_B200_TYPE_FP16 ? mxfp4_quantize_kernel<kTypeFp16>
                                            : mxfp4_quantize_kernel<kTypeFp32>;
-  kern<<<grid, 256, 0, s>>>(src, pitch_bytes, static_cast<int>(rows), static_cast<int>(cols / 32), k_tiles,
-                            static_cast<int>(pad_rows), vec32, q, scale);
+  kern<<<grid, 256, 0, s>>>(static_cast<const uint8_t*>(x), pitch_bytes, static_cast<int>(rows),
+                            static_cast<int>(cols / 32), k_tiles, vec32, q, scale);
   return cudaGetLastError() == cudaSuccess ? MOE_B200_OK : MOE_B200_ERR_CUDA;
 }
 
 // x [p->m, p->k] to 4 bits, in `to` or (`inside`) by the GEMM itself.
 int rows_to_4_bits(const void* x, int type, int64_t pitch, const MxBuffers& to, bool inside, DenseParams* p,
                    cudaStream_t s) {
-  if (!inside) return quantize(x, type, p->m, p->k, pitch, to.q, to.scale, false, s);
+  if (!inside) return quantize(x, type, p->m, p->k, pitch, to.q, to.scale, s);
   p->x_source = kFromRows;
   p->x = x;
   p->x_pitch = pitch * (type == MOE_B200_TYPE_FP32 ? 4 : 2);
@@ -249,7 +247,7 @@ int moe_b200_mxfp4_quantize(const void* x, int64_t x_pitch, int dtype, int64_t r
   Device d;
   const int st = open_device(&d);
   if (st != MOE_B200_OK) return st;
-  return quantize(x, dtype, rows, cols, x_pitch, static_cast<uint8_t*>(q), static_cast<uint8_t*>(scale), true,
+  return quantize(x, dtype, rows, cols, x_pitch, static_cast<uint8_t*>(q), static_cast<uint8_t*>(scale),
                   static_cast<cudaStream_t>(stream));
 }
 
@@ -350,7 +348,7 @@ int moe_b200_mxfp4_gated_ffn(const void* x, int64_t x_pitch, int dtype, const vo
     DenseParams p = params(d, T, I, H, dtype, activation, nullptr, 0, dtype);
     p.q = hq.q;
     p.q_scale = hq.scale;
-    st = quantize(x, dtype, T, H, x_pitch, xq.q, xq.scale, false, s);
+    st = quantize(x, dtype, T, H, x_pitch, xq.q, xq.scale, s);
     if (st != MOE_B200_OK) return st;
     st = launch_mx_pair(kEpiGatedQuant, xo, w13, p, d.sm_count, true, s);
     if (st != MOE_B200_OK) return st;

@@ -43,20 +43,47 @@ __device__ __forceinline__ void store_block(const float* v, bool live, bool padd
 
 }  // namespace
 
+// One CTA takes 128 rows x one exponent tile (four blocks). Its exponent
+// bytes meet in shared memory and leave as a whole 512-byte tile; written word
+// by word from CTAs of one row each they cost a tenth more transactions
+// (16384 x 7168 bf16 53.9 -> 45.0 us, all of the measured copy rate; with two
+// tiles a CTA 49 us). A thread's two blocks are loaded together.
 template <int kType>
-__global__ void __launch_bounds__(256)
-    mxfp4_quantize_kernel(const uint8_t* x, int64_t pitch, int rows, int blocks, int k_tiles, int pad_rows, int vec32,
-                          uint8_t* q, uint8_t* scale) {
+__global__ void __launch_bounds__(256, kType == kTypeFp32 ? 2 : 4)
+    mxfp4_quantize_kernel(const uint8_t* x, int64_t pitch, int rows, int blocks, int k_tiles, int vec32, uint8_t* q,
+                          uint8_t* scale) {
+  __shared__ __align__(16) uint8_t s_scale[512];
   pdl_launch_next();
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  const int per_row = 4 * k_tiles;
-  const int row = static_cast<int>(i / per_row);
-  const int block = static_cast<int>(i - static_cast<int64_t>(row) * per_row);
-  const bool live = row < rows && block < blocks;
-  float v[32];
-  if (live)
-    load_block<kType>(x + row * pitch + static_cast<int64_t>(block) * (kType == kTypeFp32 ? 128 : 64), vec32 != 0, v);
-  store_block(v, live, row < pad_rows, row, block, k_tiles, q + static_cast<int64_t>(row) * blocks * 16, scale);
+  constexpr int kBytes = kType == kTypeFp32 ? 128 : 64;
+  constexpr int kWords = kBytes / 4;
+  const int tid = static_cast<int>(threadIdx.x);
+  const int64_t row0 = static_cast<int64_t>(blockIdx.y) * 128 + tid / 4;   // and 64 rows further
+  const int block = static_cast<int>(blockIdx.x) * 4 + (tid & 3);
+  uint32_t raw[2][kWords];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int64_t row = row0 + 64 * j;
+    if (row < rows && block < blocks)
+      load_words<kWords>(x + row * pitch + static_cast<int64_t>(block) * kBytes, vec32 != 0, raw[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int64_t row = row0 + 64 * j;
+    uint32_t byte = 0;
+    if (row < rows && block < blocks) {
+      float v[32];
+      unpack_words<kType>(raw[j], v);
+      uint4 codes;
+      byte = mx_block(v, &codes);
+      *reinterpret_cast<uint4*>(q + (row * blocks + block) * 16) = codes;
+    }
+    const int r = tid / 4 + 64 * j;
+    s_scale[(r & 31) * 16 + (r >> 5) * 4 + (tid & 3)] = static_cast<uint8_t>(byte);
+  }
+  __syncthreads();
+  if (tid < 32)
+    *reinterpret_cast<uint4*>(scale + (static_cast<int64_t>(blockIdx.y) * k_tiles + blockIdx.x) * 512 + tid * 16) =
+        *reinterpret_cast<const uint4*>(s_scale + tid * 16);
 }
 
 // h = act(gate) * up of fp32 sums [rows, 2 n] (up, then gate), in 4 bits.
@@ -72,11 +99,11 @@ __global__ void __launch_bounds__(256)
   float v[32];
   if (live) {
     const float* up = sums + static_cast<int64_t>(row) * 64 * blocks + 32 * block;
-    float g[32];
-    load_block<kTypeFp32>(up, true, v);
-    load_block<kTypeFp32>(up + 32 * blocks, true, g);
+    uint32_t u[32], g[32];
+    load_words<32>(up, true, u);
+    load_words<32>(up + 32 * blocks, true, g);
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] *= act_value(g[j], act);
+    for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(u[j]) * act_value(__uint_as_float(g[j]), act);
   }
   store_block(v, live, row < rows, row, block, k_tiles, q + static_cast<int64_t>(row) * blocks * 16, scale);
 }
@@ -129,12 +156,9 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-template __global__ void mxfp4_quantize_kernel<kTypeBf16>(const uint8_t*, int64_t, int, int, int, int, int, uint8_t*,
-                                                          uint8_t*);
-template __global__ void mxfp4_quantize_kernel<kTypeFp16>(const uint8_t*, int64_t, int, int, int, int, int, uint8_t*,
-                                                          uint8_t*);
-template __global__ void mxfp4_quantize_kernel<kTypeFp32>(const uint8_t*, int64_t, int, int, int, int, int, uint8_t*,
-                                                          uint8_t*);
+template __global__ void mxfp4_quantize_kernel<kTypeBf16>(const uint8_t*, int64_t, int, int, int, int, uint8_t*, uint8_t*);
+template __global__ void mxfp4_quantize_kernel<kTypeFp16>(const uint8_t*, int64_t, int, int, int, int, uint8_t*, uint8_t*);
+template __global__ void mxfp4_quantize_kernel<kTypeFp32>(const uint8_t*, int64_t, int, int, int, int, uint8_t*, uint8_t*);
 template __global__ void mxfp4_dequantize_kernel<kTypeBf16>(const uint8_t*, const uint8_t*, int64_t, int, int, int,
                                                             uint8_t*);
 template __global__ void mxfp4_dequantize_kernel<kTypeFp16>(const uint8_t*, const uint8_t*, int64_t, int, int, int,

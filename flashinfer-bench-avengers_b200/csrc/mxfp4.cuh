@@ -11,11 +11,9 @@
 
 namespace moe {
 
-// 32 values of a block at `src` (16-byte aligned; whole sectors if vec32).
-template <int kType>
-__device__ __forceinline__ void load_block(const void* src, bool vec32, float* v) {
-  constexpr int kWords = kType == kTypeFp32 ? 32 : 16;
-  uint32_t r[kWords];
+// kWords 32-bit words at `src` (16-byte aligned; whole sectors if vec32).
+template <int kWords>
+__device__ __forceinline__ void load_words(const void* src, bool vec32, uint32_t* r) {
   if (vec32) {
 #pragma unroll
     for (int j = 0; j < kWords; j += 8) ld_global_32(r + j, static_cast<const uint32_t*>(src) + j);
@@ -26,8 +24,13 @@ __device__ __forceinline__ void load_block(const void* src, bool vec32, float* v
       r[j] = q.x, r[j + 1] = q.y, r[j + 2] = q.z, r[j + 3] = q.w;
     }
   }
+}
+
+// The 32 values of a block.
+template <int kType>
+__device__ __forceinline__ void unpack_words(const uint32_t* r, float* v) {
 #pragma unroll
-  for (int j = 0; j < kWords; ++j) {
+  for (int j = 0; j < (kType == kTypeFp32 ? 32 : 16); ++j) {
     if (kType == kTypeFp32) {
       v[j] = __uint_as_float(r[j]);
     } else {
@@ -53,11 +56,11 @@ __device__ __forceinline__ uint32_t mx_block(const float* v, uint4* codes) {
 }
 
 // rows x (32 * blocks) values, `pitch` bytes between rows, to codes and tiled
-// exponents. Exponents of rows up to pad_rows and of blocks up to
-// 4 * k_tiles are written as zero.
+// exponents (whole tiles: zero where no block is). Grid: (k_tiles, ceil(rows /
+// 128)).
 template <int kType>
-__global__ void mxfp4_quantize_kernel(const uint8_t* x, int64_t pitch, int rows, int blocks, int k_tiles, int pad_rows,
-                                      int vec32, uint8_t* q, uint8_t* scale);
+__global__ void mxfp4_quantize_kernel(const uint8_t* x, int64_t pitch, int rows, int blocks, int k_tiles, int vec32,
+                                      uint8_t* q, uint8_t* scale);
 __global__ void mxfp4_gate_kernel(const float* sums, int rows, int blocks, int k_tiles, int act, uint8_t* q,
                                   uint8_t* scale);
 template <int kType>

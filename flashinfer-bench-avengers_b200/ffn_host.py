@@ -131,8 +131,15 @@ def _activation(name: str) -> int:
     return act
 
 
-def _scratch(nbytes: int, dev: torch.device) -> torch.Tensor:
-    return torch.empty(nbytes, dtype=torch.uint8, device=dev)
+def _scratch(nbytes: int, x: torch.Tensor) -> torch.Tensor:
+    """Device memory beside x, in elements of x (cheaper to allocate than with
+    a type and a device to look up)."""
+    return x.new_empty(nbytes // x.element_size() + 1)
+
+
+def _mx_bytes(rows: int, cols: int) -> int:
+    """At least what a 4-bit matrix takes in a workspace, parts 256-byte aligned."""
+    return rows * cols // 2 + -(-rows // 128) * -(-cols // 128) * 512 + 1024
 
 
 def _call(name: str, dev: torch.device, *args) -> None:
@@ -255,10 +262,10 @@ def gated_ffn_backward(grad_output: torch.Tensor, x: torch.Tensor, w13: torch.Te
         raise RuntimeError("needs must be three truth values")
     grads = [x.new_empty(shape) if n else None for shape, n in zip(((T, H), (2 * inter, H), (H, inter)), needs)]
     if needs[0] or needs[1] or needs[2]:
-        ws = _scratch(4 * T * inter + 512, dev)
+        ws = _scratch(4 * T * inter + 1024, x)
         _call("moe_b200_gated_ffn_backward", dev, grad_output.data_ptr(), grad_pitch, x.data_ptr(), pitch,
               w13.data_ptr(), w2.data_ptr(), preact.data_ptr(), hidden.data_ptr(), TYPES[x.dtype], act, T, H, inter,
-              *(g.data_ptr() if g is not None else None for g in grads), ws.data_ptr(), ws.numel())
+              *(g.data_ptr() if g is not None else None for g in grads), ws.data_ptr(), ws.nbytes)
     return tuple(grads)
 
 
@@ -334,10 +341,11 @@ def _check_type(dtype) -> None:
         raise RuntimeError("dtype must be bfloat16, float16 or float32")
 
 
-def _mx_output(output, shape: tuple, dtype: torch.dtype, dev: torch.device) -> torch.Tensor:
+def _output(output, shape: tuple, x: torch.Tensor) -> torch.Tensor:
+    """``output`` checked, or a new tensor, of x's type."""
     if output is None:
-        return torch.empty(shape, dtype=dtype, device=dev)
-    _check_dense("output", output, shape, dtype, dev)
+        return x.new_empty(shape)
+    _check_dense("output", output, shape, x.dtype, x.device)
     return output
 
 
@@ -351,7 +359,10 @@ def mxfp4_matmul(a_q: torch.Tensor, a_scale: torch.Tensor, b_q: torch.Tensor, b_
         raise RuntimeError("b_q must have rows")
     _check_type(dtype)
     dev = a_q.device
-    output = _mx_output(output, (M, N), dtype, dev)
+    if output is None:
+        output = torch.empty((M, N), dtype=dtype, device=dev)
+    else:
+        _check_dense("output", output, (M, N), dtype, dev)
     if M:
         _call("moe_b200_mxfp4_matmul", dev, a_q.data_ptr(), a_scale.data_ptr(), b_q.data_ptr(), b_scale.data_ptr(),
               M, N, K, TYPES[dtype], output.data_ptr())
@@ -368,11 +379,11 @@ def mxfp4_linear(x: torch.Tensor, w_q: torch.Tensor, w_scale: torch.Tensor,
     N, _ = _check_mx("w_q", w_q, w_scale, dev, K)
     if N == 0:
         raise RuntimeError("w_q must have rows")
-    output = _mx_output(output, (T, N), x.dtype, dev)
+    output = _output(output, (T, N), x)
     if T:
-        ws = _scratch(_library().moe_b200_mxfp4_linear_workspace_bytes(T, K), dev)
+        ws = _scratch(_mx_bytes(T, K), x)
         _call("moe_b200_mxfp4_linear", dev, x.data_ptr(), pitch, TYPES[x.dtype], w_q.data_ptr(), w_scale.data_ptr(),
-              T, N, K, output.data_ptr(), ws.data_ptr(), ws.numel())
+              T, N, K, output.data_ptr(), ws.data_ptr(), ws.nbytes)
     return output
 
 
@@ -392,12 +403,12 @@ def mxfp4_gated_ffn(x: torch.Tensor, w13_q: torch.Tensor, w13_scale: torch.Tenso
         raise RuntimeError(f"w13_q must have 2 I rows, I a multiple of 32; got {two_i}")
     _check_dim("the intermediate size", inter, 32)
     _check_mx("w2_q", w2_q, w2_scale, dev, inter, H)
-    output = _mx_output(output, (T, H), x.dtype, dev)
+    output = _output(output, (T, H), x)
     if T:
-        ws = _scratch(_library().moe_b200_mxfp4_gated_ffn_workspace_bytes(T, H, inter), dev)
+        ws = _scratch(_mx_bytes(T, H) + _mx_bytes(T, inter) + 8 * T * inter + 1024, x)
         _call("moe_b200_mxfp4_gated_ffn", dev, x.data_ptr(), pitch, TYPES[x.dtype], w13_q.data_ptr(),
               w13_scale.data_ptr(), w2_q.data_ptr(), w2_scale.data_ptr(), act, T, H, inter, output.data_ptr(),
-              ws.data_ptr(), ws.numel())
+              ws.data_ptr(), ws.nbytes)
     return output
 
 
