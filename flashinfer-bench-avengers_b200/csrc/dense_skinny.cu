@@ -261,29 +261,22 @@ __global__ void __launch_bounds__(kThreads)
     const uint32_t lo_x0 = desc_lo_kmajor(base + (kQuantX ? sh.xq_off : kWeightTile));
     const uint32_t lo_sx0 = kQuantX ? desc_lo_scale(base + sh.xq_off + sh.xq_iters * sh.bn * 128)
                                     : lo_s0 + 64;
-    int stage = 0, old = sh.stages - 2;   // 4-bit: the stage before last, and its phase
-    uint32_t ph = 0, old_ph = 1, sf = 0;
+    int stage = 0;
+    uint32_t ph = 0;
     bool ok = !kQuantX || warp_wait(smem_u32(xq_bar), 0, s_abort, p.status, kStatusTimeoutMma);
     for (int i = 0; ok && i < iters; ++i) {
       if (!warp_wait(smem_u32(full_bar) + 8u * stage, ph, s_abort, p.status, kStatusTimeoutMma)) break;
       const uint32_t off = static_cast<uint32_t>(stage * (sh.stage_bytes >> 4));
       const uint32_t lo_w = lo_w0 + off;
       const uint32_t lo_x = lo_x0 + (kQuantX ? static_cast<uint32_t>(i * sh.bn * 8) : off);
-      if constexpr (kMx) {
-        // these exponent columns were last read two stages ago (the first
-        // two waits pass at once)
-        if (!warp_wait(smem_u32(empty_bar) + 8u * old, old_ph, s_abort, p.status, kStatusTimeoutMma)) break;
-        if (++old == sh.stages) {
-          old = 0;
-          old_ph ^= 1u;
-        }
-      }
       tc_fence_after();
       if (issue) {
         if constexpr (kMx) {
           const uint32_t lo_s = lo_s0 + off;
           const uint32_t lo_sx = lo_sx0 + (kQuantX ? static_cast<uint32_t>(i * 64) : off);
-          const uint32_t sfw = tmem + sh.bn + sf;
+          // each stage has its own exponent columns: a stage that is full
+          // again has been read
+          const uint32_t sfw = tmem + sh.bn + 16 * stage;
           const uint32_t sfx = sfw + 8;
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
@@ -305,7 +298,6 @@ __global__ void __launch_bounds__(kThreads)
         if (i == iters - 1) umma_commit(smem_u32(done_bar));
       }
       __syncwarp();
-      sf ^= 16u;
       if (++stage == sh.stages) {
         stage = 0;
         ph ^= 1u;
@@ -478,7 +470,7 @@ SkinnyShape choose_shape(const DenseParams& p, bool mx, bool gate, bool quant_x,
   const int red = sh.bn * 512;           // the partial sums reuse the stages
   if (bytes < red) bytes = red;
   sh.smem_bytes = bytes + kExtra;
-  const int cols = sh.bn + (mx ? 32 : 0);
+  const int cols = sh.bn + (mx ? 16 * sh.stages : 0);   // at most 128 + 6 * 16 or 64 + 12 * 16
   sh.tmem_cols = 32;
   while (sh.tmem_cols < cols) sh.tmem_cols *= 2;
   return sh;
