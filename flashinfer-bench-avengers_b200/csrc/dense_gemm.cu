@@ -22,6 +22,11 @@
 // gradients need W^T and X^T): the shared-memory descriptors take both, so
 // nothing is transposed in memory.
 //
+// Where the tiles of a forward product are few, their K range is split over 2
+// or 4 pairs of one cluster: the partial tiles meet through distributed shared
+// memory, each CTA adding the parts of its share of the rows in a fixed order
+// (block at 256 tokens 44.5 -> 35.8 us, at 512 49.5 -> 46.4 us).
+//
 // One launch takes up to two products whose tiles follow one another in the
 // walk. The backward pass has two pairs of products that do not depend on
 // each other (dh with dW2, dx with dW13): together they fill their last waves
@@ -89,6 +94,7 @@ struct DenseGroup {
   int tiles0;        // tiles of the first
   int tiles;         // of both
   int stages, stage_bytes;
+  int splits;        // pairs of a cluster that share a tile's K range
 };
 
 // Tensor maps: A, B of the first product, then of the second; 4-bit: A, B and
@@ -236,6 +242,77 @@ __device__ __forceinline__ void store_dact(const DenseParams& p, int64_t row, in
   store_row16(out + p.n, col, end, dg, p.vec32);
 }
 
+// K steps of split s begin here.
+__device__ __forceinline__ int k_begin(int k_iters, int s, int splits) {
+  return splits == 1 ? s * k_iters : k_iters * s / splits;
+}
+
+// Floats between the rows of a partial tile: 256 columns and a 16-byte shift,
+// so that threads writing different rows do not meet in a bank.
+constexpr int kPartPitch = 260;
+static_assert(128 * kPartPitch * 4 <= kRingBytes, "partial tile");
+
+// A CTA's share of its 128 rows of the cluster's tile: eight columns per
+// thread, the parts of all pairs requested together and added in a fixed
+// order (its own pair's first), then the epilogue.
+template <int kEpi>
+__device__ __forceinline__ void add_parts(const DenseParams& p, const Work& w, uint32_t smem, uint32_t rank, int split,
+                                          int splits) {
+  constexpr bool kGate = kEpi == kEpiGated;
+  const int rows = 128 / splits;
+  const int width = kGate ? p.n_step : p.bn;
+  const int eighths = width / 8;
+  uint32_t part[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+    part[q] = q < splits ? map_to_cta(smem, 2 * ((split + q) & (splits - 1)) + rank) : 0u;
+  auto sums = [&](int row, int c, uint32_t* out) {
+    float4 a[4][2];
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (q < splits) {
+        a[q][0] = ld_cluster_f32x4(part[q] + (row * kPartPitch + c) * 4);
+        a[q][1] = ld_cluster_f32x4(part[q] + (row * kPartPitch + c + 4) * 4);
+      }
+    float4 lo = a[0][0], hi = a[0][1];
+#pragma unroll
+    for (int q = 1; q < 4; ++q)
+      if (q < splits) {
+        lo.x += a[q][0].x, lo.y += a[q][0].y, lo.z += a[q][0].z, lo.w += a[q][0].w;
+        hi.x += a[q][1].x, hi.y += a[q][1].y, hi.z += a[q][1].z, hi.w += a[q][1].w;
+      }
+    out[0] = __float_as_uint(lo.x), out[1] = __float_as_uint(lo.y), out[2] = __float_as_uint(lo.z);
+    out[3] = __float_as_uint(lo.w), out[4] = __float_as_uint(hi.x), out[5] = __float_as_uint(hi.y);
+    out[6] = __float_as_uint(hi.z), out[7] = __float_as_uint(hi.w);
+  };
+  for (int i = static_cast<int>(threadIdx.x); i < rows * eighths; i += kPairThreads) {
+    const int r = split * rows + i / eighths;
+    const int c = i % eighths * 8;
+    const int64_t row = static_cast<int64_t>(w.m0) + rank * 128 + r;
+    const int col = w.n0 + c;
+    if (row >= p.m || col >= p.n) continue;
+    uint32_t v[8];
+    sums(r, c, v);
+    if constexpr (kGate) {
+      uint32_t g[8];
+      sums(r, p.n_step + c, g);
+      if (p.preact != nullptr) {
+        float* pre = p.preact + row * (2 * static_cast<int64_t>(p.n)) + col;
+        st_global_32(pre, v);
+        st_global_32(pre + p.n, g);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        v[j] = __float_as_uint(act_value(__uint_as_float(g[j]), p.act) * __uint_as_float(v[j]));
+    }
+    uint32_t out[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) out[j] = pack_16(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]), p.out_type);
+    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + row * p.ldo + col) =
+        make_uint4(out[0], out[1], out[2], out[3]);
+  }
+}
+
 // 4-bit: the columns the next accumulator needs are in registers.
 __device__ __forceinline__ void release_early(uint64_t* acce_bar, int lane) {
   tc_fence_before();
@@ -246,7 +323,7 @@ __device__ __forceinline__ void release_early(uint64_t* acce_bar, int lane) {
 }  // namespace
 
 template <bool kMx, bool kBMn, int kEpi>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+__global__ void __launch_bounds__(kPairThreads, 1)
     dense_pair_kernel(const __grid_constant__ PairMaps maps, const __grid_constant__ DenseGroup grp) {
   using Tr = PairTraits<kMx>;
   constexpr bool kGate = kEpi == kEpiGated || kEpi == kEpiGatedQuant;
@@ -265,9 +342,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  const uint32_t rank = cluster_cta_rank();
-  const int pair = blockIdx.x >> 1;
-  const int pairs = gridDim.x >> 1;
+  // Clusters of one pair walk the tiles; with K split, a cluster of several
+  // pairs takes one tile, `split` telling its pairs apart.
+  constexpr bool kSplits = !kMx && (kEpi == kEpiStore || kEpi == kEpiGated);
+  const int splits = kSplits ? grp.splits : 1;
+  const uint32_t cta = cluster_cta_rank();
+  const uint32_t rank = cta & 1u;
+  const uint32_t lead = cta & ~1u;
+  const int split = static_cast<int>(cta >> 1);
+  const uint32_t pair_mask = 3u << lead;
+  const int pair = static_cast<int>(blockIdx.x) / (2 * splits);
+  const int pairs = static_cast<int>(gridDim.x) / (2 * splits);
   const int tiles = grp.tiles;
   uint32_t* const status = grp.p[0].status;
 
@@ -305,7 +390,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     const bool issue = elect_lane();
     const uint32_t base = smem_u32(smem);
     const uint32_t full0 = smem_u32(full_bar);
-    const uint32_t full0_pair = map_to_cta(full0, 0);
+    const uint32_t full0_pair = map_to_cta(full0, lead);
     // B's part of a stage, and the count of bytes both CTAs' parts bring.
     auto load_b = [&](const Work& w, int kb, int stage) {
       const DenseParams& p = grp.p[w.g];
@@ -347,9 +432,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     // B is an input of the whole call (weights, or saved by another call):
     // its part of the first ring does not wait for the predecessor.
     const Work w0 = work_at<kGrouped>(pair, grp);
-    const int early = min(kS, grp.p[w0.g].k_iters);
+    const int first = k_begin(grp.p[w0.g].k_iters, split, splits);
+    const int early = min(kS, k_begin(grp.p[w0.g].k_iters, split + 1, splits) - first);
     if (issue)
-      for (int kb = 0; kb < early; ++kb) load_b(w0, kb, kb);
+      for (int i = 0; i < early; ++i) load_b(w0, first + i, i);
     __syncwarp();
     pdl_wait();
     int stage = 0;
@@ -357,9 +443,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     bool ok = true;
     for (int t = pair; ok && t < tiles; t += pairs) {
       const Work w = work_at<kGrouped>(t, grp);
-      const int k_iters = grp.p[w.g].k_iters;
-      const int skip = t == pair ? early : 0;   // K steps whose B is on its way already
-      for (int kb = 0; kb < k_iters; ++kb) {
+      const int kb0 = k_begin(grp.p[w.g].k_iters, split, splits);
+      const int kb1 = k_begin(grp.p[w.g].k_iters, split + 1, splits);
+      const int skip = kb0 + (t == pair ? early : 0);   // K steps whose B is on its way already
+      for (int kb = kb0; kb < kb1; ++kb) {
         if (kb >= skip &&
             !warp_wait(smem_u32(empty_bar) + 8u * stage, ph ^ 1u, s_abort, status, kStatusTimeoutProducer)) {
           ok = false;
@@ -397,7 +484,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         const uint32_t idesc1 = kMx ? idesc_mxf4(256, 256, 2) : idesc0;
         const uint32_t lo_a0 = a_mn ? desc_lo_mnmajor(base) : desc_lo_kmajor(base);
         const uint32_t a_step = a_mn ? 128 : 2;
-        const int k_iters = p.k_iters;
+        const int kb0 = k_begin(p.k_iters, split, splits), kb1 = k_begin(p.k_iters, split + 1, splits);
         const int buf = it & 1;
         const uint32_t d = tmem + (buf ? Tr::kAcc1 : 0);
         if (kMx ? it >= 1 : it >= 2) {
@@ -406,7 +493,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           if (!__all_sync(0xffffffffu, mbar_wait_cluster(bar, par, s_abort, status, kStatusTimeoutMma))) break;
           tc_fence_after();
         }
-        for (int kb = 0; kb < k_iters; ++kb) {
+        for (int kb = kb0; kb < kb1; ++kb) {
           if (!warp_wait(smem_u32(full_bar) + 8u * stage, ph, s_abort, status, kStatusTimeoutMma)) {
             ok = false;
             break;
@@ -447,10 +534,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 #pragma unroll
               for (int k = 0; k < 4; ++k)
                 umma_f16<2>(d, desc_of(kDescHiSw128, lo_a + a_step * k),
-                            desc_of(kDescHiSw128, lo_b + (kBMn ? 128 : 2) * k), idesc0, kb | k);
+                            desc_of(kDescHiSw128, lo_b + (kBMn ? 128 : 2) * k), idesc0, (kb - kb0) | k);
             }
-            umma_commit_pair(smem_u32(empty_bar) + 8u * stage);
-            if (kb == k_iters - 1) umma_commit_pair(smem_u32(&accf_bar[buf]));
+            umma_commit_pair(smem_u32(empty_bar) + 8u * stage, pair_mask);
+            if (kb == kb1 - 1) umma_commit_pair(smem_u32(&accf_bar[buf]), pair_mask);
           }
           __syncwarp();
           sf ^= 24u;
@@ -489,6 +576,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       if (!__all_sync(0xffffffffu, ready)) break;
       tc_fence_after();
       const uint32_t acc = lanes + (buf ? Tr::kAcc1 : 0);
+      if (splits > 1) {
+        // this pair's part of the sums, one row per thread, over the drained ring
+        float* part = reinterpret_cast<float*>(smem) + (quarter * 32 + lane) * kPartPitch;
+        for (int c = 32 * half; c < p.bn; c += 64) {
+          uint32_t r[32];
+          tmem_ld32(acc + c, r);
+          tmem_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 32; j += 4)
+            *reinterpret_cast<uint4*>(part + c + j) = make_uint4(r[j], r[j + 1], r[j + 2], r[j + 3]);
+        }
+        break;
+      }
       for (int i = half; i < chunks; i += 2) {
         // 4-bit operands: the columns shared with the other accumulator first
         const int c = 32 * (kMx && buf == 0 ? chunks - 1 - i : i);
@@ -520,11 +620,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       if (!kMx) {
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&acce_bar[buf]), 0));
+        if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&acce_bar[buf]), lead));
       }
     }
   }
 
+  if constexpr (kSplits) {
+    if (splits > 1) {
+      __syncwarp();
+      cluster_sync();   // every pair's part is there
+      if (*s_abort == 0) add_parts<kEpi>(grp.p[0], work_at<false>(pair, grp), smem_u32(smem), rank, split, splits);
+    }
+  }
   // No CTA leaves while the other may still reach its shared or tensor memory.
   __syncwarp();
   tc_fence_before();
@@ -551,38 +658,93 @@ int launch_pair(const PairMaps& maps, const DenseGroup& grp, int sm_count, bool 
         return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) == cudaSuccess;
       }))
     return MOE_B200_ERR_CUDA;
-  const int pairs = grp.tiles < sm_count / 2 ? grp.tiles : sm_count / 2;
-  return launch_kernel(kern, 2 * pairs, kPairThreads, smem, s, dependent, maps, grp) == cudaSuccess
-             ? MOE_B200_OK
-             : MOE_B200_ERR_CUDA;
+  const int pairs = grp.splits > 1 ? grp.tiles * grp.splits : grp.tiles < sm_count / 2 ? grp.tiles : sm_count / 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(2 * pairs));
+  cfg.blockDim = dim3(kPairThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(2 * grp.splits);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = dependent ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kern, maps, grp) == cudaSuccess ? MOE_B200_OK : MOE_B200_ERR_CUDA;
 }
 
 // Time units of a tile of bn columns: a K step costs an MMA 2 N cycles and the
 // loads 256 + N (A's 128 rows and N / 2 rows of B per CTA; at about 64 bytes a
 // cycle from L2 the two meet at N = 256; B stored along N comes in 64-column
-// atoms whatever N is); a tile's start and epilogue cost about 1500 more.
-int64_t tile_cost(const DenseParams& p, int bn, bool b_mn) {
-  const int64_t load = 256 + (b_mn ? (bn > 128 ? 256 : 128) : bn), mma = 2 * bn;
-  return div_up(p.k, 64) * (load > mma ? load : mma) + 1500;
+// atoms whatever N is), and about 400 to issue; a tile's start and epilogue
+// cost about 700 + 4 N more.
+int64_t tile_cost(const DenseParams& p, int bn, bool b_mn, int splits = 1) {
+  int64_t step = 256 + (b_mn ? (bn > 128 ? 256 : 128) : bn);
+  if (step < 2 * bn) step = 2 * bn;
+  if (step < 400) step = 400;
+  return div_up(div_up(p.k, 64), splits) * step + 700 + 4 * bn;
 }
 
 int64_t tile_count(const DenseParams& p, int step) { return div_up(p.m, 256) * div_up(p.n, step); }
 
-// Columns per tile (the MMA's N) of one product: the fewest time units over
-// all waves of tiles. Against 256 throughout: training step at 4096 tokens
-// 813 -> 786 us, at 333 x 1032 x 520 75 -> 55 us. The columns of a tile come
-// in whole 32-byte stores, so 16 features.
-int choose_bn(const DenseParams& p, bool gate, int pairs) {
-  int best = 256;
+// Clusters of `ctas` (4 or 8) that run at once on the current device; 0 if that
+// cannot be told.
+int max_clusters(int ctas) {
+  static std::atomic<int> known[2][64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  std::atomic<int>& slot = known[ctas == 8][dev];
+  int n = slot.load(std::memory_order_relaxed);
+  if (n == 0) {
+    auto kern = dense_pair_kernel<false, false, kEpiGated>;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(ctas));
+    cfg.blockDim = dim3(kPairThreads);
+    cfg.dynamicSmemBytes = kPairSmem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(ctas);
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess)
+      return 0;
+    slot.store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
+// Columns per tile (the MMA's N) and K splits of one product: the fewest time
+// units over all waves of tiles. Choosing the columns, against 256 throughout:
+// training step at 4096 tokens 813 -> 786 us, at 333 x 1032 x 520 75 -> 55 us.
+// The columns of a tile come in whole 32-byte stores, so 16 features. A split
+// product is one wave of clusters and adds its parts for kAddCost. (How many
+// clusters of 4 or 8 CTAs run at once depends on how the GPU's SMs are
+// grouped, 33 and 15 where this was measured; one more made 256 tokens take 56
+// us.)
+void choose_shape(DenseGroup* grp, bool gate, int sm_count) {
+  constexpr int64_t kAddCost = 6000;
+  DenseParams& p = grp->p[0];
   int64_t best_cost = INT64_MAX;
-  for (int bn = 256; bn >= 64; bn -= gate ? 32 : 16) {
-    const int64_t cost = div_up(tile_count(p, gate ? bn / 2 : bn), pairs) * tile_cost(p, bn, false);
-    if (cost < best_cost) {
-      best_cost = cost;
-      best = bn;
+  for (int splits = 1; splits <= 4; splits *= 2) {
+    if (splits > 1 && div_up(p.k, 64) < 4 * splits) break;
+    for (int bn = 256; bn >= 64; bn -= gate ? 32 : 16) {
+      const int64_t tiles = tile_count(p, gate ? bn / 2 : bn);
+      if (splits > 1 && tiles > max_clusters(2 * splits)) continue;
+      const int64_t waves = splits > 1 ? 1 : div_up(tiles, sm_count / 2);
+      const int64_t cost = waves * tile_cost(p, bn, false, splits) + (splits > 1 ? kAddCost : 0);
+      if (cost < best_cost) {
+        best_cost = cost;
+        p.bn = bn;
+        grp->splits = splits;
+      }
     }
   }
-  return best;
 }
 
 // The same for two products walked one after the other: the busiest pair is
@@ -624,9 +786,10 @@ int launch_dense_pair(DenseEpi epi, const DenseOperand& a, const DenseOperand& b
   const bool gate = epi == kEpiGated;
   DenseGroup grp;
   std::memset(&grp, 0, sizeof(grp));
+  grp.splits = 1;
   DenseParams& p = grp.p[0];
   p = params;
-  p.bn = choose_bn(p, gate, sm_count / 2);
+  choose_shape(&grp, gate, sm_count);
   finish(&p, gate, false);
   p.vec32 = aligned(p.out, 32) && (p.ldo * 2) % 32 == 0;
   grp.tiles0 = grp.tiles = p.m_tiles * p.n_tiles;
@@ -643,6 +806,7 @@ int launch_dense_pair(DenseEpi epi, const DenseOperand& a, const DenseOperand& b
 int launch_dense_backward(const DenseProduct* products, int count, int sm_count, bool dependent, cudaStream_t s) {
   DenseGroup grp;
   std::memset(&grp, 0, sizeof(grp));
+  grp.splits = 1;
   for (int i = 0; i < count; ++i) grp.p[i] = products[i].p;
   if (count == 1) {
     // with no second product its cost and tiles are zero
@@ -684,6 +848,7 @@ int launch_mx_pair(DenseEpi epi, const MxOperand& a, const MxOperand& b, const D
   const bool gate = epi == kEpiGatedQuant;
   DenseGroup grp;
   std::memset(&grp, 0, sizeof(grp));
+  grp.splits = 1;
   DenseParams& p = grp.p[0];
   p = params;
   p.bn = 256;

@@ -127,12 +127,12 @@ __device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols
   asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
 }
 
-// Arrives on the barrier at this offset in both CTAs once every tcgen05
-// operation this thread issued so far is done.
-__device__ __forceinline__ void umma_commit_pair(uint32_t bar) {
+// Arrives on the barrier at this offset in the CTAs of `mask` once every
+// tcgen05 operation this thread issued so far is done.
+__device__ __forceinline__ void umma_commit_pair(uint32_t bar, uint32_t mask) {
   asm volatile(
       "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
-      "h"(static_cast<uint16_t>(3))
+      "h"(static_cast<uint16_t>(mask))
       : "memory");
 }
 

@@ -20,9 +20,11 @@ def _inputs(T, H, inter, dtype, seed=0, device="cuda"):
 
 # one token to several tiles; sizes that end inside a tile in every direction
 # (token tiles of 16, 128 and 256, feature tiles of 64 and 128, 64-wide K
-# steps), the smallest sizes, and the split of K over 1 to 8 CTAs
+# steps), the smallest sizes, and the split of K over 1 to 8 CTAs and over 1,
+# 2 and 4 pairs
 SHAPES = [(1, 8, 8), (1, 7168, 2048), (3, 64, 64), (16, 520, 264), (17, 1032, 520), (64, 2048, 136), (65, 4096, 64),
-          (127, 72, 1000), (128, 256, 128), (129, 256, 128), (255, 136, 72), (257, 1032, 520), (600, 512, 1048)]
+          (127, 72, 1000), (128, 256, 128), (129, 256, 128), (255, 136, 72), (257, 1032, 520), (600, 512, 1048),
+          (130, 3200, 264), (256, 7168, 2048), (301, 2056, 1032), (513, 4104, 200)]
 
 
 @pytest.mark.gpu
