@@ -10,13 +10,21 @@
 // tile run under the MMAs of the next.
 //
 // Roles per CTA: warp 0 TMA producer, warp 1 MMA issuer (of the pair's first
-// CTA only), warp 2 owns tensor memory, warps 4-7 epilogue, one 32-lane
-// quarter of the accumulator each. The pair's loads all count on the first
+// CTA only), warp 2 owns tensor memory, warps 4-11 epilogue, two to each
+// 32-lane quarter of the accumulator. The pair's loads all count on the first
 // CTA's `full` barrier; its commits free the stage in both CTAs.
 //
 // Each epilogue thread owns an output row and writes 32-byte sectors: full
 // sectors need no staging through shared memory, and L2 merges a row's
 // sectors before they reach HBM.
+//
+// What bounds it (4096 tokens, H = 7168, I = 2048): a K step of a 256 x 256
+// tile takes 550 cycles, 512 of them MMA; the loads are then 60 bytes a cycle
+// and SM, 14 TB/s over the GPU, which is all that L2 gave the same loads
+// without MMAs. Under sustained load the power cap sets the clock (1.1 to 1.5
+// GHz), and the rate is that of the vendor's library GEMM on the same
+// operands. 4-bit operands need the same bytes per step, so their MMAs, at
+// four times the rate, reach 5.6 PFLOP/s.
 //
 // The operands may be stored along K or along the output dimension (the
 // gradients need W^T and X^T): the shared-memory descriptors take both, so

@@ -473,10 +473,15 @@ SkinnyShape choose_shape(const DenseParams& p, bool mx, bool gate, bool quant_x,
   int bytes = sh.xq_off + xq_bytes;
   const int red = (sh.bn + 1) * 512;           // the partial sums reuse the stages
   if (bytes < red) bytes = red;
-  sh.smem_bytes = bytes + kExtra;
   const int cols = sh.bn + (mx ? 16 * sh.stages : 0);   // at most 128 + 6 * 16 or 64 + 12 * 16
   sh.tmem_cols = 32;
   while (sh.tmem_cols < cols) sh.tmem_cols *= 2;
+  // At least the share of the SM's shared memory that its tensor memory is of
+  // the 512 columns: CTAs that fit an SM together then always find their
+  // columns free. Clusters whose CTAs held columns on one SM and waited for
+  // them on another could otherwise wait for each other.
+  const int least = sh.tmem_cols * (228 * 1024 / 512) - 1024;
+  sh.smem_bytes = bytes + kExtra < least ? least : bytes + kExtra;
   return sh;
 }
 

@@ -51,10 +51,6 @@ __device__ __forceinline__ float2 unpack_16(uint32_t bits, int type) {
   return __half22float2(*reinterpret_cast<const __half2*>(&bits));
 }
 
-__device__ __forceinline__ uint16_t round_16(float v, int type) {
-  return static_cast<uint16_t>(pack_16(v, 0.0f, type) & 0xffffu);
-}
-
 // ------------------------------------------------- 4-bit microscaled blocks
 // Exponent byte of a block from the largest magnitude's bits: floor(log2) - 2
 // (the largest e2m1 exponent), biased by 127, at least 0. Infinities and
@@ -81,18 +77,6 @@ __device__ __forceinline__ uint32_t mx_pack8(const float* v, float inv) {
       : "=r"(r)
       : "f"(v[0] * inv), "f"(v[1] * inv), "f"(v[2] * inv), "f"(v[3] * inv), "f"(v[4] * inv), "f"(v[5] * inv),
         "f"(v[6] * inv), "f"(v[7] * inv));
-  return r;
-}
-
-// Four values, into the low 16 bits.
-__device__ __forceinline__ uint32_t mx_pack4(const float* v, float inv) {
-  uint16_t r;
-  asm("{\n\t.reg .b8 t0, t1;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 t0, %2, %1;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 t1, %4, %3;\n\t"
-      "mov.b16 %0, {t0, t1};\n\t}"
-      : "=h"(r)
-      : "f"(v[0] * inv), "f"(v[1] * inv), "f"(v[2] * inv), "f"(v[3] * inv));
   return r;
 }
 

@@ -5,11 +5,10 @@
 // the largest magnitude) - 2, its elements the nearest e2m1 numbers (ties to
 // even, beyond 6 to 6) to x / 2^exponent; scaling by a power of two is exact,
 // so the only rounding is the 4-bit one. All three kernels give one thread
-// one block: it reads whole 32-byte sectors and holds the block in registers,
-// so the block maximum needs no exchange between threads, and a warp writes
-// 512 contiguous bytes of codes. Four neighbouring threads' exponent bytes
-// are one word of the tiled array. Bound by HBM: 2 (or 4) bytes in and 17/32
-// byte out per element.
+// whole blocks: it reads whole 32-byte sectors and holds the block in
+// registers, so the block maximum needs no exchange between threads. Bound by
+// HBM: 2 (or 4) bytes in and 17/32 byte out per element; 16384 x 7168 bf16 at
+// 6.6 TB/s (quantiser) and 6.2 TB/s (dequantiser).
 #include <cuda_runtime.h>
 
 #include <cstdint>
