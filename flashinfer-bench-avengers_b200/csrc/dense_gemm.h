@@ -42,6 +42,7 @@ struct DenseParams {
   int out_type;        // type code of `out`
   void* out;           // [m, n], row pitch ldo elements; [du | dg]: [m, 2 n]
   int64_t ldo;
+  void* out_lo;        // kEpiGated, streaming form: h - out, rounded again, when set
   float* preact;       // fp32 [m, 2 n]: written by kEpiGated when set, read by kEpiBackward
   uint8_t* q;          // kEpiGatedQuant: codes [m, n / 2]
   uint8_t* q_scale;    //   and tiled exponents
@@ -84,8 +85,11 @@ int launch_mx_pair(DenseEpi epi, const MxOperand& a, const MxOperand& b, const D
 
 // Few rows of A: out = A B^T streaming B, K split over a cluster
 // (kEpiStore and kEpiGated; 4-bit: kEpiStore).
-int launch_dense_skinny(DenseEpi epi, const DenseOperand& a, const DenseOperand& b, DenseParams p, int sm_count,
-                        bool dependent, cudaStream_t s);
+// With a_lo set the operand is the sum of the two matrices a and a_lo (at most
+// kTwoPartRows rows).
+constexpr int64_t kTwoPartRows = 16;
+int launch_dense_skinny(DenseEpi epi, const DenseOperand& a, const void* a_lo, const DenseOperand& b, DenseParams p,
+                        int sm_count, bool dependent, cudaStream_t s);
 int launch_mx_skinny(const MxOperand& a, const MxOperand& b, DenseParams p, int sm_count, bool dependent,
                      cudaStream_t s);
 

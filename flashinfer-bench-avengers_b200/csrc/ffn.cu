@@ -52,9 +52,9 @@ DenseOperand rows_of(const void* base, int64_t rows, int64_t cols, int64_t pitch
 }
 
 // ---- the forward GEMMs: out = x w^T, gated or plain ------------------------
-int forward_gemm(DenseEpi epi, const DenseOperand& x, const DenseOperand& w, const DenseParams& p, const Device& d,
-                 bool dependent, cudaStream_t s) {
-  if (p.m <= kSkinnyMaxTokens) return launch_dense_skinny(epi, x, w, p, d.sm_count, dependent, s);
+int forward_gemm(DenseEpi epi, const DenseOperand& x, const void* x_lo, const DenseOperand& w, const DenseParams& p,
+                 const Device& d, bool dependent, cudaStream_t s) {
+  if (p.m <= kSkinnyMaxTokens) return launch_dense_skinny(epi, x, x_lo, w, p, d.sm_count, dependent, s);
   return launch_dense_pair(epi, x, w, p, d.sm_count, dependent, s);
 }
 
@@ -141,7 +141,9 @@ extern "C" {
 
 size_t moe_b200_gated_ffn_workspace_bytes(int64_t num_tokens, int64_t hidden_size, int64_t inter_size) {
   if (!tokens_ok(num_tokens) || !dim_ok(hidden_size, 8) || !dim_ok(inter_size, 8)) return 0;
-  return round256(static_cast<size_t>(num_tokens) * inter_size * 2) + 256;
+  // the hidden, and what its rounding left
+  const size_t hidden = round256(static_cast<size_t>(num_tokens) * inter_size * 2);
+  return (num_tokens <= kTwoPartRows ? 2 : 1) * hidden + 256;
 }
 
 int moe_b200_gated_ffn(const void* x, int64_t x_pitch, const void* w13, const void* w2, int dtype, int activation,
@@ -152,22 +154,27 @@ int moe_b200_gated_ffn(const void* x, int64_t x_pitch, const void* w13, const vo
       !pitch_ok(x_pitch, H))
     return MOE_B200_ERR_INVALID_ARGUMENT;
   if (T == 0) return MOE_B200_OK;
-  if (!x || !w13 || !w2 || !output || (!hidden && !workspace)) return MOE_B200_ERR_INVALID_ARGUMENT;
+  const bool two_part = T <= kTwoPartRows;
+  const bool need_workspace = !hidden || two_part;
+  if (!x || !w13 || !w2 || !output || (need_workspace && !workspace)) return MOE_B200_ERR_INVALID_ARGUMENT;
   if (!aligned(x, 16) || !pitch_aligned(x_pitch, 2) || !aligned(w13, 16) || !aligned(w2, 16) || !aligned(output, 16) ||
       !aligned(preact, 32) || !aligned(hidden, 16) || !aligned(workspace, 256))
     return MOE_B200_ERR_MISALIGNED;
-  if (!hidden && workspace_bytes < moe_b200_gated_ffn_workspace_bytes(T, H, I))
+  if (need_workspace && workspace_bytes < moe_b200_gated_ffn_workspace_bytes(T, H, I))
     return MOE_B200_ERR_WORKSPACE_TOO_SMALL;
   Device d;
   int st = open_device(&d);
   if (st != MOE_B200_OK) return st;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  void* h = hidden ? hidden : workspace;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  void* h = hidden ? hidden : ws;
+  void* h_lo = two_part ? ws + round256(static_cast<size_t>(T) * I * 2) : nullptr;
   DenseParams p = params(d, T, I, H, dtype, activation, h, I, dtype);
   p.preact = preact;
-  st = forward_gemm(kEpiGated, rows_of(x, T, H, x_pitch), rows_of(w13, 2 * I, H, H), p, d, false, s);
+  p.out_lo = h_lo;
+  st = forward_gemm(kEpiGated, rows_of(x, T, H, x_pitch), nullptr, rows_of(w13, 2 * I, H, H), p, d, false, s);
   if (st != MOE_B200_OK) return st;
-  return forward_gemm(kEpiStore, rows_of(h, T, I, I), rows_of(w2, H, I, I),
+  return forward_gemm(kEpiStore, rows_of(h, T, I, I), h_lo, rows_of(w2, H, I, I),
                       params(d, T, H, I, dtype, activation, output, H, dtype), d, true, s);
 }
 

@@ -188,11 +188,15 @@ def _run_ffn(x, w13, w2, activation, output, save: bool):
         output = x.new_empty((T, H))
     else:
         _check_dense("output", output, (T, H), x.dtype, dev)
-    hidden = x.new_empty((T, inter))
-    preact = torch.empty((T, 2 * inter), dtype=torch.float32, device=dev) if save else None
+    hidden = preact = None
+    if save:
+        hidden = x.new_empty((T, inter))
+        preact = torch.empty((T, 2 * inter), dtype=torch.float32, device=dev)
     if T:
+        ws = _scratch((4 if T <= 16 else 2) * T * inter + 1024, x) if T <= 16 or not save else None
         _call("moe_b200_gated_ffn", dev, x.data_ptr(), pitch, w13.data_ptr(), w2.data_ptr(), TYPES[x.dtype], act, T,
-              H, inter, output.data_ptr(), preact.data_ptr() if save else None, hidden.data_ptr(), None, 0)
+              H, inter, output.data_ptr(), preact.data_ptr() if save else None, hidden.data_ptr() if save else None,
+              ws.data_ptr() if ws is not None else None, ws.nbytes if ws is not None else 0)
     return output, preact, hidden
 
 

@@ -343,6 +343,14 @@ def test_host_tensors_are_refused():
         ffn_host.gated_ffn_backward(dy, x, w13, w2, (torch.zeros(2, 64), torch.zeros(2, 32)))
 
 
+@pytest.mark.parametrize("T,H,inter", [(1, 8, 8), (16, 64, 64), (17, 64, 2048), (300, 7168, 2048)])
+def test_host_workspaces_cover_the_library(T, H, inter):
+    import ffn_host
+
+    lib = ffn_host._library()
+    assert (4 if T <= 16 else 2) * T * inter + 1024 >= lib.moe_b200_gated_ffn_workspace_bytes(T, H, inter)
+
+
 def test_c_abi_refusals():
     """Bad sizes, codes, pointers and workspaces come back as status codes
     before any device is touched."""
@@ -363,7 +371,10 @@ def test_c_abi_refusals():
                 {"hid": p + 8}, {"ws": p + 128}):
         assert fwd(**bad) == 2, bad
     need = lib.moe_b200_gated_ffn_workspace_bytes(4, 64, 32)
-    assert need >= 4 * 32 * 2 and fwd(n=need - 1) == 3
+    assert need >= 2 * 4 * 32 * 2 and fwd(n=need - 1) == 3
+    assert fwd(hid=p, n=need - 1) == 3 and fwd(hid=p, ws=None) == 1   # the second part of up to 16 tokens' hidden
+    need = lib.moe_b200_gated_ffn_workspace_bytes(17, 64, 32)
+    assert need >= 17 * 32 * 2 and fwd(T=17, n=need - 1) == 3
     assert fwd(T=0, x=None, out=None) == 0
 
     def bwd(dy=p, gp=64, x=p, xp=64, w13=p, w2=p, pre=p, hid=p, dtype=0, act=0, T=4, H=64, inter=32, gx=p, g13=p, g2=p,
