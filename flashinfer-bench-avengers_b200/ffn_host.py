@@ -110,13 +110,13 @@ def _pitch(t: torch.Tensor) -> int:
     return pitch
 
 
-def _is_dense(t, shape: tuple, dtype: torch.dtype, dev, align: int = 16) -> bool:
-    return (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.device == dev
-            and t.is_contiguous() and not t.data_ptr() & (align - 1))
+def _is_dense(t, shape: tuple, dtype: torch.dtype, dev_index: int, align: int = 16) -> bool:
+    return (t.dtype is dtype and t.shape == shape and t.get_device() == dev_index and t.is_contiguous()
+            and not t.data_ptr() & (align - 1))
 
 
 def _check_dense(name: str, t, shape: tuple, dtype: torch.dtype, dev, align: int = 16) -> None:
-    if _is_dense(t, shape, dtype, dev, align):
+    if isinstance(t, torch.Tensor) and _is_dense(t, shape, dtype, dev.index, align):
         return
     _check_cuda(name, t, dev)
     _check(tuple(t.shape) == shape and t.dtype == dtype and t.is_contiguous(),
@@ -125,7 +125,7 @@ def _check_dense(name: str, t, shape: tuple, dtype: torch.dtype, dev, align: int
 
 
 def _activation(name: str) -> int:
-    act = ACTIVATIONS.get(name) if isinstance(name, str) else None
+    act = ACTIVATIONS.get(name)
     if act is None:
         raise RuntimeError(f"activation must be one of {sorted(ACTIVATIONS)}, got {name!r}")
     return act
@@ -145,12 +145,13 @@ def _mx_bytes(rows: int, cols: int) -> int:
 def _call(name: str, dev: torch.device, *args) -> None:
     """The library function on the current stream of ``dev``, with ``dev`` the
     current device."""
+    idx = dev.index
     fn = getattr(_bound or _library(), name)
-    if dev.index == torch._C._cuda_getDevice():
-        code = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    if idx == torch._C._cuda_getDevice():
+        code = fn(*args, torch._C._cuda_getCurrentRawStream(idx))
     else:
-        with torch.cuda.device(dev):
-            code = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+        with torch.cuda.device(idx):
+            code = fn(*args, torch._C._cuda_getCurrentRawStream(idx))
     if code:
         _raise_on(code, name)
 
@@ -158,14 +159,16 @@ def _call(name: str, dev: torch.device, *args) -> None:
 # ------------------------------------------------- gated feed-forward block
 def _check_ffn(x, w13, w2) -> tuple[int, int, int, int]:
     """(T, H, I, x pitch) of checked inputs."""
-    if isinstance(x, torch.Tensor) and x.is_cuda and isinstance(w2, torch.Tensor) and w2.dim() == 2:
-        dtype, dev = x.dtype, x.device
-        pitch = _pitch(x)
+    try:
         H, inter = w2.shape
-        if (pitch >= 0 and x.size(1) == H and (dtype is torch.bfloat16 or dtype is torch.float16)
+        dtype, idx = x.dtype, x.get_device()
+        pitch = _pitch(x)
+        if (pitch >= 0 and x.shape[1] == H and idx >= 0 and (dtype is torch.bfloat16 or dtype is torch.float16)
                 and not (H | inter) & 7 and 8 <= H <= MAX_DIM and 8 <= inter <= MAX_DIM
-                and _is_dense(w13, (2 * inter, H), dtype, dev) and _is_dense(w2, (H, inter), dtype, dev)):
-            return x.size(0), H, inter, pitch
+                and _is_dense(w13, (2 * inter, H), dtype, idx) and _is_dense(w2, (H, inter), dtype, idx)):
+            return x.shape[0], H, inter, pitch
+    except (AttributeError, TypeError, ValueError):   # not tensors, or not matrices
+        pass
     _check_cuda("x", x)
     _check(x.dtype in (torch.bfloat16, torch.float16), "x must be bfloat16 or float16")
     pitch = _check_rows("x", x)
@@ -184,10 +187,10 @@ def _run_ffn(x, w13, w2, activation, output, save: bool):
     T, H, inter, pitch = _check_ffn(x, w13, w2)
     act = _activation(activation)
     dev = x.device
-    if output is None:
-        output = x.new_empty((T, H))
-    else:
+    if output is not None:
         _check_dense("output", output, (T, H), x.dtype, dev)
+    else:   # (the cheaper way where x has the output's layout)
+        output = torch.empty_like(x) if pitch == H else x.new_empty((T, H))
     hidden = preact = None
     if save:
         hidden = x.new_empty((T, inter))
@@ -283,7 +286,7 @@ def mxfp4_scale_shape(rows: int, cols: int) -> tuple[int, ...]:
 def _check_values(name: str, x) -> int:
     if isinstance(x, torch.Tensor) and x.is_cuda and x.dtype in TYPES:
         pitch = _pitch(x)
-        if pitch >= 0 and not x.size(1) & 31 and 32 <= x.size(1) <= MAX_DIM:
+        if pitch >= 0 and not x.shape[1] & 31 and 32 <= x.shape[1] <= MAX_DIM:
             return pitch
     _check_cuda(name, x)
     _check(x.dtype in TYPES, f"{name} must be bfloat16, float16 or float32")
@@ -294,13 +297,16 @@ def _check_values(name: str, x) -> int:
 
 def _check_mx(name: str, q, scale, dev=None, cols: int | None = None, rows: int | None = None) -> tuple[int, int]:
     """(rows, columns) of a checked 4-bit matrix."""
-    if isinstance(q, torch.Tensor) and q.is_cuda and q.dim() == 2:
+    try:
         r, half = q.shape
-        if ((dev is None or q.device == dev) and q.dtype is torch.uint8 and q.is_contiguous() and r <= MAX_TOKENS
-                and not half & 15 and 16 <= half <= MAX_DIM // 2 and (cols is None or 2 * half == cols)
-                and (rows is None or r == rows) and not q.data_ptr() & 15
-                and _is_dense(scale, mxfp4_scale_shape(r, 2 * half), torch.uint8, q.device)):
+        idx = q.get_device()
+        if (idx >= 0 and (dev is None or idx == dev.index) and q.dtype is torch.uint8 and q.is_contiguous()
+                and r <= MAX_TOKENS and not half & 15 and 16 <= half <= MAX_DIM // 2
+                and (cols is None or 2 * half == cols) and (rows is None or r == rows) and not q.data_ptr() & 15
+                and _is_dense(scale, mxfp4_scale_shape(r, 2 * half), torch.uint8, idx)):
             return r, 2 * half
+    except (AttributeError, TypeError, ValueError):
+        pass
     _check_cuda(name, q, dev)
     _check(q.dtype == torch.uint8 and q.dim() == 2 and q.is_contiguous(),
            f"{name} must be contiguous uint8 codes [R, K / 2]")
