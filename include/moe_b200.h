@@ -459,7 +459,7 @@ MOE_B200_API int moe_b200_a2a_read_status(const void* area, uint32_t* status, in
  * (rows may lie apart, each row contiguous and starting on 16 bytes). All
  * pointers are 16-byte aligned, preact 32, workspaces 256. Workspaces are
  * scratch: calls that may overlap need one each, and so do two captured
- * graphs that may.
+ * graphs that may. Outputs and workspaces must not overlap inputs.
  */
 #define MOE_B200_TYPE_BF16 0
 #define MOE_B200_TYPE_FP16 1
