@@ -218,6 +218,97 @@ def test_autograd(cuda_device):
 
 
 @pytest.mark.gpu
+def test_no_tokens_through_autograd(cuda_device):
+    import ffn_host
+
+    leaves = [t.requires_grad_() for t in _inputs(0, 64, 32, torch.bfloat16)[:3]]
+    ffn_host.gated_ffn(*leaves).sum().backward()
+    assert all(leaf.grad is not None and leaf.grad.shape == leaf.shape and not leaf.grad.any() for leaf in leaves)
+
+
+@pytest.mark.gpu
+def test_lone_row_of_a_wider_matrix(cuda_device):
+    """One row has no pitch: any stride of the first dimension will do."""
+    import ffn_host
+
+    x, w13, w2, dy = _inputs(9, 72, 40, torch.bfloat16, seed=12)
+    wide = torch.zeros(9, 100, dtype=x.dtype, device="cuda")
+    wide[:, :72] = x
+    row = wide[2:3, :72]                      # 200 bytes between rows
+    y, saved = ffn_host.gated_ffn_forward(row, w13, w2)
+    want, want_saved = ffn_host.gated_ffn_forward(x[2:3].clone(), w13, w2)
+    assert torch.equal(y, want) and y.is_contiguous()
+    for a, b in zip(ffn_host.gated_ffn_backward(dy[2:3], row, w13, w2, saved),
+                    ffn_host.gated_ffn_backward(dy[2:3], x[2:3].clone(), w13, w2, want_saved)):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_offsets_beyond_32_bits(cuda_device):
+    """The most tokens, rows of more than 2^31 elements in all: rows at both
+    ends equal those of a call on them alone (the same kernel: over 128 rows),
+    and the weights' gradients of a matrix whose other rows are zero equal
+    those of its nonzero rows."""
+    import ffn_host
+
+    T, H, inter = ffn_host.MAX_TOKENS, 8208, 64
+    _, w13, w2, _ = _inputs(1, H, inter, torch.bfloat16, seed=13)
+    x = torch.zeros(T, H, dtype=torch.bfloat16, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(14)
+    ends = torch.randn(600, H, generator=g, device="cuda").to(torch.bfloat16)
+    x[:300] = ends[:300]
+    x[T - 300:] = ends[300:]
+    y, saved = ffn_host.gated_ffn_forward(x, w13, w2)
+    few, few_saved = ffn_host.gated_ffn_forward(ends, w13, w2)
+    want = ref.ffn(ends, w13, w2, "silu", ends)
+    got = torch.cat([y[:300], y[T - 300:]])
+    ref.assert_within(got, want["y"], "y")
+    assert not y[300:T - 300].any()
+    dx, dw13, dw2 = ffn_host.gated_ffn_backward(x, x, w13, w2, saved)     # dy = x
+    ref.assert_within(torch.cat([dx[:300], dx[T - 300:]]), want["dx"], "dx")
+    # zero terms add nothing, but the sums' order is another: the bound's
+    # gamma(T) covers T / 16 additions, only those of nonzero blocks can round
+    ref.assert_within(dw13, want["dw13"], "dw13")
+    ref.assert_within(dw2, want["dw2"], "dw2")
+    assert ffn_host.read_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [16, 64])
+def test_beside_the_routed_layer(cuda_device, T):
+    """A layer's routed experts and its shared expert on the same tokens, the
+    shared expert on a side stream, many times over: each as it is alone
+    (the routed sums are fp32 atomics, so within the operator's tolerance)."""
+    import ffn_host
+    import moe_host
+    import moe_oracle
+    import workloads
+
+    inp = workloads.make_inputs(T, 3, "cuda")
+    args = workloads.as_args(inp)
+    scale = inp["hidden_states_scale"].t().repeat_interleave(128, 1)
+    x = (inp["hidden_states"].float() * scale).to(torch.bfloat16)
+    _, w13, w2, _ = _inputs(1, 7168, 2048, torch.bfloat16, seed=15)
+    routed, shared = moe_host.run(*args), ffn_host.gated_ffn(x, w13, w2)
+    q13, q2 = ffn_host.mxfp4_quantize(w13), ffn_host.mxfp4_quantize(w2)
+    four = ffn_host.mxfp4_gated_ffn(x, *q13, *q2)
+    ref.assert_within(shared, ref.ffn(x, w13, w2, "silu")["y"], "shared")
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(10):
+        with torch.cuda.stream(side):
+            s = ffn_host.gated_ffn(x, w13, w2), ffn_host.mxfp4_gated_ffn(x, *q13, *q2)
+        got.append((moe_host.run(*args), *s))
+    torch.cuda.synchronize()
+    for r, s, f in got:
+        assert torch.equal(s, shared) and torch.equal(f, four)
+        ok, matched, err, top = moe_oracle.output_close(r, routed, 1e-2, 0.999)
+        assert ok, (matched, err, top)
+    assert moe_host.read_status(moe_host.get_workspace(T, x.device)) == 0 and ffn_host.read_status() == 0
+
+
+@pytest.mark.gpu
 def test_calls_from_new_threads(cuda_device):
     """Threads that have not used CUDA before, two at once."""
     import threading

@@ -206,6 +206,73 @@ def test_zero_rows_and_no_rows(cuda_device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T", [3, 20, 200])
+def test_captured_and_on_two_streams(cuda_device, T):
+    """Linear and block captured into two graphs each, replayed on new inputs
+    in turn, and called on two streams at once."""
+    import ffn_host
+
+    H, inter = 544, 256
+    g = torch.Generator(device="cuda").manual_seed(8)
+    xs = [torch.randn(T, H, generator=g, device="cuda").to(torch.bfloat16) for _ in range(2)]
+    w13 = ffn_host.mxfp4_quantize(torch.randn(2 * inter, H, generator=g, device="cuda"))
+    w2 = ffn_host.mxfp4_quantize(torch.randn(H, inter, generator=g, device="cuda"))
+
+    def both(x):
+        return ffn_host.mxfp4_linear(x, *w13), ffn_host.mxfp4_gated_ffn(x, *w13, *w2)
+
+    want = [[t.clone() for t in both(x)] for x in xs]
+    graphs = []
+    for _ in range(2):
+        static = xs[0].clone()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = both(static)
+        graphs.append((graph, static, out))
+    for k in (1, 0):
+        for n, (graph, static, _) in enumerate(graphs):
+            static.copy_(xs[(k + n) % 2])
+        for graph, _, _ in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for n, (_, _, out) in enumerate(graphs):
+            assert all(torch.equal(a, b) for a, b in zip(out, want[(k + n) % 2]))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = []
+    for _ in range(6):
+        for s, x in zip(streams, xs):
+            with torch.cuda.stream(s):
+                outs.append(both(x))
+    torch.cuda.synchronize()
+    for i, out in enumerate(outs):
+        assert all(torch.equal(a, b) for a, b in zip(out, want[i % 2]))
+    assert ffn_host.read_status() == 0
+
+
+@pytest.mark.gpu
+def test_offsets_beyond_32_bits(cuda_device):
+    """The most rows, more than 2^31 elements in all: rows at both ends."""
+    import ffn_host
+
+    T, K, N = ffn_host.MAX_TOKENS, 8224, 8216
+    x = torch.zeros(T, K, dtype=torch.bfloat16, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(9)
+    ends = torch.randn(400, K, generator=g, device="cuda").to(torch.bfloat16)
+    x[:200], x[T - 200:] = ends[:200], ends[200:]
+    w = ffn_host.mxfp4_quantize(torch.randn(N, K, generator=g, device="cuda"))
+    q, scale = ffn_host.mxfp4_quantize(x)
+    few = ffn_host.mxfp4_quantize(ends)
+    assert torch.equal(torch.cat([q[:200], q[T - 200:]]), few[0]) and not q[200:T - 200].any()
+    back = ffn_host.mxfp4_dequantize(q, scale)
+    assert torch.equal(torch.cat([back[:200], back[T - 200:]]), ffn_host.mxfp4_dequantize(*few))
+    del back, q, scale
+    y = ffn_host.mxfp4_linear(x, *w)
+    assert torch.equal(torch.cat([y[:200], y[T - 200:]]), ffn_host.mxfp4_linear(ends, *w))
+    assert not y[200:T - 200].any()
+    assert ffn_host.read_status() == 0
+
+
+@pytest.mark.gpu
 def test_dense_operators_together(cuda_device):
     """As they are used: two fine-tuning steps of a block, its weights brought
     to 4 bits, then served to a prompt and token by token, from a captured
