@@ -9,6 +9,11 @@ modification times, so copies of the tree keep a valid build). Concurrent
 builders (several processes importing the package at once) serialise on a
 lock file. Run ``python build.py [-v] [-f]`` or call :func:`build`.
 
+:func:`build_binding` compiles ``csrc/torch_binding.cpp`` with the host
+compiler into ``_moe_b200_torch.so``, the Python binding of the dense
+operators (ffn_host); its stamp also holds the torch and Python versions it
+was built for.
+
 The package's entry module builds the library this way on import when it
 is missing or stale, as the reference solution compiles its extension on
 import (solution/cuda/main.py:6-29).
@@ -130,6 +135,76 @@ def build(verbose: bool = False, force: bool = False, ptxas_info: bool = False) 
     return LIB_PATH
 
 
+BINDING_SOURCE = os.path.join(CSRC, "torch_binding.cpp")
+BINDING_PATH = os.path.join(HERE, "_moe_b200_torch.so")
+BINDING_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden"]
+BINDING_LIBS = ["-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
+
+
+def binding_digest() -> str:
+    """SHA-256 over the binding's sources, flags and the versions it is built for."""
+    import torch
+
+    h = hashlib.sha256()
+    h.update(" ".join([torch.__version__, sys.version, *BINDING_FLAGS, *BINDING_LIBS]).encode())
+    for f in (BINDING_SOURCE, os.path.join(INCLUDE, "moe_b200.h"), os.path.abspath(__file__)):
+        with open(f, "rb") as fh:
+            h.update(fh.read())
+        h.update(b"\0")
+    return h.hexdigest()
+
+
+def binding_needs_build() -> bool:
+    if not os.path.exists(BINDING_PATH) or not os.path.exists(BINDING_PATH + ".stamp"):
+        return True
+    with open(BINDING_PATH + ".stamp") as f:
+        return f.read().strip() != binding_digest()
+
+
+def _compile_binding(verbose: bool) -> None:
+    import sysconfig
+
+    import torch
+
+    gxx = shutil.which("g++")
+    if gxx is None:
+        raise RuntimeError("g++ not found; the Python binding of the dense operators cannot be built")
+    root = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(_nvcc())))
+    tmp = f"{BINDING_PATH}.tmp{os.getpid()}"
+    cmd = [gxx, *BINDING_FLAGS, "-I" + os.path.join(root, "include"),
+           "-I" + os.path.join(root, "include", "torch", "csrc", "api", "include"),
+           "-I" + sysconfig.get_paths()["include"], "-I" + os.path.join(cuda, "include"), BINDING_SOURCE, "-o", tmp,
+           "-L" + os.path.join(root, "lib"), *BINDING_LIBS]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if verbose or res.returncode != 0:
+        sys.stderr.write(" ".join(cmd) + "\n" + res.stdout + res.stderr)
+    if res.returncode != 0:
+        raise RuntimeError("compiling the Python binding of the dense operators failed")
+    os.replace(tmp, BINDING_PATH)
+
+
+def build_binding(verbose: bool = False, force: bool = False) -> str:
+    """Compiles the Python binding when it is missing or stale (or always with
+    ``force``; about 12 s); returns its path."""
+    if not force and not binding_needs_build():
+        return BINDING_PATH
+    os.makedirs(OBJ_DIR, exist_ok=True)
+    with open(LOCK_PATH, "w") as lock:
+        fcntl.flock(lock, fcntl.LOCK_EX)
+        try:
+            if force or binding_needs_build():
+                digest = binding_digest()
+                _compile_binding(verbose)
+                with open(BINDING_PATH + ".stamp.tmp", "w") as f:
+                    f.write(digest + "\n")
+                os.replace(BINDING_PATH + ".stamp.tmp", BINDING_PATH + ".stamp")
+        finally:
+            fcntl.flock(lock, fcntl.LOCK_UN)
+    return BINDING_PATH
+
+
 if __name__ == "__main__":
     build(verbose="-v" in sys.argv, force="-f" in sys.argv, ptxas_info="--ptxas" in sys.argv)
     print(LIB_PATH)
+    print(build_binding(verbose="-v" in sys.argv, force="-f" in sys.argv))
