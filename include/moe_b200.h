@@ -471,13 +471,13 @@ MOE_B200_API int moe_b200_a2a_read_status(const void* area, uint32_t* status, in
  * Gated feed-forward block: with [u | g] = x w13^T (rows [0, I) of w13 up,
  * [I, 2I) gate, the order of gemm1_weights above), h = act(g) * u and
  * output = h w2^T. fp32 sums; h is rounded to `dtype`, the type (bf16 or fp16)
- * of x, the weights and the output. For up to 16 tokens what that rounding
+ * of x, the weights and the output. For up to 128 tokens what that rounding
  * left is kept as well, as a second number of that type, and enters output.
  *   x [T, H], w13 [2I, H], w2 [H, I], output [T, H]; H and I multiples of 8
  *   preact   fp32 [T, 2I] or NULL: receives u and g, for the gradients (kept
  *            in 32 bits, because their rounding would enter du and dg)
  *   hidden   [T, I] or NULL: receives h rounded; NULL keeps it in the workspace
- * workspace may be NULL when hidden is given and there are more than 16 tokens.
+ * workspace may be NULL when hidden is given and there are more than 128 tokens.
  */
 MOE_B200_API size_t moe_b200_gated_ffn_workspace_bytes(int64_t num_tokens, int64_t hidden_size, int64_t inter_size);
 MOE_B200_API int moe_b200_gated_ffn(const void* x, int64_t x_pitch, const void* w13, const void* w2, int dtype,

@@ -6,7 +6,7 @@ Bounds count, for every element:
     value, and half the smallest step of fp16's subnormals, 2^-25;
   * the rounding of the 16-bit intermediates (h, du, dg), carried through the
     product that reads them by the absolute values of its other operand; for up
-    to 16 tokens the forward pass reads h as two 16-bit numbers, so its
+    to 128 tokens the forward pass reads h as two 16-bit numbers, so its
     rounding there is u squared of the value;
   * the fp32 sums: a sum of k products is k / 16 additions of 16-term blocks,
     each addition off by at most 2^-23 of the sum of magnitudes (a tensor core
@@ -57,10 +57,10 @@ def ffn(x, w13, w2, name, dy=None):
     h = a * up
     e_h = e_a * up.abs() + a.abs() * e_up + e_a * e_up
     r_h = e_h + u_ * (h.abs() + e_h) + tiny            # after the rounding to 16 bits
-    y_h = e_h + u_ * u_ * (h.abs() + e_h) + tiny if T <= 16 else r_h
+    y_h = e_h + u_ * u_ * (h.abs() + e_h) + tiny if T <= 128 else r_h
     y = h @ w2.T
     # two parts: twice the terms in the sum
-    e_y = y_h @ w2.abs().T + (2 if T <= 16 else 1) * gamma(inter) * ((h.abs() + r_h) @ w2.abs().T)
+    e_y = y_h @ w2.abs().T + (2 if T <= 128 else 1) * gamma(inter) * ((h.abs() + r_h) @ w2.abs().T)
     out = {"y": (y, e_y + u_ * (y.abs() + e_y) + tiny)}
     if dy is None:
         return out

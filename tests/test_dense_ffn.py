@@ -455,9 +455,9 @@ def test_c_abi_refusals():
         assert fwd(**bad) == 2, bad
     need = lib.moe_b200_gated_ffn_workspace_bytes(4, 64, 32)
     assert need >= 2 * 4 * 32 * 2 and fwd(n=need - 1) == 3
-    assert fwd(hid=p, n=need - 1) == 3 and fwd(hid=p, ws=None) == 1   # the second part of up to 16 tokens' hidden
-    need = lib.moe_b200_gated_ffn_workspace_bytes(17, 64, 32)
-    assert need >= 17 * 32 * 2 and fwd(T=17, n=need - 1) == 3
+    assert fwd(hid=p, n=need - 1) == 3 and fwd(hid=p, ws=None) == 1   # the second part of up to 128 tokens' hidden
+    need = lib.moe_b200_gated_ffn_workspace_bytes(129, 64, 32)
+    assert need >= 129 * 32 * 2 and fwd(T=129, n=need - 1) == 3
     assert fwd(T=0, x=None, out=None) == 0
 
     def bwd(dy=p, gp=64, x=p, xp=64, w13=p, w2=p, pre=p, hid=p, dtype=0, act=0, T=4, H=64, inter=32, gx=p, g13=p, g2=p,
