@@ -730,18 +730,18 @@ int max_clusters(int ctas) {
 // Columns per tile (the MMA's N) and K splits of one product: the fewest time
 // units over all waves of tiles. Choosing the columns, against 256 throughout:
 // training step at 4096 tokens 813 -> 786 us, at 333 x 1032 x 520 75 -> 55 us.
-// The columns of a tile come in whole 32-byte stores, so 16 features. A split
-// product is one wave of clusters and adds its parts for kAddCost. (How many
-// clusters of 4 or 8 CTAs run at once depends on how the GPU's SMs are
-// grouped, 33 and 15 where this was measured; one more made 256 tokens take 56
-// us.)
+// A pair's MMA takes N in multiples of 32, which also keeps the columns of a
+// tile in whole 32-byte stores. A split product is one wave of clusters and
+// adds its parts for kAddCost. (How many clusters of 4 or 8 CTAs run at once
+// depends on how the GPU's SMs are grouped, 33 and 15 where this was measured;
+// one more made 256 tokens take 56 us.)
 void choose_shape(DenseGroup* grp, bool gate, int sm_count) {
   constexpr int64_t kAddCost = 6000;
   DenseParams& p = grp->p[0];
   int64_t best_cost = INT64_MAX;
   for (int splits = 1; splits <= 4; splits *= 2) {
     if (splits > 1 && div_up(p.k, 64) < 4 * splits) break;
-    for (int bn = 256; bn >= 64; bn -= gate ? 32 : 16) {
+    for (int bn = 256; bn >= 64; bn -= 32) {
       const int64_t tiles = tile_count(p, gate ? bn / 2 : bn);
       if (splits > 1 && tiles > max_clusters(2 * splits)) continue;
       const int64_t waves = splits > 1 ? 1 : div_up(tiles, sm_count / 2);
