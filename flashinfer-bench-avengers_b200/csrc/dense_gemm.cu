@@ -85,7 +85,7 @@ static_assert(kPairSmem <= 227 * 1024, "shared memory");
 
 template <bool kMx>
 struct PairTraits {
-  static constexpr int kScaleBytes = kMx ? 3072 : 0;   // A: 2 K tiles, B: 2 row tiles x 2 K tiles of 512 bytes
+  static constexpr int kScaleBytes = kMx ? 6 * 512 : 0;   // A: 2 K tiles, B: 2 row tiles x 2 K tiles of 512 bytes
   // Tensor memory: two accumulators of up to 256 columns. With 4-bit
   // operands 48 columns hold the staged exponents (2 x 24), and the
   // accumulators overlap in 48 columns, which the epilogue drains first.

@@ -408,9 +408,8 @@ __global__ void __launch_bounds__(kThreads)
           const uint2 v = make_uint2(pack_16(sum.x, sum.y, p.out_type), pack_16(sum.z, sum.w, p.out_type));
           uint16_t* out = static_cast<uint16_t*>(p.out) + at;
           if (kGate && p.out_lo != nullptr) {
-            const float2 a = unpack_16(v.x, p.out_type), b = unpack_16(v.y, p.out_type);
             *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out_lo) + at) =
-                make_uint2(pack_16(sum.x - a.x, sum.y - a.y, p.out_type), pack_16(sum.z - b.x, sum.w - b.y, p.out_type));
+                make_uint2(pack_rest_16(sum.x, sum.y, v.x, p.out_type), pack_rest_16(sum.z, sum.w, v.y, p.out_type));
           }
           if (p.vec32) {
             *reinterpret_cast<uint2*>(out) = v;

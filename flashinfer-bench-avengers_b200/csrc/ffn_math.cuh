@@ -51,6 +51,13 @@ __device__ __forceinline__ float2 unpack_16(uint32_t bits, int type) {
   return __half22float2(*reinterpret_cast<const __half2*>(&bits));
 }
 
+// What the rounding of (lo, hi) to `packed` left, rounded again: 0 beside an
+// infinity, so that a value beyond the type stays infinite in a sum of both.
+__device__ __forceinline__ uint32_t pack_rest_16(float lo, float hi, uint32_t packed, int type) {
+  const float2 v = unpack_16(packed, type);
+  return pack_16(isinf(v.x) ? 0.f : lo - v.x, isinf(v.y) ? 0.f : hi - v.y, type);
+}
+
 // ------------------------------------------------- 4-bit microscaled blocks
 // Exponent byte of a block from the largest magnitude's bits: floor(log2) - 2
 // (the largest e2m1 exponent), biased by 127, at least 0. Infinities and

@@ -134,6 +134,24 @@ def test_rows_do_not_mix(cuda_device, T):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T", [1, 64, 128, 129])
+def test_hidden_beyond_half_precision(cuda_device, T):
+    """A hidden value beyond fp16 is infinite, with its sign, and so are the
+    outputs it enters; nothing turns into NaN."""
+    import ffn_host
+
+    x, w13, w2, _ = _inputs(T, 256, 128, torch.float16, seed=6)
+    w13[0], w13[128] = 0, 0
+    w13[0, 0], w13[128, 0] = -300, 300     # u and g of feature 0
+    x[:, 0] = 0
+    x[T - 1, 0] = 1                        # h = -300 silu(300) = -90000
+    w2[:, 0] = torch.where(w2[:, 0] < 0, -1.0, 1.0)
+    y = ffn_host.gated_ffn(x, w13, w2)
+    assert torch.equal(y[T - 1], -w2[:, 0] * float("inf"))
+    assert torch.isfinite(y[: T - 1]).all()
+
+
+@pytest.mark.gpu
 def test_large_gates(cuda_device):
     """Gates far beyond the exponential's range: act(g) is g or 0, its slope 1
     or 0, and nothing turns into NaN."""
