@@ -148,14 +148,36 @@ struct Scratch {
 
 void* current_stream(at::Device dev) { return c10::cuda::getCurrentCUDAStream(dev.index()).stream(); }
 
+// Bytes from a tensor's first element to its last.
+uintptr_t span(const at::Tensor& t) {
+  int64_t n = 1;
+  for (int64_t d = 0; d < t.dim(); ++d) n += (t.size(d) - 1) * t.stride(d);
+  return static_cast<uintptr_t>(n * t.element_size());
+}
+
+bool overlap(const at::Tensor& a, const at::Tensor& b) {
+  if (a.numel() == 0 || b.numel() == 0) return false;
+  const uintptr_t pa = reinterpret_cast<uintptr_t>(a.const_data_ptr());
+  const uintptr_t pb = reinterpret_cast<uintptr_t>(b.const_data_ptr());
+  return pa < pb + span(b) && pb < pa + span(a);
+}
+
 // `given` if it is an output of this shape and type, a new tensor if it is
-// None; nullopt if it will not do.
-std::optional<at::Tensor> output(PyObject* given, int64_t rows, int64_t cols, at::ScalarType type, at::Device dev) {
+// None; nullopt if it will not do. A given one is written in place: it may
+// overlap no input, autograd must not follow it, and its version goes up, so
+// that a backward pass which saved it notices.
+std::optional<at::Tensor> output(PyObject* given, int64_t rows, int64_t cols, at::ScalarType type, at::Device dev,
+                                 std::initializer_list<const at::Tensor*> inputs) {
   if (given == Py_None) return matrix(rows, cols, type, dev);
   const at::Tensor* t = tensor(given);
-  if (!dense(t, rows, cols, type, dev)) return std::nullopt;
+  if (!dense(t, rows, cols, type, dev) || (at::GradMode::is_enabled() && t->requires_grad())) return std::nullopt;
+  for (const at::Tensor* in : inputs)
+    if (overlap(*t, *in)) return std::nullopt;
+  if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
   return *t;
 }
+
+bool followed(const at::Tensor& t) { return t.requires_grad() || t._fw_grad(0).defined(); }
 
 PyObject* result(int code, const at::Tensor& t) { return code ? PyLong_FromLong(code) : THPVariable_Wrap(t); }
 
@@ -203,10 +225,9 @@ PyObject* gated_ffn(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!ready(n, 5)) return nullptr;
   Ffn f;
   if (!read_ffn(a[0], a[1], a[2], &f)) Py_RETURN_NONE;
-  if (at::GradMode::is_enabled() && (f.x->requires_grad() || f.w13->requires_grad() || f.w2->requires_grad()))
-    Py_RETURN_FALSE;
+  if (at::GradMode::is_enabled() && (followed(*f.x) || followed(*f.w13) || followed(*f.w2))) Py_RETURN_FALSE;
   const at::Device dev = f.x->device();
-  const std::optional<at::Tensor> out = output(a[4], f.T, f.H, f.x->scalar_type(), dev);
+  const std::optional<at::Tensor> out = output(a[4], f.T, f.H, f.x->scalar_type(), dev, {f.x, f.w13, f.w2});
   if (!out) Py_RETURN_NONE;
   int code = 0;
   if (f.T > 0) {
@@ -338,7 +359,7 @@ PyObject* mxfp4_matmul(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!type || !read_mx(a[0], a[1], nullptr, &l)) Py_RETURN_NONE;
   const at::Device dev = l.q->device();
   if (!read_mx(a[2], a[3], &dev, &r) || r.cols != l.cols || r.rows == 0) Py_RETURN_NONE;
-  const std::optional<at::Tensor> out = output(a[5], l.rows, r.rows, *type, dev);
+  const std::optional<at::Tensor> out = output(a[5], l.rows, r.rows, *type, dev, {l.q, l.scale, r.q, r.scale});
   if (!out) Py_RETURN_NONE;
   int code = 0;
   if (l.rows > 0) {
@@ -362,7 +383,7 @@ PyObject* mxfp4_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int64_t T = x->size(0), K = x->size(1);
   Mx w;
   if (!read_mx(a[1], a[2], &dev, &w) || w.cols != K || w.rows == 0) Py_RETURN_NONE;
-  const std::optional<at::Tensor> out = output(a[3], T, w.rows, x->scalar_type(), dev);
+  const std::optional<at::Tensor> out = output(a[3], T, w.rows, x->scalar_type(), dev, {x, w.q, w.scale});
   if (!out) Py_RETURN_NONE;
   int code = 0;
   if (T > 0) {
@@ -389,7 +410,8 @@ PyObject* mxfp4_gated_ffn(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!read_mx(a[1], a[2], &dev, &w13) || !read_mx(a[3], a[4], &dev, &w2) || w13.cols != H || w2.rows != H ||
       w13.rows != 2 * w2.cols)
     Py_RETURN_NONE;
-  const std::optional<at::Tensor> out = output(a[6], T, H, x->scalar_type(), dev);
+  const std::optional<at::Tensor> out =
+      output(a[6], T, H, x->scalar_type(), dev, {x, w13.q, w13.scale, w2.q, w2.scale});
   if (!out) Py_RETURN_NONE;
   int code = 0;
   if (T > 0) {

@@ -11,7 +11,9 @@ Calls go through a small native binding (csrc/torch_binding.cpp), which tests
 their conditions, allocates and launches; where it declines, the checks here
 find the argument at fault and say so. They run on the current stream of the
 inputs' device. Scratch comes from torch's caching allocator call by call, so
-calls on several streams and captured graphs never share it.
+calls on several streams and captured graphs never share it. An ``output`` is
+written in place; it may overlap no input. Gradients are recorded by gated_ffn
+alone; the 4-bit functions serve.
 """
 from __future__ import annotations
 
@@ -120,9 +122,20 @@ def _check_dense(name: str, t, shape: tuple, dtype: torch.dtype, dev, align: int
     _check(t.data_ptr() % align == 0, f"{name} must be {align}-byte aligned")
 
 
-def _check_output(output, shape: tuple, dtype: torch.dtype, dev) -> None:
-    if output is not None:
-        _check_dense("output", output, shape, dtype, dev)
+def _span(t: torch.Tensor) -> tuple[int, int]:
+    elements = 1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (elements * t.element_size() if t.numel() else 0)
+
+
+def _check_output(output, shape: tuple, dtype: torch.dtype, dev, *inputs: torch.Tensor) -> None:
+    if output is None:
+        return
+    _check_dense("output", output, shape, dtype, dev)
+    _check(not (torch.is_grad_enabled() and output.requires_grad), "output must not require gradients")
+    begin, end = _span(output)
+    for t in inputs:
+        first, last = _span(t)
+        _check(end <= first or last <= begin, "output must not overlap an input")
 
 
 def _check_ffn(x, w13, w2) -> tuple[int, int, int]:
@@ -230,7 +243,7 @@ def gated_ffn(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, activation: 
 
     def explain():
         T, H, _ = _check_ffn(x, w13, w2)
-        _check_output(output, (T, H), x.dtype, x.device)
+        _check_output(output, (T, H), x.dtype, x.device, x, w13, w2)
 
     return _answer("moe_b200_gated_ffn", got, explain)
 
@@ -307,7 +320,7 @@ def mxfp4_matmul(a_q: torch.Tensor, a_scale: torch.Tensor, b_q: torch.Tensor, b_
         M, K = _check_mx("a_q", a_q, a_scale)
         N, _ = _check_mx("b_q", b_q, b_scale, a_q.device, K)
         _check(N > 0, "b_q must have rows")
-        _check_output(output, (M, N), dtype, a_q.device)
+        _check_output(output, (M, N), dtype, a_q.device, a_q, a_scale, b_q, b_scale)
 
     return _answer("moe_b200_mxfp4_matmul", got, explain)
 
@@ -324,7 +337,7 @@ def mxfp4_linear(x: torch.Tensor, w_q: torch.Tensor, w_scale: torch.Tensor,
         _check_values("x", x)
         N, _ = _check_mx("w_q", w_q, w_scale, x.device, x.size(1))
         _check(N > 0, "w_q must have rows")
-        _check_output(output, (x.size(0), N), x.dtype, x.device)
+        _check_output(output, (x.size(0), N), x.dtype, x.device, x, w_q, w_scale)
 
     return _answer("moe_b200_mxfp4_linear", got, explain)
 
@@ -345,7 +358,7 @@ def mxfp4_gated_ffn(x: torch.Tensor, w13_q: torch.Tensor, w13_scale: torch.Tenso
         two_i, _ = _check_mx("w13_q", w13_q, w13_scale, x.device, H)
         _check(two_i > 0 and two_i % 64 == 0, f"w13_q must have 2 I rows, I a multiple of 32; got {two_i}")
         _check_mx("w2_q", w2_q, w2_scale, x.device, two_i // 2, H)
-        _check_output(output, (T, H), x.dtype, x.device)
+        _check_output(output, (T, H), x.dtype, x.device, x, w13_q, w13_scale, w2_q, w2_scale)
 
     return _answer("moe_b200_mxfp4_gated_ffn", got, explain)
 

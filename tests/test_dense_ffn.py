@@ -440,6 +440,54 @@ def test_refusals_on_the_gpu(cuda_device):
         ffn_host.gated_ffn_backward(dy, x, w13, w2, (saved[0], saved[1][:2]))
 
 
+@pytest.mark.gpu
+def test_output_argument(cuda_device):
+    """A given output is returned, its version goes up like that of any tensor
+    written in place, and one that overlaps an input or that autograd follows
+    is refused; so is forward-mode differentiation."""
+    import ffn_host
+    import torch.autograd.forward_ad as fwad
+
+    x, w13, w2, _ = _inputs(8, 64, 32, torch.bfloat16, seed=8)
+    want = ffn_host.gated_ffn(x, w13, w2)
+    out = torch.empty_like(x)
+    version = out._version
+    assert ffn_host.gated_ffn(x, w13, w2, output=out) is out
+    assert torch.equal(out, want) and out._version > version
+    with torch.inference_mode():
+        inner = torch.empty_like(x)
+    assert torch.equal(ffn_host.gated_ffn(x, w13, w2, output=inner), want)
+
+    leaf = torch.empty_like(x).requires_grad_()
+    with pytest.raises(RuntimeError, match="output must not require gradients"):
+        ffn_host.gated_ffn(x, w13, w2, output=leaf)
+    with torch.no_grad():
+        ffn_host.gated_ffn(x, w13, w2, output=leaf)
+    assert torch.equal(leaf, want)
+    buffer = torch.zeros(24, 64, dtype=x.dtype, device="cuda")
+    for first in (1, 8, 15):
+        with pytest.raises(RuntimeError, match="output must not overlap an input"):
+            ffn_host.gated_ffn(buffer[8:16], w13, w2, output=buffer[first:first + 8])
+    ffn_host.gated_ffn(buffer[8:16], w13, w2, output=buffer[:8])
+    ffn_host.gated_ffn(buffer[8:16], w13, w2, output=buffer[16:])
+
+    q, scale = ffn_host.mxfp4_quantize(w13)
+    q2, scale2 = ffn_host.mxfp4_quantize(w2)
+    square = torch.zeros(8, 64, dtype=x.dtype, device="cuda")
+    for call in (lambda: ffn_host.mxfp4_gated_ffn(square, q, scale, q2, scale2, output=square),
+                 lambda: ffn_host.mxfp4_linear(square, q, scale, output=square)):
+        with pytest.raises(RuntimeError, match="output must not overlap an input"):
+            call()
+    raw = torch.zeros(4096, dtype=torch.uint8, device="cuda")
+    a = raw[:1024].view(32, 32)
+    a_scale = ffn_host.mxfp4_quantize(torch.zeros(32, 64, device="cuda"))[1]
+    with pytest.raises(RuntimeError, match="output must not overlap an input"):
+        ffn_host.mxfp4_matmul(a, a_scale, a, a_scale, output=raw[512:512 + 2048].view(torch.bfloat16).view(32, 32))
+
+    with fwad.dual_level(), pytest.raises(RuntimeError):
+        ffn_host.gated_ffn(fwad.make_dual(x, torch.ones_like(x)), w13, w2)
+
+
 def test_host_tensors_are_refused():
     import ffn_host
 
