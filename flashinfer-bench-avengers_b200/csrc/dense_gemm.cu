@@ -383,7 +383,6 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     tmem_alloc_pair(smem_u32(s_tmem), 512);
     tmem_relinquish_pair();
   }
-  pdl_launch_next();
   tc_fence_before();
   __syncthreads();
   cluster_sync();
@@ -391,7 +390,10 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   const uint32_t tmem = *s_tmem;
   // Everything above overlaps the previous kernel's tail. (The producer waits
   // for that kernel below; no bounded wait of the others starts before.)
-  if (warp != 0) pdl_wait();
+  if (warp != 0) {
+    pdl_wait();
+    pdl_launch_next();
+  }
 
   if (warp == 0) {
     // ---------------------------------------------------------- producer
@@ -438,10 +440,11 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       }
     };
     // B is an input of the whole call (weights, or saved by another call):
-    // its part of the first ring does not wait for the predecessor.
+    // behind a kernel of the same call its part of the first ring does not
+    // wait for that kernel.
     const Work w0 = work_at<kGrouped>(pair, grp);
     const int first = k_begin(grp.p[w0.g].k_iters, split, splits);
-    const int early = min(kS, k_begin(grp.p[w0.g].k_iters, split + 1, splits) - first);
+    const int early = grp.p[0].early ? min(kS, k_begin(grp.p[w0.g].k_iters, split + 1, splits) - first) : 0;
     if (issue)
       for (int i = 0; i < early; ++i) load_b(w0, first + i, i);
     __syncwarp();
@@ -658,7 +661,8 @@ void set_ring(DenseGroup* grp, int stage_bytes) {
 }
 
 template <bool kMx, bool kBMn, int kEpi>
-int launch_pair(const PairMaps& maps, const DenseGroup& grp, int sm_count, bool dependent, cudaStream_t s) {
+int launch_pair(const PairMaps& maps, DenseGroup grp, int sm_count, bool dependent, cudaStream_t s) {
+  grp.p[0].early = dependent;
   auto kern = dense_pair_kernel<kMx, kBMn, kEpi>;
   constexpr int smem = kPairSmem;
   static OncePerDevice ready;
@@ -680,7 +684,7 @@ int launch_pair(const PairMaps& maps, const DenseGroup& grp, int sm_count, bool 
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = dependent ? 2 : 1;
+  cfg.numAttrs = 2;
   return cudaLaunchKernelEx(&cfg, kern, maps, grp) == cudaSuccess ? MOE_B200_OK : MOE_B200_ERR_CUDA;
 }
 

@@ -52,6 +52,7 @@ struct DenseParams {
   int64_t x_pitch;
   // derived by the launcher
   int bn, n_step, b_half, m_tiles, n_tiles, k_iters, vec32, a_mn, copy_bytes;
+  int early;           // B may be read before the kernel before has finished
 };
 
 // D = A B^T with B stored K x N, and A stored M x K or (a_mn) K x M.
@@ -67,8 +68,14 @@ struct MxOperand {
   int64_t rows;
 };
 
-// B of every GEMM must be complete before the call's first kernel starts: it
-// is read before the previous kernel has finished. A may be its result.
+// Every kernel starts under the end of the one before it, whatever that was
+// (programmatic dependent launch), and waits for it before it touches memory:
+// block at one token 21.2 -> 20.3 us, 4-bit linear 8.1 -> 6.9, training step
+// 333 x 1032 x 520 36 -> 34 against ordinary launches of a call's first
+// kernel. With `dependent` the kernel follows another of the same call; then
+// it reads B, an input of the whole call, before it waits. That is sound
+// because each kernel waits before it lets the next one start: when a call's
+// second kernel starts, all work before the call is complete.
 //
 // D = A B^T over CTA pairs, both operands stored along K (kEpiStore,
 // kEpiGated: B has 2 n rows, up then gate). Returns a MOE_B200 status code.

@@ -28,9 +28,9 @@
 // less; equal at four tokens, slower from eight: 10.1 against 11.8 us).
 //
 // Two GEMMs of a call overlap (programmatic dependent launch): weights are
-// inputs of the whole call, so a kernel requests its first ring of weight
-// tiles before it waits for its predecessor; only the token operand comes
-// from the kernel before. It is let go when its predecessor requests its own
+// inputs of the whole call, so the second kernel requests its first ring of
+// weight tiles before it waits for the first; only the token operand comes
+// from that. It is let go when its predecessor requests its own
 // last ring, so HBM does not idle under the first one's tail. (Asking for the
 // rest of the K range into L2 as well was no faster.)
 #include <cuda.h>
@@ -233,13 +233,16 @@ __global__ void __launch_bounds__(kThreads)
     // The next kernel of the call may start once this CTA requests its last
     // ring (25.5 us for the block at one token; 26.3 released at the start).
     const int release = max(iters - sh.stages, 0);
-    if (issue)
+    if (issue && p.early)
       for (int i = 0; i < first; ++i) load_w(i, i);
-    if (release < first) pdl_launch_next();
     __syncwarp();
     pdl_wait();
+    if (release < first) pdl_launch_next();
     if (issue)
-      for (int i = 0; i < first; ++i) load_x(i, i);
+      for (int i = 0; i < first; ++i) {
+        if (!p.early) load_w(i, i);
+        load_x(i, i);
+      }
     __syncwarp();
     int stage = first == sh.stages ? 0 : first;
     uint32_t ph = 0;
@@ -433,8 +436,8 @@ namespace {
 
 template <bool kMx, int kEpi, int kSrc>
 int launch_skinny(const CUtensorMap& w, const CUtensorMap& x, const CUtensorMap& sfw, const CUtensorMap& sfx,
-                  const DenseParams& p, const SkinnyShape& sh, int units, int token_tiles, bool dependent,
-                  cudaStream_t s) {
+                  DenseParams p, const SkinnyShape& sh, int units, int token_tiles, bool dependent, cudaStream_t s) {
+  p.early = dependent;
   auto kern = dense_skinny_kernel<kMx, kEpi, kSrc>;
   static OncePerDevice ready;
   if (!ready([&] {
@@ -455,7 +458,7 @@ int launch_skinny(const CUtensorMap& w, const CUtensorMap& x, const CUtensorMap&
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = dependent ? 2 : 1;
+  cfg.numAttrs = 2;
   return cudaLaunchKernelEx(&cfg, kern, w, x, sfw, sfx, p, sh) == cudaSuccess ? MOE_B200_OK : MOE_B200_ERR_CUDA;
 }
 

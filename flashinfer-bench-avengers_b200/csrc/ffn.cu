@@ -85,9 +85,10 @@ int quantize(const void* x, int type, int64_t rows, int64_t cols, int64_t pitch,
   auto kern = type == MOE_B200_TYPE_BF16   ? mxfp4_quantize_kernel<kTypeBf16>
               : type == MOE_B200_TYPE_FP16 ? mxfp4_quantize_kernel<kTypeFp16>
                                            : mxfp4_quantize_kernel<kTypeFp32>;
-  kern<<<grid, 256, 0, s>>>(static_cast<const uint8_t*>(x), pitch_bytes, static_cast<int>(rows),
-                            static_cast<int>(cols / 32), k_tiles, vec32, q, scale);
-  return cudaGetLastError() == cudaSuccess ? MOE_B200_OK : MOE_B200_ERR_CUDA;
+  return launch_kernel(kern, grid, 256, 0, s, true, static_cast<const uint8_t*>(x), pitch_bytes,
+                       static_cast<int>(rows), static_cast<int>(cols / 32), k_tiles, vec32, q, scale) == cudaSuccess
+             ? MOE_B200_OK
+             : MOE_B200_ERR_CUDA;
 }
 
 // x [p->m, p->k] to 4 bits, in `to` or (`inside`) by the GEMM itself.
@@ -272,10 +273,12 @@ int moe_b200_mxfp4_dequantize(const void* q, const void* scale, int64_t rows, in
   auto kern = dtype == MOE_B200_TYPE_BF16   ? mxfp4_dequantize_kernel<kTypeBf16>
               : dtype == MOE_B200_TYPE_FP16 ? mxfp4_dequantize_kernel<kTypeFp16>
                                             : mxfp4_dequantize_kernel<kTypeFp32>;
-  kern<<<static_cast<unsigned>(div_up(total, 256)), 256, 0, static_cast<cudaStream_t>(stream)>>>(
-      static_cast<const uint8_t*>(q), static_cast<const uint8_t*>(scale), total, blocks,
-      static_cast<int>(div_up(cols, 128)), aligned(out, 32), static_cast<uint8_t*>(out));
-  return cudaGetLastError() == cudaSuccess ? MOE_B200_OK : MOE_B200_ERR_CUDA;
+  const int vec32 = aligned(out, 32);
+  return launch_kernel(kern, static_cast<unsigned>(div_up(total, 256)), 256, 0, static_cast<cudaStream_t>(stream), true,
+                       static_cast<const uint8_t*>(q), static_cast<const uint8_t*>(scale), total, blocks,
+                       static_cast<int>(div_up(cols, 128)), vec32, static_cast<uint8_t*>(out)) == cudaSuccess
+             ? MOE_B200_OK
+             : MOE_B200_ERR_CUDA;
 }
 
 int moe_b200_mxfp4_matmul(const void* a_q, const void* a_scale, const void* b_q, const void* b_scale, int64_t m,

@@ -52,6 +52,7 @@ __global__ void __launch_bounds__(256, kType == kTypeFp32 ? 2 : 4)
     mxfp4_quantize_kernel(const uint8_t* x, int64_t pitch, int rows, int blocks, int k_tiles, int vec32, uint8_t* q,
                           uint8_t* scale) {
   __shared__ __align__(16) uint8_t s_scale[512];
+  pdl_wait();
   pdl_launch_next();
   constexpr int kBytes = kType == kTypeFp32 ? 128 : 64;
   constexpr int kWords = kBytes / 4;
@@ -111,6 +112,8 @@ template <int kType>
 __global__ void __launch_bounds__(256)
     mxfp4_dequantize_kernel(const uint8_t* q, const uint8_t* scale, int64_t total, int blocks, int k_tiles, int vec32,
                             uint8_t* out) {
+  pdl_wait();
+  pdl_launch_next();
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   if (i >= total) return;
   const int64_t row = i / blocks;

@@ -250,6 +250,64 @@ def test_captured_and_on_two_streams(cuda_device, T):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T", [1, 16, 300])
+def test_weights_written_just_before(cuda_device, T):
+    """Weights that a long kernel of the library, or a copy on a joined
+    stream, writes right before the call: every kernel of the call sees them,
+    eager and captured."""
+    import ffn_host
+
+    rows, H, inter = 16384, 1024, 512
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    big = [torch.randn(rows, H, device="cuda", generator=gen, dtype=torch.bfloat16) for _ in range(2)]
+    narrow = [b.view(2 * rows, inter) for b in big]
+    x = torch.randn(T, H, device="cuda", generator=gen, dtype=torch.bfloat16)
+
+    def linear(i):
+        q, s = ffn_host.mxfp4_quantize(big[i])
+        return ffn_host.mxfp4_linear(x, q[-1024:], s[-8:])
+
+    def block4(i):
+        q, s = ffn_host.mxfp4_quantize(big[i])
+        q2, s2 = ffn_host.mxfp4_quantize(narrow[i])          # the last one written feeds the last GEMM
+        return ffn_host.mxfp4_gated_ffn(x, q[-1024:], s[-8:], q2[-1024:], s2[-8:])
+
+    def block16(i):
+        w13 = ffn_host.mxfp4_dequantize(*ffn_host.mxfp4_quantize(big[i]))[-1024:]
+        w2 = ffn_host.mxfp4_dequantize(*ffn_host.mxfp4_quantize(narrow[i]))[-1024:]
+        return ffn_host.gated_ffn(x, w13, w2)
+
+    for call in (linear, block4, block16):
+        want = []
+        for i in range(2):
+            torch.cuda.synchronize()
+            want.append(call(i).clone())
+        for r in range(6):      # memory of the last round's weights, with the other weights in it
+            assert torch.equal(call(r % 2), want[r % 2])
+
+    w13, w2 = big[0][:1024].clone(), narrow[0][:1024].clone()
+    source13, source2, side = big[0].clone(), narrow[0].clone(), torch.cuda.Stream()
+    full2 = torch.zeros_like(narrow[0])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        main = torch.cuda.current_stream()
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            full2.copy_(source2)                             # 34 MB
+        w13.copy_(source13[-1024:])
+        main.wait_stream(side)
+        y = ffn_host.gated_ffn(x, w13, full2[-1024:])
+        z = ffn_host.gated_ffn(x, w13, w2)
+    for i in (1, 0, 1):
+        source13.copy_(big[i]), source2.copy_(narrow[i])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, ffn_host.gated_ffn(x, big[i][-1024:], narrow[i][-1024:]))
+        assert torch.equal(z, ffn_host.gated_ffn(x, big[i][-1024:], w2))
+    assert ffn_host.read_status() == 0
+
+
+@pytest.mark.gpu
 def test_offsets_beyond_32_bits(cuda_device):
     """The most rows, more than 2^31 elements in all: rows at both ends."""
     import ffn_host
