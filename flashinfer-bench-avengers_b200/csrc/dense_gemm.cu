@@ -587,6 +587,9 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       if (!__all_sync(0xffffffffu, ready)) break;
       tc_fence_after();
       const uint32_t acc = lanes + (buf ? Tr::kAcc1 : 0);
+      // A tile to come needs these columns. Otherwise nobody waits for the
+      // arrival, and it could reach the first CTA after that has left.
+      const bool reused = tiles - t > (kMx ? pairs : 2 * pairs);
       if (splits > 1) {
         // this pair's part of the sums, one row per thread, over the drained ring
         float* part = reinterpret_cast<float*>(smem) + (quarter * 32 + lane) * kPartPitch;
@@ -611,12 +614,12 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           tmem_ld32(acc + c, r);
           tmem_ld32(acc + p.n_step + c, g);
           tmem_wait_ld();
-          if (kMx && i == half) release_early(acce_bar, lane);
+          if (kMx && i == half && reused) release_early(acce_bar, lane);
           if (live && col < end) store_gated<kEpi>(p, row, col, end, r, g);
         } else {
           tmem_ld32(acc + c, r);
           tmem_wait_ld();
-          if (kMx && i == half) release_early(acce_bar, lane);
+          if (kMx && i == half && reused) release_early(acce_bar, lane);
           if (dact) {
             const int next = i + 2 < chunks && live ? end : 0;
             if (live && col < end) store_dact(p, row, col, end, r, saved[0]);
@@ -628,7 +631,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           }
         }
       }
-      if (!kMx) {
+      if (!kMx && reused) {
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&acce_bar[buf]), lead));
