@@ -203,9 +203,15 @@ __device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint64_t desc) 
 constexpr uint32_t kDescHiSw128 = (1024u >> 4) | (1u << 14) | (2u << 29);
 constexpr uint32_t kDescHiPlain = (128u >> 4) | (1u << 14);
 
-__device__ __forceinline__ uint32_t desc_lo_kmajor(uint32_t addr) { return (addr >> 4) | (1u << 16); }
-__device__ __forceinline__ uint32_t desc_lo_mnmajor(uint32_t addr) { return (addr >> 4) | ((8192u >> 4) << 16); }
-__device__ __forceinline__ uint32_t desc_lo_scale(uint32_t addr) { return (addr >> 4) | ((128u >> 4) << 16); }
+// An address in a cluster carries the CTA's rank above its offset, which is all
+// that a descriptor takes; what is above would land in the next field, the
+// distance to the next 64 elements.
+__device__ __forceinline__ uint32_t desc_address(uint32_t addr) { return (addr & 0x3ffffu) >> 4; }
+__device__ __forceinline__ uint32_t desc_lo_kmajor(uint32_t addr) { return desc_address(addr) | (1u << 16); }
+__device__ __forceinline__ uint32_t desc_lo_mnmajor(uint32_t addr) {
+  return desc_address(addr) | ((8192u >> 4) << 16);
+}
+__device__ __forceinline__ uint32_t desc_lo_scale(uint32_t addr) { return desc_address(addr) | ((128u >> 4) << 16); }
 
 __device__ __forceinline__ uint64_t desc_of(uint32_t hi, uint32_t lo) {
   return (static_cast<uint64_t>(hi) << 32) | lo;
