@@ -42,7 +42,7 @@ struct DenseParams {
   int out_type;        // type code of `out`
   void* out;           // [m, n], row pitch ldo elements; [du | dg]: [m, 2 n]
   int64_t ldo;
-  void* out_lo;        // kEpiGated, streaming form: h - out, rounded again, when set
+  void* out_lo;        // streaming form: what the rounding of h (when set) or [du | dg] left, rounded again
   float* preact;       // fp32 [m, 2 n]: written by kEpiGated when set, read by kEpiBackward
   uint8_t* q;          // kEpiGatedQuant: codes [m, n / 2]
   uint8_t* q_scale;    //   and tiled exponents
@@ -91,7 +91,8 @@ int launch_mx_pair(DenseEpi epi, const MxOperand& a, const MxOperand& b, const D
                    bool dependent, cudaStream_t s);
 
 // Few rows of A: out = A B^T streaming B, K split over a cluster
-// (kEpiStore and kEpiGated; 4-bit: kEpiStore).
+// (kEpiStore and kEpiGated; kEpiBackward with B stored K x N; 4-bit:
+// kEpiStore).
 // With a_lo set the operand is the sum of the two matrices a and a_lo (at most
 // kTwoPartRows rows).
 constexpr int64_t kTwoPartRows = 128;

@@ -13,7 +13,13 @@
 // Gated form (16-bit): the tile's 128 rows are 64 up rows and the 64 gate
 // rows of the same features, and the adding threads apply the activation.
 //
-// The 16-bit block keeps its hidden as the sum of two 16-bit numbers, h rounded
+// Backward form (16-bit): the weights are stored K x N, as dh = dy W2 and dx =
+// [du | dg] W13 read them; the descriptor takes them so, and the adding
+// threads of dh compute du and dg, in two parts like the hidden (gradients at
+// 16 tokens, H = 7168, I = 2048, against CTA pairs: 89 -> 55 us; at 128 95 ->
+// 80; 16 x 2048 x 1024 29 -> 17).
+//
+// The 16-bit block keeps its hidden (and [du | dg] for dx) as the sum of two 16-bit numbers, h rounded
 // and what that left, rounded again: the second product takes both as
 // neighbouring token tiles of one MMA (N = 2 x 16 to 2 x 128) and their sums
 // are added with the parts. The result then carries one rounding instead of
@@ -144,6 +150,29 @@ __device__ __forceinline__ void stage_tokens(const DenseParams& p, const SkinnyS
   }
 }
 
+// [du | dg] of four columns and a token, in two parts, from dh and the saved
+// u and g (`pre`).
+__device__ __forceinline__ void store_dact(const DenseParams& p, const float* pre, int64_t at, const float4& dh) {
+  const float4 u = *reinterpret_cast<const float4*>(pre);
+  const float4 g = *reinterpret_cast<const float4*>(pre + p.n);
+  const float d[4] = {dh.x, dh.y, dh.z, dh.w}, up[4] = {u.x, u.y, u.z, u.w}, gate[4] = {g.x, g.y, g.z, g.w};
+  float v[2][4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    float value, slope;
+    act_value_slope(gate[j], p.act, value, slope);
+    v[0][j] = d[j] * value;
+    v[1][j] = d[j] * up[j] * slope;
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint2 hi = make_uint2(pack_16(v[i][0], v[i][1], p.type), pack_16(v[i][2], v[i][3], p.type));
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at + i * p.n) = hi;
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out_lo) + at + i * p.n) =
+        make_uint2(pack_rest_16(v[i][0], v[i][1], hi.x, p.type), pack_rest_16(v[i][2], v[i][3], hi.y, p.type));
+  }
+}
+
 }  // namespace
 
 template <bool kMx, int kEpi, int kSrc>
@@ -152,6 +181,7 @@ __global__ void __launch_bounds__(kThreads)
                         const __grid_constant__ CUtensorMap tm_sfw, const __grid_constant__ CUtensorMap tm_sfx,
                         const DenseParams p, const SkinnyShape sh) {
   constexpr bool kGate = kEpi == kEpiGated;
+  constexpr bool kWMn = kEpi == kEpiBackward;  // weights stored K x N
   constexpr bool kQuantX = kSrc != kFromMatrix;
   constexpr int kUnit = kGate ? 64 : 128;      // features per cluster
   static_assert(!(kMx && kGate) && (kMx || !kQuantX), "");
@@ -216,6 +246,9 @@ __global__ void __launch_bounds__(kThreads)
       if constexpr (kMx) {
         tma_load_2d(sw, &tm_w, bar, x, n0);
         tma_load_2d(sw + kWeightTile + x_bytes, &tm_sfw, bar, 0, (n0 >> 7) * kt + 2 * (kb0 + i));
+      } else if constexpr (kWMn) {
+        tma_load_2d(sw, &tm_w, bar, n0, x);
+        tma_load_2d(sw + kWeightTile / 2, &tm_w, bar, n0 + 64, x);
       } else {
         tma_load_2d(sw, &tm_w, bar, x, n0);
         tma_load_2d(sw + kWeightTile / 2, &tm_w, bar, x, n0 + (kGate ? p.n : 64));
@@ -265,10 +298,10 @@ __global__ void __launch_bounds__(kThreads)
   } else if (warp == 1) {
     // --------------------------------------------------------------- MMA
     const bool issue = elect_lane();
-    const uint32_t idesc0 = kMx ? idesc_mxf4(128, sh.bn, 0) : idesc_f16(128, sh.x_rows, p.type == kTypeFp16, false, false);
+    const uint32_t idesc0 = kMx ? idesc_mxf4(128, sh.bn, 0) : idesc_f16(128, sh.x_rows, p.type == kTypeFp16, kWMn, false);
     const uint32_t idesc1 = kMx ? idesc_mxf4(128, sh.bn, 2) : idesc0;
     const uint32_t base = smem_u32(smem);
-    const uint32_t lo_w0 = desc_lo_kmajor(base);
+    const uint32_t lo_w0 = kWMn ? desc_lo_mnmajor(base) : desc_lo_kmajor(base);
     const uint32_t lo_s0 = desc_lo_scale(base + kWeightTile + x_bytes);
     const uint32_t lo_x0 = desc_lo_kmajor(base + (kQuantX ? sh.xq_off : kWeightTile));
     const uint32_t lo_sx0 = kQuantX ? desc_lo_scale(base + sh.xq_off + sh.xq_iters * sh.bn * 128)
@@ -304,7 +337,7 @@ __global__ void __launch_bounds__(kThreads)
         } else {
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            umma_f16<1>(tmem, desc_of(kDescHiSw128, lo_w + 2 * k), desc_of(kDescHiSw128, lo_x + 2 * k), idesc0, i | k);
+            umma_f16<1>(tmem, desc_of(kDescHiSw128, lo_w + (kWMn ? 128 : 2) * k), desc_of(kDescHiSw128, lo_x + 2 * k), idesc0, i | k);
         }
         umma_commit(smem_u32(empty_bar) + 8u * stage);
         if (i == iters - 1) umma_commit(smem_u32(done_bar));
@@ -397,7 +430,9 @@ __global__ void __launch_bounds__(kThreads)
           sum.z *= act_value(gate.z, p.act), sum.w *= act_value(gate.w, p.act);
         }
         const int64_t at = row * p.ldo + n0 + f;
-        if (p.out_type == kTypeFp32) {
+        if (kWMn && p.preact != nullptr) {
+          store_dact(p, p.preact + row * (2 * static_cast<int64_t>(p.n)) + n0 + f, at, sum);
+        } else if (p.out_type == kTypeFp32) {
           float* out = static_cast<float*>(p.out) + at;
           if (p.vec32) {
             *reinterpret_cast<float4*>(out) = sum;
@@ -524,6 +559,8 @@ int launch_dense_skinny(DenseEpi epi, const DenseOperand& a, const void* a_lo, c
       !encode_2d(&tx, a.base, 2, a.cols, a.rows, a.pitch, 64, sh.bn) ||
       !encode_2d(&tlo, a_lo != nullptr ? a_lo : a.base, 2, a.cols, a.rows, a.pitch, 64, sh.bn))
     return MOE_B200_ERR_DRIVER;
+  if (epi == kEpiBackward)
+    return launch_skinny<false, kEpiBackward, kFromMatrix>(tw, tx, tw, tlo, p, sh, units, token_tiles, dependent, s);
   return gate ? launch_skinny<false, kEpiGated, kFromMatrix>(tw, tx, tw, tlo, p, sh, units, token_tiles, dependent, s)
               : launch_skinny<false, kEpiStore, kFromMatrix>(tw, tx, tw, tlo, p, sh, units, token_tiles, dependent, s);
 }

@@ -18,9 +18,11 @@ namespace moe {
 namespace {
 
 constexpr int64_t kMaxDim = 65536;
-// Up to this many tokens the forward GEMMs stream the weights through
-// dense_skinny.cu; above, they run over CTA pairs.
+// Up to this many tokens the GEMMs stream the weights through
+// dense_skinny.cu; above (and for the weights' gradients), they run over CTA
+// pairs.
 constexpr int64_t kSkinnyMaxTokens = 128;
+static_assert(kSkinnyMaxTokens == kTwoPartRows, "the streaming form keeps two parts");
 
 size_t round256(size_t x) { return (x + 255) / 256 * 256; }
 
@@ -181,7 +183,8 @@ int moe_b200_gated_ffn(const void* x, int64_t x_pitch, const void* w13, const vo
 
 size_t moe_b200_gated_ffn_backward_workspace_bytes(int64_t num_tokens, int64_t hidden_size, int64_t inter_size) {
   if (!tokens_ok(num_tokens) || !dim_ok(hidden_size, 8) || !dim_ok(inter_size, 8)) return 0;
-  return round256(static_cast<size_t>(num_tokens) * inter_size * 4) + 256;
+  // [du | dg], and what its rounding left
+  return round256(static_cast<size_t>(num_tokens) * inter_size * 4 * (num_tokens <= kTwoPartRows ? 2 : 1)) + 256;
 }
 
 int moe_b200_gated_ffn_backward(const void* grad_output, int64_t grad_pitch, const void* x, int64_t x_pitch,
@@ -216,26 +219,40 @@ int moe_b200_gated_ffn_backward(const void* grad_output, int64_t grad_pitch, con
   if (st != MOE_B200_OK) return st;
   const DenseOperand dy = rows_of(grad_output, T, H, grad_pitch);
   const DenseOperand dact = rows_of(workspace, T, 2 * I, 2 * I);
-  // dh = dy W2, in its epilogue [du | dg], together with dW2 = dy^T h; then
-  // dx = [du | dg] W13 together with dW13 = [du | dg]^T x.
-  DenseProduct first[2], second[2];
-  int n1 = 0, n2 = 0;
-  if (need_dact) {
-    first[n1] = {dy, rows_of(w2, H, I, I), false, params(d, T, I, H, dtype, activation, workspace, 2 * I, dtype)};
-    first[n1++].p.preact = const_cast<float*>(preact);
-  }
-  if (grad_w2)
-    first[n1++] = {dy, rows_of(hidden, T, I, I), true, params(d, H, I, T, dtype, activation, grad_w2, I, dtype)};
-  if (grad_x)
-    second[n2++] = {dact, rows_of(w13, 2 * I, H, H), false, params(d, T, H, 2 * I, dtype, activation, grad_x, H, dtype)};
-  if (grad_w13)
-    second[n2++] = {dact, rows_of(x, T, H, x_pitch), true,
-                    params(d, 2 * I, H, T, dtype, activation, grad_w13, H, dtype)};
-  if (n1 > 0) {
-    st = launch_dense_backward(first, n1, d.sm_count, false, s);
+  // dh = dy W2 gives [du | dg]; then dx = [du | dg] W13, dW13 = [du | dg]^T x
+  // and dW2 = dy^T h.
+  DenseParams p_dh = params(d, T, I, H, dtype, activation, workspace, 2 * I, dtype);
+  p_dh.preact = const_cast<float*>(preact);
+  const DenseProduct dh = {dy, rows_of(w2, H, I, I), false, p_dh};
+  const DenseProduct dx = {dact, rows_of(w13, 2 * I, H, H), false,
+                           params(d, T, H, 2 * I, dtype, activation, grad_x, H, dtype)};
+  const DenseProduct dw13 = {dact, rows_of(x, T, H, x_pitch), true,
+                             params(d, 2 * I, H, T, dtype, activation, grad_w13, H, dtype)};
+  const DenseProduct dw2 = {dy, rows_of(hidden, T, I, I), true,
+                            params(d, H, I, T, dtype, activation, grad_w2, I, dtype)};
+  DenseProduct group[2];
+  int n = 0;
+  if (T <= kSkinnyMaxTokens) {
+    // the weights are streamed as in the forward pass, then written
+    void* lo = need_dact ? static_cast<uint8_t*>(workspace) + static_cast<size_t>(T) * I * 4 : nullptr;
+    p_dh.out_lo = lo;
+    if (need_dact) st = launch_dense_skinny(kEpiBackward, dh.a, nullptr, dh.b, p_dh, d.sm_count, false, s);
+    if (st == MOE_B200_OK && grad_x)
+      st = launch_dense_skinny(kEpiBackward, dx.a, lo, dx.b, dx.p, d.sm_count, true, s);
     if (st != MOE_B200_OK) return st;
+    if (grad_w13) group[n++] = dw13;
+    if (grad_w2) group[n++] = dw2;
+    return n > 0 ? launch_dense_backward(group, n, d.sm_count, need_dact, s) : MOE_B200_OK;
   }
-  return n2 > 0 ? launch_dense_backward(second, n2, d.sm_count, true, s) : MOE_B200_OK;
+  // dh together with dW2, then dx together with dW13
+  if (need_dact) group[n++] = dh;
+  if (grad_w2) group[n++] = dw2;
+  if (n > 0) st = launch_dense_backward(group, n, d.sm_count, false, s);
+  if (st != MOE_B200_OK) return st;
+  n = 0;
+  if (grad_x) group[n++] = dx;
+  if (grad_w13) group[n++] = dw13;
+  return n > 0 ? launch_dense_backward(group, n, d.sm_count, true, s) : MOE_B200_OK;
 }
 
 size_t moe_b200_mxfp4_scale_bytes(int64_t rows, int64_t cols) {

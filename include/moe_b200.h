@@ -488,7 +488,8 @@ MOE_B200_API int moe_b200_gated_ffn(const void* x, int64_t x_pitch, const void* 
 /*
  * Gradients of the block for grad_output [T, H], from the preact and hidden
  * that the forward call saved: with dh = grad_output w2, du = dh act(g) and
- * dg = dh u act'(g) (rounded to dtype as operands of the products below),
+ * dg = dh u act'(g) (rounded to dtype as operands of the products below; for
+ * up to 128 tokens what that left enters grad_x as well),
  *   grad_x   = [du | dg] w13          [T, H]
  *   grad_w13 = [du | dg]^T x          [2I, H]
  *   grad_w2  = grad_output^T hidden   [H, I]

@@ -6,8 +6,8 @@ Bounds count, for every element:
     value, and half the smallest step of fp16's subnormals, 2^-25;
   * the rounding of the 16-bit intermediates (h, du, dg), carried through the
     product that reads them by the absolute values of its other operand; for up
-    to 128 tokens the forward pass reads h as two 16-bit numbers, so its
-    rounding there is u squared of the value;
+    to 128 tokens y and dx read them as two 16-bit numbers, so the rounding
+    there is u squared of the value;
   * the fp32 sums: a sum of k products is k / 16 additions of 16-term blocks,
     each addition off by at most 2^-23 of the sum of magnitudes (a tensor core
     may truncate), so GAMMA(k) = (k / 16 + 16) 2^-23 times that sum;
@@ -75,13 +75,16 @@ def ffn(x, w13, w2, name, dy=None):
     e_d = torch.cat([e_du, e_dg], 1)
     r_d = e_d + u_ * (d.abs() + e_d) + tiny
 
-    def product(left, e_left, right, k):
+    # dx of few tokens reads [du | dg] in two parts, like y
+    d_x = e_d + u_ * u_ * (d.abs() + e_d) + tiny if T <= 128 else r_d
+
+    def product(left, e_left, right, k, parts=1):
         v = left @ right
         m = e_left @ right.abs()
-        e = m + gamma(k) * (left.abs() @ right.abs() + m)
+        e = m + parts * gamma(k) * (left.abs() @ right.abs() + m)
         return v, e + u_ * (v.abs() + e) + tiny
 
-    out["dx"] = product(d, r_d, w13, 2 * inter)
+    out["dx"] = product(d, d_x, w13, 2 * inter, 2 if T <= 128 else 1)
     out["dw13"] = product(d.T, r_d.T, x, T)
     v, e = product(h.T, r_h.T, dy, T)
     out["dw2"] = (v.T, e.T)
