@@ -30,16 +30,19 @@
 // gradients need W^T and X^T): the shared-memory descriptors take both, so
 // nothing is transposed in memory.
 //
-// Where the tiles of a forward product are few, their K range is split over 2
-// or 4 pairs of one cluster: the partial tiles meet through distributed shared
+// Where the tiles of a product are few, their K range is split over 2 or 4
+// pairs of one cluster: the partial tiles meet through distributed shared
 // memory, each CTA adding the parts of its share of the rows in a fixed order
 // (block at 256 tokens 44.5 -> 35.8 us, at 512 49.5 -> 46.4 us).
 //
-// One launch takes up to two products whose tiles follow one another in the
-// walk. The backward pass has two pairs of products that do not depend on
-// each other (dh with dW2, dx with dW13): together they fill their last waves
-// and save a kernel's start and end each (training step at 4096 tokens 824 ->
-// 796 us, 333 x 1032 x 520 48 -> 39 us).
+// One launch takes up to three products whose tiles follow one another in the
+// walk. Of the backward pass's products dW2 depends on neither dh nor dx and
+// dW13, and dx and dW13 not on each other: in two launches, dW2 in the one
+// where it costs less, they fill their last waves and save a kernel's start
+// and end each (training step at 4096 tokens 824 -> 796 us, 333 x 1032 x 520
+// 48 -> 39 us). With dh split and dW2 beside dx and dW13, against dW2 always
+// beside an unsplit dh: gradients at H = 7168, I = 2048 and 129 tokens 95 ->
+// 68 us, at 512 103 -> 93, at 1024 156 -> 147; 1024 x 2048 x 1024 41 -> 37.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -96,25 +99,50 @@ constexpr int kScaleCol = 464;   // 4-bit: the first of those 48 columns
 constexpr int kEpiWarps = 8;
 constexpr int kPairThreads = (4 + kEpiWarps) * 32;
 
-// One launch: up to two products, their tiles numbered one after the other.
+// One launch: up to three products, their tiles numbered one after the other.
 struct DenseGroup {
-  DenseParams p[2];
-  int tiles0;        // tiles of the first
-  int tiles;         // of both
+  DenseParams p[3];
+  int tiles0, tiles1;   // tiles of the first, of the first two
+  int tiles;            // of all
+  int own, more, lead;  // tile_at
   int stages, stage_bytes;
   int splits;        // pairs of a cluster that share a tile's K range
 };
 
-// Tensor maps: A, B of the first product, then of the second; 4-bit: A, B and
+// Tensor maps: A, B of the first product, then of the others; 4-bit: A, B and
 // their exponents.
 struct PairMaps {
-  CUtensorMap m[4];
+  CUtensorMap m[6];
 };
 
 struct Work {
   int g;             // which product
   int m0, n0;        // first output row of the pair, first output column
 };
+
+// The j-th tile of a pair, -1 behind its last. The pairs take turns, first at
+// the tiles of the first product: each has `own` of them, the first `more`
+// pairs one more. The others then take `lead` tiles of the other products
+// before the turns go on, for the tiles of the first may be several times as
+// long.
+template <bool kGrouped>
+__device__ __forceinline__ int tile_at(const DenseGroup& grp, int pair, int pairs, int j) {
+  int t = pair + j * pairs;
+  if constexpr (kGrouped) {
+    int s = j - grp.own - (pair < grp.more);
+    if (s >= 0) {
+      const int idle = pairs - grp.more;
+      if (pair >= grp.more && s < grp.lead) {
+        t = s * idle + pair - grp.more;
+      } else {
+        if (pair >= grp.more) s -= grp.lead;
+        t = grp.lead * idle + s * pairs + pair;
+      }
+      t += grp.tiles0;
+    }
+  }
+  return t < grp.tiles ? t : -1;
+}
 
 // Tiles in bands of 8 row tiles, rows fastest: the pairs running at one time
 // cover a near-square block of the output, so A and B slices are re-read
@@ -123,8 +151,8 @@ template <bool kGrouped>
 __device__ __forceinline__ Work work_at(int t, const DenseGroup& grp) {
   constexpr int kBand = 8;
   Work o;
-  o.g = kGrouped && t >= grp.tiles0 ? 1 : 0;
-  if (o.g) t -= grp.tiles0;
+  o.g = kGrouped ? (t >= grp.tiles0) + (t >= grp.tiles1) : 0;
+  if (o.g) t -= o.g == 1 ? grp.tiles0 : grp.tiles1;
   const DenseParams& p = grp.p[o.g];
   const int per_band = kBand * p.n_tiles;
   const int band = t / per_band;
@@ -227,24 +255,28 @@ __device__ __forceinline__ void load_saved(const DenseParams& p, int64_t row, in
     }
 }
 
-// [du | dg] = [dh act(g) | dh u act'(g)] of 16 columns.
+// [du | dg] = [dh act(g) | dh u act'(g)] of two columns, rounded to 16 bits.
+__device__ __forceinline__ void dact_pair(const uint32_t* dh, const uint32_t* u, const uint32_t* g,
+                                          const DenseParams& p, uint32_t& du, uint32_t& dg) {
+  float v[2], w[2];
+#pragma unroll
+  for (int l = 0; l < 2; ++l) {
+    float value, slope;
+    act_value_slope(__uint_as_float(g[l]), p.act, value, slope);
+    const float d = __uint_as_float(dh[l]);
+    v[l] = d * value;
+    w[l] = d * __uint_as_float(u[l]) * slope;
+  }
+  du = pack_16(v[0], v[1], p.type);
+  dg = pack_16(w[0], w[1], p.type);
+}
+
+// The same of 16 columns, stored.
 __device__ __forceinline__ void store_dact(const DenseParams& p, int64_t row, int col, int end, const uint32_t* dh,
                                            const Saved& s) {
   uint32_t du[8], dg[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    float v[2], w[2];
-#pragma unroll
-    for (int l = 0; l < 2; ++l) {
-      float value, slope;
-      act_value_slope(__uint_as_float(s.g[2 * e + l]), p.act, value, slope);
-      const float d = __uint_as_float(dh[2 * e + l]);
-      v[l] = d * value;
-      w[l] = d * __uint_as_float(s.u[2 * e + l]) * slope;
-    }
-    du[e] = pack_16(v[0], v[1], p.type);
-    dg[e] = pack_16(w[0], w[1], p.type);
-  }
+  for (int e = 0; e < 8; ++e) dact_pair(dh + 2 * e, s.u + 2 * e, s.g + 2 * e, p, du[e], dg[e]);
   uint16_t* out = static_cast<uint16_t*>(p.out) + row * p.ldo;
   store_row16(out, col, end, du, p.vec32);
   store_row16(out + p.n, col, end, dg, p.vec32);
@@ -313,11 +345,21 @@ __device__ __forceinline__ void add_parts(const DenseParams& p, const Work& w, u
       for (int j = 0; j < 8; ++j)
         v[j] = __float_as_uint(act_value(__uint_as_float(g[j]), p.act) * __uint_as_float(v[j]));
     }
-    uint32_t out[4];
+    uint16_t* out = static_cast<uint16_t*>(p.out) + row * p.ldo + col;
+    uint32_t o[4];
+    if (kEpi == kEpiBackward && p.preact != nullptr) {
+      const float* pre = p.preact + row * (2 * static_cast<int64_t>(p.n)) + col;
+      uint32_t u[8], g[8], dg[4];
+      ld_global_32(u, pre);
+      ld_global_32(g, pre + p.n);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) out[j] = pack_16(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]), p.out_type);
-    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + row * p.ldo + col) =
-        make_uint4(out[0], out[1], out[2], out[3]);
+      for (int j = 0; j < 4; ++j) dact_pair(v + 2 * j, u + 2 * j, g + 2 * j, p, o[j], dg[j]);
+      *reinterpret_cast<uint4*>(out + p.n) = make_uint4(dg[0], dg[1], dg[2], dg[3]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] = pack_16(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]), p.out_type);
+    }
+    *reinterpret_cast<uint4*>(out) = make_uint4(o[0], o[1], o[2], o[3]);
   }
 }
 
@@ -330,12 +372,15 @@ __device__ __forceinline__ void release_early(uint64_t* acce_bar, int lane) {
 
 }  // namespace
 
-template <bool kMx, bool kBMn, int kEpi>
+// kSplits: clusters of several pairs take one tile each, `split` telling the
+// pairs apart; otherwise clusters of one pair walk the tiles. (One kernel for
+// both took 0.3 us longer per launch.)
+template <bool kMx, bool kBMn, int kEpi, bool kSplits>
 __global__ void __launch_bounds__(kPairThreads, 1)
     dense_pair_kernel(const __grid_constant__ PairMaps maps, const __grid_constant__ DenseGroup grp) {
   using Tr = PairTraits<kMx>;
   constexpr bool kGate = kEpi == kEpiGated || kEpi == kEpiGatedQuant;
-  constexpr bool kGrouped = kEpi == kEpiBackward;   // two products, A stored either way
+  constexpr bool kGrouped = kEpi == kEpiBackward;   // several products, A stored either way
   const int kS = grp.stages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -350,18 +395,16 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  // Clusters of one pair walk the tiles; with K split, a cluster of several
-  // pairs takes one tile, `split` telling its pairs apart.
-  constexpr bool kSplits = !kMx && (kEpi == kEpiStore || kEpi == kEpiGated);
   const int splits = kSplits ? grp.splits : 1;
   const uint32_t cta = cluster_cta_rank();
   const uint32_t rank = cta & 1u;
   const uint32_t lead = cta & ~1u;
-  const int split = static_cast<int>(cta >> 1);
+  const int split = kSplits ? static_cast<int>(cta >> 1) : 0;
   const uint32_t pair_mask = 3u << lead;
-  const int pair = static_cast<int>(blockIdx.x) / (2 * splits);
-  const int pairs = static_cast<int>(gridDim.x) / (2 * splits);
-  const int tiles = grp.tiles;
+  const int log_ctas = kSplits ? 32 - __clz(splits) : 1;   // of a cluster
+  const int pair = static_cast<int>(blockIdx.x >> log_ctas);
+  const int pairs = static_cast<int>(gridDim.x >> log_ctas);
+  auto tile_of = [&](int j) { return tile_at<kGrouped>(grp, pair, pairs, j); };
   uint32_t* const status = grp.p[0].status;
 
   if (warp == 0 && lane == 0) {
@@ -442,9 +485,11 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     // B is an input of the whole call (weights, or saved by another call):
     // behind a kernel of the same call its part of the first ring does not
     // wait for that kernel.
-    const Work w0 = work_at<kGrouped>(pair, grp);
+    const int t0 = tile_of(0);
+    const Work w0 = work_at<kGrouped>(max(t0, 0), grp);
     const int first = k_begin(grp.p[w0.g].k_iters, split, splits);
-    const int early = grp.p[0].early ? min(kS, k_begin(grp.p[w0.g].k_iters, split + 1, splits) - first) : 0;
+    const int early =
+        grp.p[0].early && t0 >= 0 ? min(kS, k_begin(grp.p[w0.g].k_iters, split + 1, splits) - first) : 0;
     if (issue)
       for (int i = 0; i < early; ++i) load_b(w0, first + i, i);
     __syncwarp();
@@ -452,11 +497,11 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     int stage = 0;
     uint32_t ph = 0;
     bool ok = true;
-    for (int t = pair; ok && t < tiles; t += pairs) {
+    for (int it = 0, t; ok && (t = tile_of(it)) >= 0; ++it) {
       const Work w = work_at<kGrouped>(t, grp);
       const int kb0 = k_begin(grp.p[w.g].k_iters, split, splits);
       const int kb1 = k_begin(grp.p[w.g].k_iters, split + 1, splits);
-      const int skip = kb0 + (t == pair ? early : 0);   // K steps whose B is on its way already
+      const int skip = kb0 + (it == 0 ? early : 0);   // K steps whose B is on its way already
       for (int kb = kb0; kb < kb1; ++kb) {
         if (kb >= skip &&
             !warp_wait(smem_u32(empty_bar) + 8u * stage, ph ^ 1u, s_abort, status, kStatusTimeoutProducer)) {
@@ -482,13 +527,12 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       int stage = 0;
       uint32_t ph = 0;
       bool ok = true;
-      int it = 0;                 // tiles done by this pair
       int old = kS - 2;           // 4-bit: the stage before last, and its phase
       uint32_t old_ph = 1, sf = 0;
       const uint32_t base = smem_u32(smem);
       const uint32_t lo_b0 = kBMn ? desc_lo_mnmajor(base + kTileBytes) : desc_lo_kmajor(base + kTileBytes);
       const uint32_t lo_s0 = desc_lo_scale(base + 2 * kTileBytes);
-      for (int t = pair; ok && t < tiles; t += pairs, ++it) {
+      for (int it = 0, t; ok && (t = tile_of(it)) >= 0; ++it) {   // `it` tiles are done
         const DenseParams& p = grp.p[work_at<kGrouped>(t, grp).g];
         const bool a_mn = kGrouped && p.a_mn;
         const uint32_t idesc0 = kMx ? idesc_mxf4(256, 256, 0) : idesc_f16(256, p.bn, p.type == kTypeFp16, a_mn, kBMn);
@@ -564,9 +608,11 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     const int quarter = warp & 3;
     const int half = (warp - 4) >> 2;   // two warps per quarter, taking turns at 32-column chunks
     const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
-    int it = 0;
-    for (int t = pair; t < tiles; t += pairs, ++it) {
-      const Work w = work_at<kGrouped>(t, grp);
+    int next[2] = {tile_of(0), tile_of(1)};
+    for (int it = 0; next[0] >= 0; ++it) {
+      const Work w = work_at<kGrouped>(next[0], grp);
+      next[0] = next[1];
+      next[1] = next[1] >= 0 ? tile_of(it + 2) : -1;
       const DenseParams& p = grp.p[w.g];
       const int width = kGate ? p.n_step : p.bn;   // output columns of a tile
       const int chunks = (width + 31) >> 5;
@@ -576,7 +622,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       const int end = min(p.n, w.n0 + width);      // first column past this tile
       // dh: the saved sums of the first two 16-column pieces are on their way
       // while the accumulator is still being computed.
-      const bool dact = kEpi == kEpiBackward && p.preact != nullptr;
+      const bool dact = kEpi == kEpiBackward && p.preact != nullptr && !kSplits;
       Saved saved[2];
       if (dact) {
         load_saved(p, row, w.n0 + 32 * half, live ? end : 0, saved[0]);
@@ -589,8 +635,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       const uint32_t acc = lanes + (buf ? Tr::kAcc1 : 0);
       // A tile to come needs these columns. Otherwise nobody waits for the
       // arrival, and it could reach the first CTA after that has left.
-      const bool reused = tiles - t > (kMx ? pairs : 2 * pairs);
-      if (splits > 1) {
+      const bool reused = next[kMx ? 0 : 1] >= 0;
+      if constexpr (kSplits) {
         // this pair's part of the sums, one row per thread, over the drained ring
         float* part = reinterpret_cast<float*>(smem) + (quarter * 32 + lane) * kPartPitch;
         for (int c = 32 * half; c < p.bn; c += 64) {
@@ -640,11 +686,9 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   }
 
   if constexpr (kSplits) {
-    if (splits > 1) {
-      __syncwarp();
-      cluster_sync();   // every pair's part is there
-      if (*s_abort == 0) add_parts<kEpi>(grp.p[0], work_at<false>(pair, grp), smem_u32(smem), rank, split, splits);
-    }
+    __syncwarp();
+    cluster_sync();   // every pair's part is there
+    if (*s_abort == 0) add_parts<kEpi>(grp.p[0], work_at<false>(pair, grp), smem_u32(smem), rank, split, splits);
   }
   // No CTA leaves while the other may still reach its shared or tensor memory.
   __syncwarp();
@@ -663,10 +707,10 @@ void set_ring(DenseGroup* grp, int stage_bytes) {
   grp->stages = kRingBytes / stage_bytes < kMaxStages ? kRingBytes / stage_bytes : kMaxStages;
 }
 
-template <bool kMx, bool kBMn, int kEpi>
-int launch_pair(const PairMaps& maps, DenseGroup grp, int sm_count, bool dependent, cudaStream_t s) {
+template <bool kMx, bool kBMn, int kEpi, bool kSplits>
+int launch_kernel_pair(const PairMaps& maps, DenseGroup grp, int sm_count, bool dependent, cudaStream_t s) {
   grp.p[0].early = dependent;
-  auto kern = dense_pair_kernel<kMx, kBMn, kEpi>;
+  auto kern = dense_pair_kernel<kMx, kBMn, kEpi, kSplits>;
   constexpr int smem = kPairSmem;
   static OncePerDevice ready;
   if (!ready([&] {
@@ -674,6 +718,10 @@ int launch_pair(const PairMaps& maps, DenseGroup grp, int sm_count, bool depende
       }))
     return MOE_B200_ERR_CUDA;
   const int pairs = grp.splits > 1 ? grp.tiles * grp.splits : grp.tiles < sm_count / 2 ? grp.tiles : sm_count / 2;
+  const int walkers = pairs / grp.splits;
+  grp.own = grp.tiles0 / walkers;
+  grp.more = grp.tiles0 % walkers;
+  if (grp.more == 0) grp.lead = 0;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(2 * pairs));
   cfg.blockDim = dim3(kPairThreads);
@@ -689,6 +737,13 @@ int launch_pair(const PairMaps& maps, DenseGroup grp, int sm_count, bool depende
   cfg.attrs = attr;
   cfg.numAttrs = 2;
   return cudaLaunchKernelEx(&cfg, kern, maps, grp) == cudaSuccess ? MOE_B200_OK : MOE_B200_ERR_CUDA;
+}
+
+template <bool kMx, bool kBMn, int kEpi>
+int launch_pair(const PairMaps& maps, const DenseGroup& grp, int sm_count, bool dependent, cudaStream_t s) {
+  if constexpr (!kMx)
+    if (grp.splits > 1) return launch_kernel_pair<kMx, kBMn, kEpi, true>(maps, grp, sm_count, dependent, s);
+  return launch_kernel_pair<kMx, kBMn, kEpi, false>(maps, grp, sm_count, dependent, s);
 }
 
 // Time units of a tile of bn columns: a K step costs an MMA 2 N cycles and the
@@ -714,7 +769,7 @@ int max_clusters(int ctas) {
   std::atomic<int>& slot = known[ctas == 8][dev];
   int n = slot.load(std::memory_order_relaxed);
   if (n == 0) {
-    auto kern = dense_pair_kernel<false, false, kEpiGated>;
+    auto kern = dense_pair_kernel<false, false, kEpiGated, true>;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(ctas));
     cfg.blockDim = dim3(kPairThreads);
@@ -742,46 +797,55 @@ int max_clusters(int ctas) {
 // adds its parts for kAddCost. (How many clusters of 4 or 8 CTAs run at once
 // depends on how the GPU's SMs are grouped, 33 and 15 where this was measured;
 // one more made 256 tokens take 56 us.)
-void choose_shape(DenseGroup* grp, bool gate, int sm_count) {
+DensePlan choose_shape(const DenseParams& p, bool gate, bool b_mn, int sm_count) {
   constexpr int64_t kAddCost = 6000;
-  DenseParams& p = grp->p[0];
-  int64_t best_cost = INT64_MAX;
+  DensePlan plan = {};
+  plan.cost = INT64_MAX;
   for (int splits = 1; splits <= 4; splits *= 2) {
     if (splits > 1 && div_up(p.k, 64) < 4 * splits) break;
     for (int bn = 256; bn >= 64; bn -= 32) {
       const int64_t tiles = tile_count(p, gate ? bn / 2 : bn);
       if (splits > 1 && tiles > max_clusters(2 * splits)) continue;
       const int64_t waves = splits > 1 ? 1 : div_up(tiles, sm_count / 2);
-      const int64_t cost = waves * tile_cost(p, bn, false, splits) + (splits > 1 ? kAddCost : 0);
-      if (cost < best_cost) {
-        best_cost = cost;
-        p.bn = bn;
-        grp->splits = splits;
+      const int64_t cost = waves * tile_cost(p, bn, b_mn, splits) + (splits > 1 ? kAddCost : 0);
+      if (cost < plan.cost) plan = DensePlan{{bn, 0}, splits, 0, cost};
+    }
+  }
+  return plan;
+}
+
+// The same for several products of which all but the first have one K and take
+// one width. Before the last turns every pair has `own` tiles of the first
+// product, some one more, the others `lead` tiles of the rest (tile_at): as
+// many as fit beside it, or one.
+DensePlan choose_shapes(const DenseProduct* products, int count, int sm_count) {
+  constexpr int kWidths = 7;   // 256, 224, .. 64
+  const int pairs = sm_count / 2;
+  int tiles[2][kWidths] = {}, costs[2][kWidths] = {};
+  for (int i = 0; i < count; ++i)
+    for (int w = 0; w < kWidths; ++w) {
+      tiles[i > 0][w] += static_cast<int>(tile_count(products[i].p, 256 - 32 * w));
+      costs[i > 0][w] = static_cast<int>(tile_cost(products[i].p, 256 - 32 * w, true));
+    }
+  DensePlan plan = {};
+  plan.cost = INT64_MAX;
+  for (int w0 = 0; w0 < kWidths; ++w0) {
+    const int own = tiles[0][w0] / pairs, more = tiles[0][w0] % pairs, idle = pairs - more;
+    const int64_t c0 = costs[0][w0];
+    for (int w1 = 0; w1 < kWidths; ++w1) {
+      const int rest = tiles[1][w1], c1 = costs[1][w1];
+      const int fit = static_cast<int>(c0) / c1;
+      for (int lead = 1; lead <= fit + 1; lead = lead < fit ? fit : lead + 1) {
+        const int ahead = more == 0 ? 0 : lead * idle < rest ? lead * idle : rest;
+        const int64_t beside = static_cast<int64_t>(div_up(ahead, idle)) * c1;
+        const int64_t last = more == 0 ? 0 : c0 > beside ? c0 : beside;
+        const int64_t cost = own * c0 + last + div_up(rest - ahead, pairs) * c1;
+        if (cost < plan.cost) plan = DensePlan{{256 - 32 * w0, 256 - 32 * w1}, 1, lead, cost};
+        if (more == 0) break;
       }
     }
   }
-}
-
-// The same for two products walked one after the other: the busiest pair is
-// the first one (the most tiles of the first product) or the last to take one
-// of the second's.
-void choose_bn_two(DenseParams* p, int pairs) {
-  int64_t best_cost = INT64_MAX;
-  for (int b0 = 256; b0 >= 64; b0 -= 32)
-    for (int b1 = 256; b1 >= 64; b1 -= 32) {
-      const int64_t t0 = tile_count(p[0], b0), t1 = tile_count(p[1], b1);
-      const int64_t c0 = tile_cost(p[0], b0, true), c1 = tile_cost(p[1], b1, true);
-      const int64_t all = div_up(t0 + t1, pairs), most0 = div_up(t0, pairs), least0 = t0 / pairs;
-      int64_t cost = most0 * c0 + (all - most0) * c1;
-      const int64_t other = least0 * c0 + (all - least0) * c1;
-      if ((t0 + t1) % pairs == 0 || (t0 + t1) % pairs > t0 % pairs)   // a pair has one tile of the first less
-        cost = cost > other ? cost : other;
-      if (cost < best_cost) {
-        best_cost = cost;
-        p[0].bn = b0;
-        p[1].bn = b1;
-      }
-    }
+  return plan;
 }
 
 // Derived fields of a 16-bit product with its bn chosen.
@@ -804,56 +868,52 @@ int launch_dense_pair(DenseEpi epi, const DenseOperand& a, const DenseOperand& b
   grp.splits = 1;
   DenseParams& p = grp.p[0];
   p = params;
-  choose_shape(&grp, gate, sm_count);
+  const DensePlan plan = choose_shape(p, gate, false, sm_count);
+  p.bn = plan.bn[0];
+  grp.splits = plan.splits;
   finish(&p, gate, false);
   p.vec32 = aligned(p.out, 32) && (p.ldo * 2) % 32 == 0;
-  grp.tiles0 = grp.tiles = p.m_tiles * p.n_tiles;
+  grp.tiles0 = grp.tiles1 = grp.tiles = p.m_tiles * p.n_tiles;
   set_ring(&grp, p.copy_bytes);
   PairMaps maps;
   if (!encode_2d(&maps.m[0], a.base, 2, a.cols, a.rows, a.pitch, 64, 128) ||
       !encode_2d(&maps.m[1], b.base, 2, b.cols, b.rows, b.pitch, 64, p.bn / 2))
     return MOE_B200_ERR_DRIVER;
-  maps.m[2] = maps.m[3] = maps.m[0];
+  for (int i = 2; i < 6; ++i) maps.m[i] = maps.m[0];
   return gate ? launch_pair<false, false, kEpiGated>(maps, grp, sm_count, dependent, s)
               : launch_pair<false, false, kEpiStore>(maps, grp, sm_count, dependent, s);
 }
 
-int launch_dense_backward(const DenseProduct* products, int count, int sm_count, bool dependent, cudaStream_t s) {
+DensePlan plan_dense_backward(const DenseProduct* products, int count, int sm_count) {
+  return count == 1 ? choose_shape(products[0].p, false, true, sm_count) : choose_shapes(products, count, sm_count);
+}
+
+int launch_dense_backward(const DenseProduct* products, int count, const DensePlan& plan, int sm_count, bool dependent,
+                          cudaStream_t s) {
   DenseGroup grp;
   std::memset(&grp, 0, sizeof(grp));
-  grp.splits = 1;
-  for (int i = 0; i < count; ++i) grp.p[i] = products[i].p;
-  if (count == 1) {
-    // with no second product its cost and tiles are zero
-    DenseParams* p = grp.p;
-    int64_t best = INT64_MAX;
-    for (int bn = 256; bn >= 64; bn -= 32) {
-      const int64_t cost = div_up(tile_count(*p, bn), sm_count / 2) * tile_cost(*p, bn, true);
-      if (cost < best) {
-        best = cost;
-        p->bn = bn;
-      }
-    }
-  } else {
-    choose_bn_two(grp.p, sm_count / 2);
-  }
+  grp.splits = plan.splits;
+  grp.lead = plan.lead;
   PairMaps maps;
   int stage = 0;
   for (int i = 0; i < count; ++i) {
     const DenseOperand &a = products[i].a, &b = products[i].b;
     DenseParams& p = grp.p[i];
+    p = products[i].p;
+    p.bn = plan.bn[i > 0];
     p.a_mn = products[i].a_mn;
     finish(&p, false, true);
     // kEpiDact writes du and, n columns on, dg
     p.vec32 = aligned(p.out, 32) && (p.ldo * 2) % 32 == 0 && (p.preact == nullptr || p.n % 16 == 0);
     grp.tiles += p.m_tiles * p.n_tiles;
     if (i == 0) grp.tiles0 = grp.tiles;
+    if (i <= 1) grp.tiles1 = grp.tiles;
     stage = stage > p.copy_bytes ? stage : p.copy_bytes;
     if (!encode_2d(&maps.m[2 * i], a.base, 2, a.cols, a.rows, a.pitch, 64, p.a_mn ? 64 : 128) ||
         !encode_2d(&maps.m[2 * i + 1], b.base, 2, b.cols, b.rows, b.pitch, 64, 64))
       return MOE_B200_ERR_DRIVER;
   }
-  if (count == 1) maps.m[2] = maps.m[3] = maps.m[0];
+  for (int i = 2 * count; i < 6; ++i) maps.m[i] = maps.m[0];
   set_ring(&grp, stage);
   return launch_pair<false, true, kEpiBackward>(maps, grp, sm_count, dependent, s);
 }
@@ -875,7 +935,7 @@ int launch_mx_pair(DenseEpi epi, const MxOperand& a, const MxOperand& b, const D
   p.copy_bytes = 2 * kTileBytes + PairTraits<true>::kScaleBytes;
   const int esz = p.out_type == kTypeFp32 ? 4 : 2;
   p.vec32 = aligned(p.out, 32) && (p.ldo * esz) % 32 == 0 && p.n % 8 == 0;
-  grp.tiles0 = grp.tiles = p.m_tiles * p.n_tiles;
+  grp.tiles0 = grp.tiles1 = grp.tiles = p.m_tiles * p.n_tiles;
   set_ring(&grp, p.copy_bytes);
   const int64_t kt = div_up(p.k, 128);
   PairMaps maps;
@@ -884,6 +944,7 @@ int launch_mx_pair(DenseEpi epi, const MxOperand& a, const MxOperand& b, const D
       !encode_2d(&maps.m[2], a.scale, 2, 256, div_up(a.rows, 128) * kt, 512, 256, 2, false) ||
       !encode_2d(&maps.m[3], b.scale, 2, 256, div_up(b.rows, 128) * kt, 512, 256, 2, false))
     return MOE_B200_ERR_DRIVER;
+  maps.m[4] = maps.m[5] = maps.m[0];
   return gate ? launch_pair<true, false, kEpiGatedQuant>(maps, grp, sm_count, dependent, s)
               : launch_pair<true, false, kEpiStore>(maps, grp, sm_count, dependent, s);
 }

@@ -82,9 +82,19 @@ struct MxOperand {
 int launch_dense_pair(DenseEpi epi, const DenseOperand& a, const DenseOperand& b, const DenseParams& p, int sm_count,
                       bool dependent, cudaStream_t s);
 
-// One or two products of the backward pass that do not depend on each other,
-// in one launch.
-int launch_dense_backward(const DenseProduct* products, int count, int sm_count, bool dependent, cudaStream_t s);
+// How a launch cuts its products into tiles.
+struct DensePlan {
+  int bn[2];           // columns per tile of the first product, of the others
+  int splits;          // K parts (a single product)
+  int lead;
+  int64_t cost;        // expected, in cycles
+};
+
+// Up to three products of the backward pass that do not depend on each other,
+// in one launch; all but the first have the same K.
+DensePlan plan_dense_backward(const DenseProduct* products, int count, int sm_count);
+int launch_dense_backward(const DenseProduct* products, int count, const DensePlan& plan, int sm_count, bool dependent,
+                          cudaStream_t s);
 
 // 4-bit operands over CTA pairs (kEpiStore, kEpiGatedQuant).
 int launch_mx_pair(DenseEpi epi, const MxOperand& a, const MxOperand& b, const DenseParams& p, int sm_count,

@@ -230,8 +230,6 @@ int moe_b200_gated_ffn_backward(const void* grad_output, int64_t grad_pitch, con
                              params(d, 2 * I, H, T, dtype, activation, grad_w13, H, dtype)};
   const DenseProduct dw2 = {dy, rows_of(hidden, T, I, I), true,
                             params(d, H, I, T, dtype, activation, grad_w2, I, dtype)};
-  DenseProduct group[2];
-  int n = 0;
   if (T <= kSkinnyMaxTokens) {
     // the weights are streamed as in the forward pass, then written
     void* lo = need_dact ? static_cast<uint8_t*>(workspace) + static_cast<size_t>(T) * I * 4 : nullptr;
@@ -239,20 +237,37 @@ int moe_b200_gated_ffn_backward(const void* grad_output, int64_t grad_pitch, con
     if (need_dact) st = launch_dense_skinny(kEpiBackward, dh.a, nullptr, dh.b, p_dh, d.sm_count, false, s);
     if (st == MOE_B200_OK && grad_x)
       st = launch_dense_skinny(kEpiBackward, dx.a, lo, dx.b, dx.p, d.sm_count, true, s);
-    if (st != MOE_B200_OK) return st;
-    if (grad_w13) group[n++] = dw13;
-    if (grad_w2) group[n++] = dw2;
-    return n > 0 ? launch_dense_backward(group, n, d.sm_count, need_dact, s) : MOE_B200_OK;
+    DenseProduct dw[2];
+    int n = 0;
+    if (grad_w13) dw[n++] = dw13;
+    if (grad_w2) dw[n++] = dw2;
+    if (st != MOE_B200_OK || n == 0) return st;
+    return launch_dense_backward(dw, n, plan_dense_backward(dw, n, d.sm_count), d.sm_count, need_dact, s);
   }
-  // dh together with dW2, then dx together with dW13
-  if (need_dact) group[n++] = dh;
-  if (grad_w2) group[n++] = dw2;
-  if (n > 0) st = launch_dense_backward(group, n, d.sm_count, false, s);
-  if (st != MOE_B200_OK) return st;
-  n = 0;
-  if (grad_x) group[n++] = dx;
-  if (grad_w13) group[n++] = dw13;
-  return n > 0 ? launch_dense_backward(group, n, d.sm_count, true, s) : MOE_B200_OK;
+  DenseProduct first[2], second[3];
+  int n1 = 0, n2 = 0;
+  if (need_dact) first[n1++] = dh;
+  if (grad_x) second[n2++] = dx;
+  if (grad_w13) second[n2++] = dw13;
+  DensePlan plan1 = {}, plan2 = {};
+  if (n1 > 0) plan1 = plan_dense_backward(first, n1, d.sm_count);
+  if (n2 > 0) plan2 = plan_dense_backward(second, n2, d.sm_count);
+  if (grad_w2) {
+    // beside dh, or beside the others while dh has its K range split
+    first[n1] = second[n2] = dw2;
+    const DensePlan with1 = plan_dense_backward(first, n1 + 1, d.sm_count);
+    const DensePlan with2 = n2 > 0 ? plan_dense_backward(second, n2 + 1, d.sm_count) : DensePlan{};
+    if (n2 == 0 || with1.cost + plan2.cost <= plan1.cost + with2.cost) {
+      plan1 = with1;
+      ++n1;
+    } else {
+      plan2 = with2;
+      ++n2;
+    }
+  }
+  if (n1 > 0) st = launch_dense_backward(first, n1, plan1, d.sm_count, false, s);
+  if (st != MOE_B200_OK || n2 == 0) return st;
+  return launch_dense_backward(second, n2, plan2, d.sm_count, n1 > 0, s);
 }
 
 size_t moe_b200_mxfp4_scale_bytes(int64_t rows, int64_t cols) {

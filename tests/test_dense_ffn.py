@@ -200,6 +200,28 @@ def test_needs(cuda_device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T,H,inter", [(16, 520, 264), (129, 4104, 264), (600, 2056, 1032)])
+def test_every_subset_of_gradients(cuda_device, T, H, inter):
+    """Which gradients are asked for decides how the products share launches
+    and whether K is split: each subset holds the bounds."""
+    import ffn_host
+
+    x, w13, w2, dy = _inputs(T, H, inter, torch.bfloat16, seed=9)
+    _, saved = ffn_host.gated_ffn_forward(x, w13, w2)
+    want = ref.ffn(x, w13, w2, "silu", dy)
+    for mask in range(1, 8):
+        needs = [bool(mask >> i & 1) for i in range(3)]
+        got = ffn_host.gated_ffn_backward(dy, x, w13, w2, saved, needs=needs)
+        again = ffn_host.gated_ffn_backward(dy, x, w13, w2, saved, needs=needs)
+        for name, need, g, h in zip(("dx", "dw13", "dw2"), needs, got, again):
+            assert (g is not None) == need
+            if need:
+                ref.assert_within(g, want[name], name)
+                assert torch.equal(g, h)
+    assert ffn_host.read_status() == 0
+
+
+@pytest.mark.gpu
 def test_no_tokens(cuda_device):
     import ffn_host
 
