@@ -104,8 +104,7 @@ int launch_mx_pair(DenseEpi epi, const MxOperand& a, const MxOperand& b, const D
 // (kEpiStore and kEpiGated; kEpiBackward with B stored K x N; 4-bit:
 // kEpiStore).
 // With a_lo set the operand is the sum of the two matrices a and a_lo (at most
-// kTwoPartRows rows).
-constexpr int64_t kTwoPartRows = 128;
+// 128 rows).
 int launch_dense_skinny(DenseEpi epi, const DenseOperand& a, const void* a_lo, const DenseOperand& b, DenseParams p,
                         int sm_count, bool dependent, cudaStream_t s);
 int launch_mx_skinny(const MxOperand& a, const MxOperand& b, DenseParams p, int sm_count, bool dependent,

@@ -1,5 +1,5 @@
 // Dense GEMMs with few rows (sm_100a): out[t, n] = sum_k x[t, k] w[n, k] for
-// up to 128 tokens per tile, where streaming the weights is the whole cost.
+// up to 64 tokens (4-bit operands: 128), where streaming the weights is the whole cost.
 //
 // The weights take the MMA's M side (128 rows per tile) and the tokens its N
 // side (16 to 128), so a handful of tokens wastes no tensor time and every
@@ -16,15 +16,15 @@
 // Backward form (16-bit): the weights are stored K x N, as dh = dy W2 and dx =
 // [du | dg] W13 read them; the descriptor takes them so, and the adding
 // threads of dh compute du and dg, in two parts like the hidden (gradients at
-// 16 tokens, H = 7168, I = 2048, against CTA pairs: 89 -> 55 us; at 128 95 ->
-// 80; 16 x 2048 x 1024 29 -> 17).
+// 16 tokens, H = 7168, I = 2048, against CTA pairs: 67 -> 57 us, at 64 69 ->
+// 64; H = 2048, I = 1024 at 16 tokens 21 -> 17).
 //
 // The 16-bit block keeps its hidden (and [du | dg] for dx) as the sum of two 16-bit numbers, h rounded
 // and what that left, rounded again: the second product takes both as
-// neighbouring token tiles of one MMA (N = 2 x 16 to 2 x 128) and their sums
+// neighbouring token tiles of one MMA (N = 2 x 16 to 2 x 64) and their sums
 // are added with the parts. The result then carries one rounding instead of
 // two. Up to 32 tokens this is free, the tokens being next to nothing beside
-// the weights; at 64 it costs 3 % (25.6 -> 26.4 us), at 128 4 %.
+// the weights; at 64 it costs 3 % (25.6 -> 26.4 us).
 //
 // 4-bit, up to four tokens: the kernel brings its token operand to 4 bits
 // itself, from x or from the fp32 up and gate sums of the GEMM before. Each

@@ -20,9 +20,12 @@ namespace {
 constexpr int64_t kMaxDim = 65536;
 // Up to this many tokens the GEMMs stream the weights through
 // dense_skinny.cu; above (and for the weights' gradients), they run over CTA
-// pairs.
-constexpr int64_t kSkinnyMaxTokens = 128;
-static_assert(kSkinnyMaxTokens == kTwoPartRows, "the streaming form keeps two parts");
+// pairs. 16 bits, block over pairs / streaming at 64, 96 and 128 tokens: H =
+// 2048, I = 1024 15.2 / 13.9, 16.3 / 21.2 and 17.3 / 24.3 us; 7168, 512 17.9 /
+// 16.5, 19.2 / 17.9 and 19.1 / 19.9; 7168, 2048 30.5 / 25.3, 31.1 / 28.3 and
+// 31.7 / 31.2. 4 bits, linear 4096 x 7168: 15.5 / 12.0 at 128.
+constexpr int64_t kStreamTokens = MOE_B200_FFN_TWO_PART_TOKENS;
+constexpr int64_t kMxStreamTokens = 128;
 
 size_t round256(size_t x) { return (x + 255) / 256 * 256; }
 
@@ -56,7 +59,7 @@ DenseOperand rows_of(const void* base, int64_t rows, int64_t cols, int64_t pitch
 // ---- the forward GEMMs: out = x w^T, gated or plain ------------------------
 int forward_gemm(DenseEpi epi, const DenseOperand& x, const void* x_lo, const DenseOperand& w, const DenseParams& p,
                  const Device& d, bool dependent, cudaStream_t s) {
-  if (p.m <= kSkinnyMaxTokens) return launch_dense_skinny(epi, x, x_lo, w, p, d.sm_count, dependent, s);
+  if (p.m <= kStreamTokens) return launch_dense_skinny(epi, x, x_lo, w, p, d.sm_count, dependent, s);
   return launch_dense_pair(epi, x, w, p, d.sm_count, dependent, s);
 }
 
@@ -114,7 +117,7 @@ int rows_to_4_bits(const void* x, int type, int64_t pitch, const MxBuffers& to, 
 
 int mx_gemm(const MxOperand& a, const MxOperand& b, const DenseParams& p, const Device& d, bool dependent,
             cudaStream_t s) {
-  if (p.m <= kSkinnyMaxTokens) return launch_mx_skinny(a, b, p, d.sm_count, dependent, s);
+  if (p.m <= kMxStreamTokens) return launch_mx_skinny(a, b, p, d.sm_count, dependent, s);
   return launch_mx_pair(kEpiStore, a, b, p, d.sm_count, dependent, s);
 }
 
@@ -138,7 +141,7 @@ DenseParams params(const Device& d, int64_t m, int64_t n, int64_t k, int type, i
 // epilogue, where the gate rows start on an exponent tile. Otherwise the sums
 // go through memory in fp32. (The streaming form with its up and gate tiles
 // in one cluster was slower than that: 32 against 24 us at 128 tokens.)
-bool fused_gate_quant(int64_t T, int64_t I) { return T > kSkinnyMaxTokens && I % 128 == 0; }
+bool fused_gate_quant(int64_t T, int64_t I) { return T > kMxStreamTokens && I % 128 == 0; }
 
 size_t mx_ffn_bytes(int64_t T, int64_t H, int64_t I) {
   return mx_bytes(T, H) + mx_bytes(T, I) + (fused_gate_quant(T, I) ? 0 : round256(static_cast<size_t>(T) * I * 8));
@@ -155,7 +158,7 @@ size_t moe_b200_gated_ffn_workspace_bytes(int64_t num_tokens, int64_t hidden_siz
   if (!tokens_ok(num_tokens) || !dim_ok(hidden_size, 8) || !dim_ok(inter_size, 8)) return 0;
   // the hidden, and what its rounding left
   const size_t hidden = round256(static_cast<size_t>(num_tokens) * inter_size * 2);
-  return (num_tokens <= kTwoPartRows ? 2 : 1) * hidden + 256;
+  return (num_tokens <= kStreamTokens ? 2 : 1) * hidden + 256;
 }
 
 int moe_b200_gated_ffn(const void* x, int64_t x_pitch, const void* w13, const void* w2, int dtype, int activation,
@@ -166,7 +169,7 @@ int moe_b200_gated_ffn(const void* x, int64_t x_pitch, const void* w13, const vo
       !pitch_ok(x_pitch, H))
     return MOE_B200_ERR_INVALID_ARGUMENT;
   if (T == 0) return MOE_B200_OK;
-  const bool two_part = T <= kTwoPartRows;
+  const bool two_part = T <= kStreamTokens;
   const bool need_workspace = !hidden || two_part;
   if (!x || !w13 || !w2 || !output || (need_workspace && !workspace)) return MOE_B200_ERR_INVALID_ARGUMENT;
   if (!aligned(x, 16) || !pitch_aligned(x_pitch, 2) || !aligned(w13, 16) || !aligned(w2, 16) || !aligned(output, 16) ||
@@ -193,7 +196,7 @@ int moe_b200_gated_ffn(const void* x, int64_t x_pitch, const void* w13, const vo
 size_t moe_b200_gated_ffn_backward_workspace_bytes(int64_t num_tokens, int64_t hidden_size, int64_t inter_size) {
   if (!tokens_ok(num_tokens) || !dim_ok(hidden_size, 8) || !dim_ok(inter_size, 8)) return 0;
   // [du | dg], and what its rounding left
-  return round256(static_cast<size_t>(num_tokens) * inter_size * 4 * (num_tokens <= kTwoPartRows ? 2 : 1)) + 256;
+  return round256(static_cast<size_t>(num_tokens) * inter_size * 4 * (num_tokens <= kStreamTokens ? 2 : 1)) + 256;
 }
 
 int moe_b200_gated_ffn_backward(const void* grad_output, int64_t grad_pitch, const void* x, int64_t x_pitch,
@@ -239,7 +242,7 @@ int moe_b200_gated_ffn_backward(const void* grad_output, int64_t grad_pitch, con
                              params(d, 2 * I, H, T, dtype, activation, grad_w13, H, dtype)};
   const DenseProduct dw2 = {dy, rows_of(hidden, T, I, I), true,
                             params(d, H, I, T, dtype, activation, grad_w2, I, dtype)};
-  if (T <= kSkinnyMaxTokens) {
+  if (T <= kStreamTokens) {
     // the weights are streamed as in the forward pass, then written
     void* lo = need_dact ? static_cast<uint8_t*>(workspace) + static_cast<size_t>(T) * I * 4 : nullptr;
     p_dh.out_lo = lo;

@@ -255,7 +255,7 @@ PyObject* gated_ffn_save(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (f.T > 0) {
     const c10::cuda::CUDAGuard guard(dev);
     // (a few tokens keep a second part of the hidden in the workspace)
-    const Scratch ws(f.T <= 128 ? lib.gated_ffn_bytes(f.T, f.H, f.I) : 0, dev);
+    const Scratch ws(f.T <= MOE_B200_FFN_TWO_PART_TOKENS ? lib.gated_ffn_bytes(f.T, f.H, f.I) : 0, dev);
     code = lib.gated_ffn(f.x->const_data_ptr(), f.pitch, f.w13->const_data_ptr(), f.w2->const_data_ptr(), f.type,
                          static_cast<int>(PyLong_AsLong(a[3])), f.T, f.H, f.I, out.mutable_data_ptr(),
                          static_cast<float*>(preact.mutable_data_ptr()), hidden.mutable_data_ptr(), ws.ptr(),

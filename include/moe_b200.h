@@ -464,6 +464,7 @@ MOE_B200_API int moe_b200_a2a_read_status(const void* area, uint32_t* status, in
 #define MOE_B200_TYPE_BF16 0
 #define MOE_B200_TYPE_FP16 1
 #define MOE_B200_TYPE_FP32 2
+#define MOE_B200_FFN_TWO_PART_TOKENS 64
 #define MOE_B200_ACT_SILU 0
 #define MOE_B200_ACT_GELU_TANH 1
 
@@ -471,13 +472,14 @@ MOE_B200_API int moe_b200_a2a_read_status(const void* area, uint32_t* status, in
  * Gated feed-forward block: with [u | g] = x w13^T (rows [0, I) of w13 up,
  * [I, 2I) gate, the order of gemm1_weights above), h = act(g) * u and
  * output = h w2^T. fp32 sums; h is rounded to `dtype`, the type (bf16 or fp16)
- * of x, the weights and the output. For up to 128 tokens what that rounding
+ * of x, the weights and the output. For up to MOE_B200_FFN_TWO_PART_TOKENS
+ * tokens, which stream the weights through other kernels, what that rounding
  * left is kept as well, as a second number of that type, and enters output.
  *   x [T, H], w13 [2I, H], w2 [H, I], output [T, H]; H and I multiples of 8
  *   preact   fp32 [T, 2I] or NULL: receives u and g, for the gradients (kept
  *            in 32 bits, because their rounding would enter du and dg)
  *   hidden   [T, I] or NULL: receives h rounded; NULL keeps it in the workspace
- * workspace may be NULL when hidden is given and there are more than 128 tokens.
+ * workspace may be NULL when hidden is given and there are more tokens than that.
  */
 MOE_B200_API size_t moe_b200_gated_ffn_workspace_bytes(int64_t num_tokens, int64_t hidden_size, int64_t inter_size);
 MOE_B200_API int moe_b200_gated_ffn(const void* x, int64_t x_pitch, const void* w13, const void* w2, int dtype,
@@ -489,7 +491,7 @@ MOE_B200_API int moe_b200_gated_ffn(const void* x, int64_t x_pitch, const void* 
  * Gradients of the block for grad_output [T, H], from the preact and hidden
  * that the forward call saved: with dh = grad_output w2, du = dh act(g) and
  * dg = dh u act'(g) (rounded to dtype as operands of the products below; for
- * up to 128 tokens what that left enters grad_x as well),
+ * up to MOE_B200_FFN_TWO_PART_TOKENS tokens what that left enters grad_x too),
  *   grad_x   = [du | dg] w13          [T, H]
  *   grad_w13 = [du | dg]^T x          [2I, H]
  *   grad_w2  = grad_output^T hidden   [H, I]

@@ -6,7 +6,7 @@ Bounds count, for every element:
     value, and half the smallest step of fp16's subnormals, 2^-25;
   * the rounding of the 16-bit intermediates (h, du, dg), carried through the
     product that reads them by the absolute values of its other operand; for up
-    to 128 tokens y and dx read them as two 16-bit numbers, so the rounding
+    to 64 tokens y and dx read them as two 16-bit numbers, so the rounding
     there is u squared of the value;
   * the fp32 sums: a sum of k products is k / 16 additions of 16-term blocks,
     each addition off by at most 2^-23 of the sum of magnitudes (a tensor core
@@ -23,6 +23,7 @@ import torch
 U = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}
 TINY = {torch.bfloat16: 0.0, torch.float16: 2.0 ** -25, torch.float32: 0.0}
 ACT = 4e-6
+TWO_PART = 64
 
 
 def gamma(k: int) -> float:
@@ -57,10 +58,10 @@ def ffn(x, w13, w2, name, dy=None):
     h = a * up
     e_h = e_a * up.abs() + a.abs() * e_up + e_a * e_up
     r_h = e_h + u_ * (h.abs() + e_h) + tiny            # after the rounding to 16 bits
-    y_h = e_h + u_ * u_ * (h.abs() + e_h) + tiny if T <= 128 else r_h
+    y_h = e_h + u_ * u_ * (h.abs() + e_h) + tiny if T <= TWO_PART else r_h
     y = h @ w2.T
     # two parts: twice the terms in the sum
-    e_y = y_h @ w2.abs().T + (2 if T <= 128 else 1) * gamma(inter) * ((h.abs() + r_h) @ w2.abs().T)
+    e_y = y_h @ w2.abs().T + (2 if T <= TWO_PART else 1) * gamma(inter) * ((h.abs() + r_h) @ w2.abs().T)
     out = {"y": (y, e_y + u_ * (y.abs() + e_y) + tiny)}
     if dy is None:
         return out
@@ -76,7 +77,7 @@ def ffn(x, w13, w2, name, dy=None):
     r_d = e_d + u_ * (d.abs() + e_d) + tiny
 
     # dx of few tokens reads [du | dg] in two parts, like y
-    d_x = e_d + u_ * u_ * (d.abs() + e_d) + tiny if T <= 128 else r_d
+    d_x = e_d + u_ * u_ * (d.abs() + e_d) + tiny if T <= TWO_PART else r_d
 
     def product(left, e_left, right, k, parts=1):
         v = left @ right
@@ -84,7 +85,7 @@ def ffn(x, w13, w2, name, dy=None):
         e = m + parts * gamma(k) * (left.abs() @ right.abs() + m)
         return v, e + u_ * (v.abs() + e) + tiny
 
-    out["dx"] = product(d, d_x, w13, 2 * inter, 2 if T <= 128 else 1)
+    out["dx"] = product(d, d_x, w13, 2 * inter, 2 if T <= TWO_PART else 1)
     out["dw13"] = product(d.T, r_d.T, x, T)
     v, e = product(h.T, r_h.T, dy, T)
     out["dw2"] = (v.T, e.T)

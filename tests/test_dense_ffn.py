@@ -19,7 +19,7 @@ def _inputs(T, H, inter, dtype, seed=0, device="cuda"):
 
 
 # one token to several tiles; sizes that end inside a tile in every direction
-# (token tiles of 16, 128 and 256, feature tiles of 64 and 128, 64-wide K
+# (token tiles of 16, 64 and 256, feature tiles of 64 and 128, 64-wide K
 # steps), the smallest sizes, and the split of K over 1 to 8 CTAs and over 1,
 # 2 and 4 pairs
 SHAPES = [(1, 8, 8), (1, 7168, 2048), (3, 64, 64), (16, 520, 264), (17, 1032, 520), (64, 2048, 136), (65, 4096, 64),
@@ -134,7 +134,7 @@ def test_rows_do_not_mix(cuda_device, T):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("T", [1, 64, 128, 129])
+@pytest.mark.parametrize("T", [1, 64, 65, 129])
 def test_hidden_beyond_half_precision(cuda_device, T):
     """A hidden value beyond fp16 is infinite, with its sign, and so are the
     outputs it enters; nothing turns into NaN."""
@@ -543,7 +543,7 @@ def test_c_abi_refusals():
         assert fwd(**bad) == 2, bad
     need = lib.moe_b200_gated_ffn_workspace_bytes(4, 64, 32)
     assert need >= 2 * 4 * 32 * 2 and fwd(n=need - 1) == 3
-    assert fwd(hid=p, n=need - 1) == 3 and fwd(hid=p, ws=None) == 1   # the second part of up to 128 tokens' hidden
+    assert fwd(hid=p, n=need - 1) == 3 and fwd(hid=p, ws=None) == 1   # the second part of up to 64 tokens' hidden
     need = lib.moe_b200_gated_ffn_workspace_bytes(129, 64, 32)
     assert need >= 129 * 32 * 2 and fwd(T=129, n=need - 1) == 3
     assert fwd(T=0, x=None, out=None) == 0
