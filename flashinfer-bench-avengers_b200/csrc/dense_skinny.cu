@@ -1,5 +1,6 @@
 // Dense GEMMs with few rows (sm_100a): out[t, n] = sum_k x[t, k] w[n, k] for
-// up to 64 tokens (4-bit operands: 128), where streaming the weights is the whole cost.
+// up to 64 tokens (a 4-bit product alone: 128), where streaming the weights is
+// the whole cost.
 //
 // The weights take the MMA's M side (128 rows per tile) and the tokens its N
 // side (16 to 128), so a handful of tokens wastes no tensor time and every

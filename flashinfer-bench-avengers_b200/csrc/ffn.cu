@@ -23,7 +23,10 @@ constexpr int64_t kMaxDim = 65536;
 // pairs. 16 bits, block over pairs / streaming at 64, 96 and 128 tokens: H =
 // 2048, I = 1024 15.2 / 13.9, 16.3 / 21.2 and 17.3 / 24.3 us; 7168, 512 17.9 /
 // 16.5, 19.2 / 17.9 and 19.1 / 19.9; 7168, 2048 30.5 / 25.3, 31.1 / 28.3 and
-// 31.7 / 31.2. 4 bits, linear 4096 x 7168: 15.5 / 12.0 at 128.
+// 31.7 / 31.2. 4 bits, the same block: at 80 tokens 14.1 / 15.7, 18.8 / 17.3
+// and 21.5 / 20.1, at 128 14.9 / 18.2, 19.3 / 21.0 and 22.3 / 24.1. A 4-bit
+// product alone, whose sums take no further kernel, streams for longer (4096 x
+// 7168 at 128 tokens 15.4 / 12.2, 1024 x 2048 9.1 / 7.8).
 constexpr int64_t kStreamTokens = MOE_B200_FFN_TWO_PART_TOKENS;
 constexpr int64_t kMxStreamTokens = 128;
 
@@ -115,9 +118,9 @@ int rows_to_4_bits(const void* x, int type, int64_t pitch, const MxBuffers& to, 
   return MOE_B200_OK;
 }
 
-int mx_gemm(const MxOperand& a, const MxOperand& b, const DenseParams& p, const Device& d, bool dependent,
-            cudaStream_t s) {
-  if (p.m <= kMxStreamTokens) return launch_mx_skinny(a, b, p, d.sm_count, dependent, s);
+int mx_gemm(const MxOperand& a, const MxOperand& b, const DenseParams& p, const Device& d, int64_t stream_tokens,
+            bool dependent, cudaStream_t s) {
+  if (p.m <= stream_tokens) return launch_mx_skinny(a, b, p, d.sm_count, dependent, s);
   return launch_mx_pair(kEpiStore, a, b, p, d.sm_count, dependent, s);
 }
 
@@ -141,7 +144,7 @@ DenseParams params(const Device& d, int64_t m, int64_t n, int64_t k, int type, i
 // epilogue, where the gate rows start on an exponent tile. Otherwise the sums
 // go through memory in fp32. (The streaming form with its up and gate tiles
 // in one cluster was slower than that: 32 against 24 us at 128 tokens.)
-bool fused_gate_quant(int64_t T, int64_t I) { return T > kMxStreamTokens && I % 128 == 0; }
+bool fused_gate_quant(int64_t T, int64_t I) { return T > kStreamTokens && I % 128 == 0; }
 
 size_t mx_ffn_bytes(int64_t T, int64_t H, int64_t I) {
   return mx_bytes(T, H) + mx_bytes(T, I) + (fused_gate_quant(T, I) ? 0 : round256(static_cast<size_t>(T) * I * 8));
@@ -337,7 +340,8 @@ int moe_b200_mxfp4_matmul(const void* a_q, const void* a_scale, const void* b_q,
   const int st = open_device(&d);
   if (st != MOE_B200_OK) return st;
   return mx_gemm(MxOperand{a_q, a_scale, m}, MxOperand{b_q, b_scale, n},
-                 params(d, m, n, k, MOE_B200_TYPE_BF16, 0, out, n, dtype), d, false, static_cast<cudaStream_t>(stream));
+                 params(d, m, n, k, MOE_B200_TYPE_BF16, 0, out, n, dtype), d, kMxStreamTokens, false,
+                 static_cast<cudaStream_t>(stream));
 }
 
 size_t moe_b200_mxfp4_linear_workspace_bytes(int64_t num_tokens, int64_t k) {
@@ -366,7 +370,7 @@ int moe_b200_mxfp4_linear(const void* x, int64_t x_pitch, int dtype, const void*
   const bool inside = mx_skinny_quantizes(T, n, k, d.sm_count);
   st = rows_to_4_bits(x, dtype, x_pitch, xq, inside, &p, d, s);
   if (st != MOE_B200_OK) return st;
-  return mx_gemm(MxOperand{xq.q, xq.scale, T}, MxOperand{w_q, w_scale, n}, p, d, !inside, s);
+  return mx_gemm(MxOperand{xq.q, xq.scale, T}, MxOperand{w_q, w_scale, n}, p, d, kMxStreamTokens, !inside, s);
 }
 
 size_t moe_b200_mxfp4_gated_ffn_workspace_bytes(int64_t num_tokens, int64_t hidden_size, int64_t inter_size) {
@@ -406,14 +410,14 @@ int moe_b200_mxfp4_gated_ffn(const void* x, int64_t x_pitch, int dtype, const vo
     if (st != MOE_B200_OK) return st;
     st = launch_mx_pair(kEpiGatedQuant, xo, w13, p, d.sm_count, true, s);
     if (st != MOE_B200_OK) return st;
-    return mx_gemm(ho, w2, params(d, T, H, I, dtype, activation, output, H, dtype), d, true, s);
+    return mx_gemm(ho, w2, params(d, T, H, I, dtype, activation, output, H, dtype), d, kStreamTokens, true, s);
   }
   float* sums = reinterpret_cast<float*>(ws + mx_bytes(T, H) + mx_bytes(T, I));
   DenseParams p = params(d, T, 2 * I, H, dtype, activation, sums, 2 * I, MOE_B200_TYPE_FP32);
   const bool x_inside = mx_skinny_quantizes(T, 2 * I, H, d.sm_count);
   st = rows_to_4_bits(x, dtype, x_pitch, xq, x_inside, &p, d, s);
   if (st != MOE_B200_OK) return st;
-  st = mx_gemm(xo, w13, p, d, !x_inside, s);
+  st = mx_gemm(xo, w13, p, d, kStreamTokens, !x_inside, s);
   if (st != MOE_B200_OK) return st;
   DenseParams p2 = params(d, T, H, I, dtype, activation, output, H, dtype);
   if (mx_skinny_quantizes(T, H, I, d.sm_count)) {
@@ -427,7 +431,7 @@ int moe_b200_mxfp4_gated_ffn(const void* x, int64_t x_pitch, int dtype, const vo
                       activation, hq.q, hq.scale) != cudaSuccess)
       return MOE_B200_ERR_CUDA;
   }
-  return mx_gemm(ho, w2, p2, d, true, s);
+  return mx_gemm(ho, w2, p2, d, kStreamTokens, true, s);
 }
 
 int moe_b200_dense_read_status(uint32_t* status, void* stream) {

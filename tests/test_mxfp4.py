@@ -107,7 +107,7 @@ def test_nan_blocks_stay_in_their_rows(cuda_device, M):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("T", [1, 20, 130, 400])
+@pytest.mark.parametrize("T", [1, 20, 65, 128, 130, 400])
 @pytest.mark.parametrize("dtype", TYPES)
 def test_linear(cuda_device, T, dtype):
     """Equal to quantiser and product called one after the other, within the
@@ -171,7 +171,8 @@ def _check_block(x, w13, w2, activation, y, what):
 # T <= 128 and ragged I: the sums go through memory; T > 128 and whole
 # 128-feature tiles: the hidden is brought to 4 bits in the GEMM's epilogue
 @pytest.mark.gpu
-@pytest.mark.parametrize("T,H,inter", [(1, 256, 128), (16, 544, 288), (128, 256, 256), (129, 256, 256), (200, 288, 96),
+@pytest.mark.parametrize("T,H,inter", [(1, 256, 128), (16, 544, 288), (64, 256, 256), (65, 544, 288),
+                                       (100, 288, 256), (128, 256, 256), (129, 256, 256), (200, 288, 96),
                                        (300, 512, 640)])
 @pytest.mark.parametrize("dtype,activation", [(torch.bfloat16, "silu"), (torch.float16, "gelu_tanh")])
 def test_block(cuda_device, T, H, inter, dtype, activation):
