@@ -24,7 +24,7 @@
 // without MMAs. Under sustained load the power cap sets the clock (1.1 to 1.5
 // GHz), and the rate is that of the vendor's library GEMM on the same
 // operands. 4-bit operands need the same bytes per step, so their MMAs, at
-// four times the rate, reach 5.6 PFLOP/s.
+// four times the rate, reach 6.1 PFLOP/s.
 //
 // The operands may be stored along K or along the output dimension (the
 // gradients need W^T and X^T): the shared-memory descriptors take both, so

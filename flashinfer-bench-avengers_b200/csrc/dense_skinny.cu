@@ -17,8 +17,9 @@
 // Backward form (16-bit): the weights are stored K x N, as dh = dy W2 and dx =
 // [du | dg] W13 read them; the descriptor takes them so, and the adding
 // threads of dh compute du and dg, in two parts like the hidden (gradients at
-// 16 tokens, H = 7168, I = 2048, against CTA pairs: 67 -> 57 us, at 64 69 ->
-// 64; H = 2048, I = 1024 at 16 tokens 21 -> 17).
+// 16 tokens, H = 7168, I = 2048, against CTA pairs: 53 -> 50 us, of x alone 34
+// -> 22; H = 2048, I = 1024 21 -> 17; at 64 tokens 55 -> 57, 38 -> 29 and 22
+// -> 22).
 //
 // The 16-bit block keeps its hidden (and [du | dg] for dx) as the sum of two 16-bit numbers, h rounded
 // and what that left, rounded again: the second product takes both as

@@ -168,7 +168,7 @@ def _check_block(x, w13, w2, activation, y, what):
     ref.assert_within(y.cpu(), (value, bound + spread * (1 + 2 * ref.U[dt])), what)
 
 
-# T <= 128 and ragged I: the sums go through memory; T > 128 and whole
+# T <= 64 and ragged I: the sums go through memory; T > 64 and whole
 # 128-feature tiles: the hidden is brought to 4 bits in the GEMM's epilogue
 @pytest.mark.gpu
 @pytest.mark.parametrize("T,H,inter", [(1, 256, 128), (16, 544, 288), (64, 256, 256), (65, 544, 288),
