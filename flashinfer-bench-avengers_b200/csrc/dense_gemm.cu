@@ -794,11 +794,13 @@ int max_clusters(int ctas) {
 // training step at 4096 tokens 813 -> 786 us, at 333 x 1032 x 520 75 -> 55 us.
 // A pair's MMA takes N in multiples of 32, which also keeps the columns of a
 // tile in whole 32-byte stores. A split product is one wave of clusters and
-// adds its parts for kAddCost. (How many clusters of 4 or 8 CTAs run at once
+// adds its parts for 6000 units, in the backward pass for fewer with narrow
+// tiles (training step at 333 x 1032 x 520 32.5 -> 30.5 us, at 512 x 7168 x
+// 2048 135.5 -> 128.4; in the forward pass that chose worse: block at 129 x
+// 1024 x 512 10.6 -> 11.6). (How many clusters of 4 or 8 CTAs run at once
 // depends on how the GPU's SMs are grouped, 33 and 15 where this was measured;
 // one more made 256 tokens take 56 us.)
 DensePlan choose_shape(const DenseParams& p, bool gate, bool b_mn, int sm_count) {
-  constexpr int64_t kAddCost = 6000;
   DensePlan plan = {};
   plan.cost = INT64_MAX;
   for (int splits = 1; splits <= 4; splits *= 2) {
@@ -807,7 +809,7 @@ DensePlan choose_shape(const DenseParams& p, bool gate, bool b_mn, int sm_count)
       const int64_t tiles = tile_count(p, gate ? bn / 2 : bn);
       if (splits > 1 && tiles > max_clusters(2 * splits)) continue;
       const int64_t waves = splits > 1 ? 1 : div_up(tiles, sm_count / 2);
-      const int64_t cost = waves * tile_cost(p, bn, b_mn, splits) + (splits > 1 ? kAddCost : 0);
+      const int64_t cost = waves * tile_cost(p, bn, b_mn, splits) + (splits > 1 ? (b_mn ? 2500 + 14 * bn : 6000) : 0);
       if (cost < plan.cost) plan = DensePlan{{bn, 0}, splits, 0, cost};
     }
   }
