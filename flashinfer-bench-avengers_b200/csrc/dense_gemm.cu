@@ -42,7 +42,8 @@
 // and end each (training step at 4096 tokens 824 -> 796 us, 333 x 1032 x 520
 // 48 -> 39 us). With dh split and dW2 beside dx and dW13, against dW2 always
 // beside an unsplit dh: gradients at H = 7168, I = 2048 and 129 tokens 95 ->
-// 68 us, at 512 103 -> 93, at 1024 156 -> 147; 1024 x 2048 x 1024 41 -> 37.
+// 68 us, at 512 103 -> 93, at 1024 156 -> 147; 1024 x 2048 x 1024 41 -> 37 (57,
+// 86, 147 and 37 since).
 #include <cuda.h>
 #include <cuda_runtime.h>
 
