@@ -520,6 +520,16 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         }
       }
     }
+    // The MMAs hand back the last ring's stages too, by arrivals in both CTAs
+    // that no load waits for: they are awaited here, so that none is still on
+    // its way to a CTA that has left. (A stage never used passes at once.)
+    for (int s = 0; ok && s < kS; ++s) {
+      ok = warp_wait(smem_u32(empty_bar) + 8u * stage, ph ^ 1u, s_abort, status, kStatusTimeoutProducer);
+      if (++stage == kS) {
+        stage = 0;
+        ph ^= 1u;
+      }
+    }
     if (!ok) drain_copies();
   } else if (warp == 1) {
     // --------------------------------------------------------------- MMA

@@ -281,11 +281,10 @@ __global__ void __launch_bounds__(kThreads)
     __syncwarp();
     int stage = first == sh.stages ? 0 : first;
     uint32_t ph = 0;
+    bool ok = true;
     for (int i = first; i < iters; ++i) {
-      if (!warp_wait(smem_u32(empty_bar) + 8u * stage, ph, s_abort, p.status, kStatusTimeoutProducer)) {
-        drain_copies();
-        break;
-      }
+      ok = warp_wait(smem_u32(empty_bar) + 8u * stage, ph, s_abort, p.status, kStatusTimeoutProducer);
+      if (!ok) break;
       if (issue) {
         load_w(i, stage);
         load_x(i, stage);
@@ -297,6 +296,12 @@ __global__ void __launch_bounds__(kThreads)
         ph ^= 1u;
       }
     }
+    // The last ring's stages are handed back too: no arrival may still be on
+    // its way to this CTA's shared memory when it leaves.
+    for (int i = iters - first; ok && i < iters; ++i)
+      ok = warp_wait(smem_u32(empty_bar) + 8u * (i % sh.stages), (i / sh.stages) & 1, s_abort, p.status,
+                     kStatusTimeoutProducer);
+    if (!ok) drain_copies();
   } else if (warp == 1) {
     // --------------------------------------------------------------- MMA
     const bool issue = elect_lane();
