@@ -17,6 +17,7 @@
 #include <ATen/core/Tensor.h>
 #include <ATen/core/grad_mode.h>
 #include <ATen/ops/empty.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -162,22 +163,32 @@ bool overlap(const at::Tensor& a, const at::Tensor& b) {
   return pa < pb + span(b) && pb < pa + span(a);
 }
 
+// Whether one of these carries a forward-mode tangent, which no call here
+// computes. (Gradient mode says nothing about forward mode: torch.no_grad()
+// leaves it on.)
+bool tangents(std::initializer_list<const at::Tensor*> ts) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return false;
+  for (const at::Tensor* t : ts)
+    if (t->_fw_grad(0).defined()) return true;
+  return false;
+}
+
 // `given` if it is an output of this shape and type, a new tensor if it is
 // None; nullopt if it will not do. A given one is written in place: it may
-// overlap no input, autograd must not follow it, and its version goes up, so
-// that a backward pass which saved it notices.
+// overlap no input, autograd must not follow it (a tangent would stay that of the
+// old values), and its version goes up, so that a backward pass which saved it
+// notices.
 std::optional<at::Tensor> output(PyObject* given, int64_t rows, int64_t cols, at::ScalarType type, at::Device dev,
                                  std::initializer_list<const at::Tensor*> inputs) {
   if (given == Py_None) return matrix(rows, cols, type, dev);
   const at::Tensor* t = tensor(given);
-  if (!dense(t, rows, cols, type, dev) || (at::GradMode::is_enabled() && t->requires_grad())) return std::nullopt;
+  if (!dense(t, rows, cols, type, dev) || (at::GradMode::is_enabled() && t->requires_grad()) || tangents({t}))
+    return std::nullopt;
   for (const at::Tensor* in : inputs)
     if (overlap(*t, *in)) return std::nullopt;
   if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
   return *t;
 }
-
-bool followed(const at::Tensor& t) { return t.requires_grad() || t._fw_grad(0).defined(); }
 
 PyObject* result(int code, const at::Tensor& t) { return code ? PyLong_FromLong(code) : THPVariable_Wrap(t); }
 
@@ -224,8 +235,9 @@ PyObject* gated_ffn(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (!ready(n, 5)) return nullptr;
   Ffn f;
-  if (!read_ffn(a[0], a[1], a[2], &f)) Py_RETURN_NONE;
-  if (at::GradMode::is_enabled() && (followed(*f.x) || followed(*f.w13) || followed(*f.w2))) Py_RETURN_FALSE;
+  if (!read_ffn(a[0], a[1], a[2], &f) || tangents({f.x, f.w13, f.w2})) Py_RETURN_NONE;
+  if (at::GradMode::is_enabled() && (f.x->requires_grad() || f.w13->requires_grad() || f.w2->requires_grad()))
+    Py_RETURN_FALSE;
   const at::Device dev = f.x->device();
   const std::optional<at::Tensor> out = output(a[4], f.T, f.H, f.x->scalar_type(), dev, {f.x, f.w13, f.w2});
   if (!out) Py_RETURN_NONE;
@@ -246,7 +258,7 @@ PyObject* gated_ffn_save(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (!ready(n, 4)) return nullptr;
   Ffn f;
-  if (!read_ffn(a[0], a[1], a[2], &f)) Py_RETURN_NONE;
+  if (!read_ffn(a[0], a[1], a[2], &f) || tangents({f.x, f.w13, f.w2})) Py_RETURN_NONE;
   const at::Device dev = f.x->device();
   const at::Tensor out = matrix(f.T, f.H, f.x->scalar_type(), dev);
   const at::Tensor preact = matrix(f.T, 2 * f.I, at::kFloat, dev);
@@ -277,7 +289,8 @@ PyObject* gated_ffn_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const at::Device dev = f.x->device();
   const int64_t dy_pitch = pitch_of(*dy);
   if (dy_pitch < 0 || dy->size(0) != f.T || dy->size(1) != f.H || dy->scalar_type() != type || dy->device() != dev ||
-      !dense(preact, f.T, 2 * f.I, at::kFloat, dev, 32) || !dense(hidden, f.T, f.I, type, dev))
+      !dense(preact, f.T, 2 * f.I, at::kFloat, dev, 32) || !dense(hidden, f.T, f.I, type, dev) ||
+      tangents({dy, f.x, f.w13, f.w2, preact, hidden}))
     Py_RETURN_NONE;
   at::Tensor grads[3];
   const int64_t shape[3][2] = {{f.T, f.H}, {2 * f.I, f.H}, {f.H, f.I}};
@@ -382,7 +395,7 @@ PyObject* mxfp4_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const at::Device dev = x->device();
   const int64_t T = x->size(0), K = x->size(1);
   Mx w;
-  if (!read_mx(a[1], a[2], &dev, &w) || w.cols != K || w.rows == 0) Py_RETURN_NONE;
+  if (!read_mx(a[1], a[2], &dev, &w) || w.cols != K || w.rows == 0 || tangents({x})) Py_RETURN_NONE;
   const std::optional<at::Tensor> out = output(a[3], T, w.rows, x->scalar_type(), dev, {x, w.q, w.scale});
   if (!out) Py_RETURN_NONE;
   int code = 0;
@@ -408,7 +421,7 @@ PyObject* mxfp4_gated_ffn(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int64_t T = x->size(0), H = x->size(1);
   Mx w13, w2;
   if (!read_mx(a[1], a[2], &dev, &w13) || !read_mx(a[3], a[4], &dev, &w2) || w13.cols != H || w2.rows != H ||
-      w13.rows != 2 * w2.cols)
+      w13.rows != 2 * w2.cols || tangents({x}))
     Py_RETURN_NONE;
   const std::optional<at::Tensor> out =
       output(a[6], T, H, x->scalar_type(), dev, {x, w13.q, w13.scale, w2.q, w2.scale});

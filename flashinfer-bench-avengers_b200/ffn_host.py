@@ -13,7 +13,9 @@ find the argument at fault and say so. They run on the current stream of the
 inputs' device. Scratch comes from torch's caching allocator call by call, so
 calls on several streams and captured graphs never share it. An ``output`` is
 written in place; it may overlap no input. Gradients are recorded by gated_ffn
-alone; the 4-bit functions serve.
+alone; the 4-bit functions serve. No function computes forward-mode
+derivatives: tensors with a tangent are refused while forward mode is on, with
+torch.no_grad() too.
 """
 from __future__ import annotations
 
@@ -23,6 +25,7 @@ import importlib.util
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 import moe_host
 
@@ -127,11 +130,18 @@ def _span(t: torch.Tensor) -> tuple[int, int]:
     return t.data_ptr(), t.data_ptr() + (elements * t.element_size() if t.numel() else 0)
 
 
+def _check_no_tangents(*tensors: torch.Tensor) -> None:
+    for t in tensors:
+        _check(forward_ad.unpack_dual(t, level=0).tangent is None,
+               "forward-mode derivatives are not computed: a tensor of the call has a tangent")
+
+
 def _check_output(output, shape: tuple, dtype: torch.dtype, dev, *inputs: torch.Tensor) -> None:
     if output is None:
         return
     _check_dense("output", output, shape, dtype, dev)
     _check(not (torch.is_grad_enabled() and output.requires_grad), "output must not require gradients")
+    _check_no_tangents(output)
     begin, end = _span(output)
     for t in inputs:
         first, last = _span(t)
@@ -243,6 +253,7 @@ def gated_ffn(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, activation: 
 
     def explain():
         T, H, _ = _check_ffn(x, w13, w2)
+        _check_no_tangents(x, w13, w2)
         _check_output(output, (T, H), x.dtype, x.device, x, w13, w2)
 
     return _answer("moe_b200_gated_ffn", got, explain)
@@ -253,7 +264,11 @@ def gated_ffn_forward(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, acti
     gated_ffn_backward: u and g in fp32 [T, 2I], and h [T, I]."""
     got = (_native or _load()).gated_ffn_save(x, w13, w2, _activation(activation))
     if not isinstance(got, tuple):
-        got = _answer("moe_b200_gated_ffn", got, lambda: _check_ffn(x, w13, w2))
+        def explain():
+            _check_ffn(x, w13, w2)
+            _check_no_tangents(x, w13, w2)
+
+        got = _answer("moe_b200_gated_ffn", got, explain)
     return got[0], got[1:]
 
 
@@ -279,6 +294,7 @@ def gated_ffn_backward(grad_output: torch.Tensor, x: torch.Tensor, w13: torch.Te
         _check_rows("grad_output", grad_output, H)
         _check_dense("saved u and g", saved[0], (T, 2 * inter), torch.float32, dev, 32)
         _check_dense("saved hidden", saved[1], (T, inter), x.dtype, dev)
+        _check_no_tangents(grad_output, x, w13, w2, *saved)
 
     return _answer("moe_b200_gated_ffn_backward", got, explain)
 
@@ -337,6 +353,7 @@ def mxfp4_linear(x: torch.Tensor, w_q: torch.Tensor, w_scale: torch.Tensor,
         _check_values("x", x)
         N, _ = _check_mx("w_q", w_q, w_scale, x.device, x.size(1))
         _check(N > 0, "w_q must have rows")
+        _check_no_tangents(x)
         _check_output(output, (x.size(0), N), x.dtype, x.device, x, w_q, w_scale)
 
     return _answer("moe_b200_mxfp4_linear", got, explain)
@@ -358,6 +375,7 @@ def mxfp4_gated_ffn(x: torch.Tensor, w13_q: torch.Tensor, w13_scale: torch.Tenso
         two_i, _ = _check_mx("w13_q", w13_q, w13_scale, x.device, H)
         _check(two_i > 0 and two_i % 64 == 0, f"w13_q must have 2 I rows, I a multiple of 32; got {two_i}")
         _check_mx("w2_q", w2_q, w2_scale, x.device, two_i // 2, H)
+        _check_no_tangents(x)
         _check_output(output, (T, H), x.dtype, x.device, x, w13_q, w13_scale, w2_q, w2_scale)
 
     return _answer("moe_b200_mxfp4_gated_ffn", got, explain)
