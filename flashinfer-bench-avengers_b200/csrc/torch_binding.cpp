@@ -173,6 +173,10 @@ bool tangents(std::initializer_list<const at::Tensor*> ts) {
   return false;
 }
 
+// Whether autograd is to record a call on x, which the 4-bit functions do not:
+// their results would silently cut the graph.
+bool recorded(const at::Tensor& x) { return at::GradMode::is_enabled() && x.requires_grad(); }
+
 // `given` if it is an output of this shape and type, a new tensor if it is
 // None; nullopt if it will not do. A given one is written in place: it may
 // overlap no input, autograd must not follow it (a tangent would stay that of the
@@ -395,7 +399,8 @@ PyObject* mxfp4_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const at::Device dev = x->device();
   const int64_t T = x->size(0), K = x->size(1);
   Mx w;
-  if (!read_mx(a[1], a[2], &dev, &w) || w.cols != K || w.rows == 0 || tangents({x})) Py_RETURN_NONE;
+  if (!read_mx(a[1], a[2], &dev, &w) || w.cols != K || w.rows == 0 || tangents({x}) || recorded(*x))
+    Py_RETURN_NONE;
   const std::optional<at::Tensor> out = output(a[3], T, w.rows, x->scalar_type(), dev, {x, w.q, w.scale});
   if (!out) Py_RETURN_NONE;
   int code = 0;
@@ -421,7 +426,7 @@ PyObject* mxfp4_gated_ffn(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int64_t T = x->size(0), H = x->size(1);
   Mx w13, w2;
   if (!read_mx(a[1], a[2], &dev, &w13) || !read_mx(a[3], a[4], &dev, &w2) || w13.cols != H || w2.rows != H ||
-      w13.rows != 2 * w2.cols || tangents({x}))
+      w13.rows != 2 * w2.cols || tangents({x}) || recorded(*x))
     Py_RETURN_NONE;
   const std::optional<at::Tensor> out =
       output(a[6], T, H, x->scalar_type(), dev, {x, w13.q, w13.scale, w2.q, w2.scale});

@@ -12,9 +12,12 @@ their conditions, allocates and launches; where it declines, the checks here
 find the argument at fault and say so. They run on the current stream of the
 inputs' device. Scratch comes from torch's caching allocator call by call, so
 calls on several streams and captured graphs never share it. An ``output`` is
-written in place; it may overlap no input. Gradients are recorded by gated_ffn
-alone; the 4-bit functions serve. No function computes forward-mode
-derivatives: tensors with a tangent are refused while forward mode is on, with
+written in place; it may overlap no input.
+
+Gradients are recorded by gated_ffn alone. The 4-bit functions serve: an x that
+requires gradients is refused while gradients are recorded (but for the
+quantiser, whose codes are integers). No function computes forward-mode
+derivatives: a tensor with a tangent is refused while forward mode is on, with
 torch.no_grad() too.
 """
 from __future__ import annotations
@@ -134,6 +137,13 @@ def _check_no_tangents(*tensors: torch.Tensor) -> None:
     for t in tensors:
         _check(forward_ad.unpack_dual(t, level=0).tangent is None,
                "forward-mode derivatives are not computed: a tensor of the call has a tangent")
+
+
+def _check_serves(x: torch.Tensor) -> None:
+    """x carries no derivative that a 4-bit function would drop."""
+    _check_no_tangents(x)
+    _check(not (torch.is_grad_enabled() and x.requires_grad),
+           "x requires gradients, which the 4-bit functions do not record: detach it, or call under torch.no_grad()")
 
 
 def _check_output(output, shape: tuple, dtype: torch.dtype, dev, *inputs: torch.Tensor) -> None:
@@ -309,7 +319,8 @@ def mxfp4_scale_shape(rows: int, cols: int) -> tuple[int, ...]:
 def mxfp4_quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """x [R, K] (bf16, fp16 or fp32; K a multiple of 32; rows may lie apart) in
     4 bits: codes uint8 [R, K / 2] and exponent bytes uint8 of
-    mxfp4_scale_shape(R, K) (moe_b200_mxfp4_quantize)."""
+    mxfp4_scale_shape(R, K) (moe_b200_mxfp4_quantize). They are integers, through
+    which no gradient passes: x may be a parameter."""
     got = (_native or _load()).mxfp4_quantize(x)
     if isinstance(got, tuple):
         return got
@@ -353,7 +364,7 @@ def mxfp4_linear(x: torch.Tensor, w_q: torch.Tensor, w_scale: torch.Tensor,
         _check_values("x", x)
         N, _ = _check_mx("w_q", w_q, w_scale, x.device, x.size(1))
         _check(N > 0, "w_q must have rows")
-        _check_no_tangents(x)
+        _check_serves(x)
         _check_output(output, (x.size(0), N), x.dtype, x.device, x, w_q, w_scale)
 
     return _answer("moe_b200_mxfp4_linear", got, explain)
@@ -375,7 +386,7 @@ def mxfp4_gated_ffn(x: torch.Tensor, w13_q: torch.Tensor, w13_scale: torch.Tenso
         two_i, _ = _check_mx("w13_q", w13_q, w13_scale, x.device, H)
         _check(two_i > 0 and two_i % 64 == 0, f"w13_q must have 2 I rows, I a multiple of 32; got {two_i}")
         _check_mx("w2_q", w2_q, w2_scale, x.device, two_i // 2, H)
-        _check_no_tangents(x)
+        _check_serves(x)
         _check_output(output, (T, H), x.dtype, x.device, x, w13_q, w13_scale, w2_q, w2_scale)
 
     return _answer("moe_b200_mxfp4_gated_ffn", got, explain)

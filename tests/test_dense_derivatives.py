@@ -49,3 +49,29 @@ def test_tangents_are_refused(cuda_device, grad_mode):
             ffn_host.gated_ffn(x, w13, w2, output=_dual((torch.empty_like(x),), 0)[0])
         with torch.inference_mode():       # stops forward mode too
             assert torch.equal(ffn_host.gated_ffn(dual, w13, w2), want)
+
+
+@pytest.mark.gpu
+def test_4_bit_functions_refuse_gradients(cuda_device):
+    """The 4-bit functions record no gradients, so that an input which asks for
+    them is refused while gradients are recorded; detached, or where they are
+    not recorded, it is taken. Codes are integers and never ask."""
+    import ffn_host
+
+    x, w13, w2, _ = _block()
+    with torch.no_grad():
+        q13, q2 = ffn_host.mxfp4_quantize(w13), ffn_host.mxfp4_quantize(w2)
+    leaf = x.clone().requires_grad_()
+    calls = (lambda t: ffn_host.mxfp4_linear(t, *q13), lambda t: ffn_host.mxfp4_gated_ffn(t, *q13, *q2))
+    for call in calls:
+        want = call(x)
+        for t in (leaf, leaf * 1):
+            with pytest.raises(RuntimeError, match="gradients"):
+                call(t)
+        with torch.no_grad():
+            assert torch.equal(call(leaf), want)
+        with torch.inference_mode():
+            assert torch.equal(call(leaf), want)
+        assert torch.equal(call(leaf.detach()), want)
+    for a, b in zip(ffn_host.mxfp4_quantize(torch.nn.Parameter(w13)), q13):
+        assert a.dtype == torch.uint8 and not a.requires_grad and torch.equal(a, b)
