@@ -150,6 +150,10 @@ size_t mx_ffn_bytes(int64_t T, int64_t H, int64_t I) {
   return mx_bytes(T, H) + mx_bytes(T, I) + (fused_gate_quant(T, I) ? 0 : round256(static_cast<size_t>(T) * I * 8));
 }
 
+// Only the bits that this read reports: kernels on other streams set bits at
+// any time, and one set after the copy is the next read's.
+__global__ void clear_status_kernel(uint32_t* word, uint32_t reported) { atomicAnd(word, ~reported); }
+
 }  // namespace
 }  // namespace moe
 
@@ -434,6 +438,14 @@ int moe_b200_mxfp4_gated_ffn(const void* x, int64_t x_pitch, int dtype, const vo
   return mx_gemm(ho, w2, p2, d, kStreamTokens, true, s);
 }
 
+int moe_b200_dense_status_address(void** address) {
+  if (address == nullptr) return MOE_B200_ERR_INVALID_ARGUMENT;
+  Device d;
+  const int st = open_device(&d);
+  if (st == MOE_B200_OK) *address = d.status;
+  return st;
+}
+
 int moe_b200_dense_read_status(uint32_t* status, void* stream) {
   if (status == nullptr) return MOE_B200_ERR_INVALID_ARGUMENT;
   Device d;
@@ -442,8 +454,12 @@ int moe_b200_dense_read_status(uint32_t* status, void* stream) {
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   uint32_t v = 0;
   if (cudaMemcpyAsync(&v, d.status, sizeof(v), cudaMemcpyDeviceToHost, s) != cudaSuccess ||
-      cudaMemsetAsync(d.status, 0, sizeof(v), s) != cudaSuccess || cudaStreamSynchronize(s) != cudaSuccess)
+      cudaStreamSynchronize(s) != cudaSuccess)
     return MOE_B200_ERR_CUDA;
+  if (v != 0) {
+    clear_status_kernel<<<1, 1, 0, s>>>(d.status, v);
+    if (cudaGetLastError() != cudaSuccess || cudaStreamSynchronize(s) != cudaSuccess) return MOE_B200_ERR_CUDA;
+  }
   *status = v;
   return v == 0 ? MOE_B200_OK : MOE_B200_ERR_DEVICE_TIMEOUT;
 }

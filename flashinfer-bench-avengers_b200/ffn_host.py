@@ -61,6 +61,7 @@ _SIGNATURES = {
     "moe_b200_mxfp4_gated_ffn_workspace_bytes": (_SIZE, [_I64, _I64, _I64]),
     "moe_b200_mxfp4_scale_bytes": (_SIZE, [_I64, _I64]),
     "moe_b200_dense_read_status": (_INT, [ctypes.POINTER(ctypes.c_uint32), _P]),
+    "moe_b200_dense_status_address": (_INT, [ctypes.POINTER(_P)]),
 }
 # Those the binding calls, in the order it takes them.
 _BINDING_CALLS = tuple(_SIGNATURES)[:11]
@@ -394,7 +395,7 @@ def mxfp4_gated_ffn(x: torch.Tensor, w13_q: torch.Tensor, w13_scale: torch.Tenso
 
 def read_status(device: torch.device | None = None) -> int:
     """Status word of the dense operators on ``device`` since the last read
-    (0 = clean); synchronises the current stream and clears the word."""
+    (0 = clean); synchronises the current stream and clears what it returns."""
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     st = ctypes.c_uint32(0)
     with torch.cuda.device(dev):

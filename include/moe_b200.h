@@ -559,9 +559,18 @@ MOE_B200_API int moe_b200_mxfp4_gated_ffn(const void* x, int64_t x_pitch, int dt
  * Status word of the dense operators on the current device: bits 1 << 0..2
  * (moe_b200_read_status) since the last read, set when a kernel gave up a
  * bounded wait; outputs of calls since then are not valid. Synchronises
- * `stream` and clears the word; MOE_B200_ERR_DEVICE_TIMEOUT when it was set.
+ * `stream` and clears the bits it returns, no others: one that a kernel on
+ * another stream sets meanwhile is left for the next read.
+ * MOE_B200_ERR_DEVICE_TIMEOUT when there were any.
  */
 MOE_B200_API int moe_b200_dense_read_status(uint32_t* status, void* stream);
+
+/*
+ * The word's device address on the current device: for callers that copy it
+ * out in the order of their own work (a captured graph, say, which cannot
+ * synchronise).
+ */
+MOE_B200_API int moe_b200_dense_status_address(void** address);
 
 /* ABI version of this header (bumped on any signature or struct layout change). */
 MOE_B200_API int moe_b200_abi_version(void);
