@@ -308,7 +308,9 @@ PyObject* gated_ffn_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   int code = 0;
   if (any) {
     const c10::cuda::CUDAGuard guard(dev);
-    const Scratch ws(lib.gated_ffn_backward_bytes(f.T, f.H, f.I), dev);
+    // [du | dg], which the gradient of w2 alone does not read
+    const bool dact = grads[0].defined() || grads[1].defined();
+    const Scratch ws(dact ? lib.gated_ffn_backward_bytes(f.T, f.H, f.I) : 0, dev);
     auto at_of = [](const at::Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; };
     code = lib.gated_ffn_backward(dy->const_data_ptr(), dy_pitch, f.x->const_data_ptr(), f.pitch,
                                   f.w13->const_data_ptr(), f.w2->const_data_ptr(),

@@ -496,9 +496,9 @@ MOE_B200_API int moe_b200_gated_ffn(const void* x, int64_t x_pitch, const void* 
  *   grad_w13 = [du | dg]^T x          [2I, H]
  *   grad_w2  = grad_output^T hidden   [H, I]
  * Any gradient may be NULL and is then not computed (with it the inputs that
- * only it needs may be NULL). Written in full, not added to; no atomics, so
- * repeated calls agree bit for bit. With no tokens the weights' gradients
- * are set to zero.
+ * only it needs may be NULL, and the workspace for grad_w2 alone). Written in
+ * full, not added to; no atomics, so repeated calls agree bit for bit. With no
+ * tokens the weights' gradients are set to zero.
  */
 MOE_B200_API size_t moe_b200_gated_ffn_backward_workspace_bytes(int64_t num_tokens, int64_t hidden_size,
                                                                 int64_t inter_size);
