@@ -21,8 +21,9 @@
 // -> 22; H = 2048, I = 1024 21 -> 17; at 64 tokens 55 -> 57, 38 -> 29 and 22
 // -> 22).
 //
-// The 16-bit block keeps its hidden (and [du | dg] for dx) as the sum of two 16-bit numbers, h rounded
-// and what that left, rounded again: the second product takes both as
+// The 16-bit block keeps its hidden (and [du | dg] for dx) in two 16-bit
+// numbers, h rounded and what that left, rounded again (times a factor that
+// keeps it in range, rest_scale): the second product takes both as
 // neighbouring token tiles of one MMA (N = 2 x 16 to 2 x 64) and their sums
 // are added with the parts. The result then carries one rounding instead of
 // two. Up to 32 tokens this is free, the tokens being next to nothing beside
@@ -379,6 +380,7 @@ __global__ void __launch_bounds__(kThreads)
     tc_fence_after();
     const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const int row = (warp & 3) * 32 + lane;
+    const float unscale = rest_unscale(p.type);
     for (int c = 16 * (warp >> 2); c < sh.bn; c += 32) {   // every other 16 tokens
       uint32_t r[16];
       tmem_ld16(lanes + c, r);
@@ -388,7 +390,7 @@ __global__ void __launch_bounds__(kThreads)
         tmem_ld16(lanes + sh.bn + c, lo);
         tmem_wait_ld();
 #pragma unroll
-        for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) + __uint_as_float(lo[j]));
+        for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(fmaf(__uint_as_float(lo[j]), unscale, __uint_as_float(r[j])));
       }
 #pragma unroll
       for (int j = 0; j < 16; ++j) red[(row >> 2) * pitch + 4 * (c + j) + (row & 3)] = __uint_as_float(r[j]);

@@ -286,7 +286,10 @@ def gated_ffn_forward(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, acti
 def gated_ffn_backward(grad_output: torch.Tensor, x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, saved,
                        activation: str = "silu", needs=(True, True, True)):
     """(grad_x, grad_w13, grad_w2) for ``grad_output`` [T, H], in the inputs'
-    type; None where ``needs`` is false. Bit for bit the same on every call."""
+    type; None where ``needs`` is false. Bit for bit the same on every call.
+    fp16 training wants a loss scale: act(g) and u act'(g) times the hidden's
+    gradient are rounded to fp16, where values below 2^-14 lose bits
+    (moe_b200_gated_ffn_backward)."""
     if not isinstance(saved, (tuple, list)) or len(saved) != 2:
         raise RuntimeError("saved must be the pair that gated_ffn_forward returned")
     if len(needs) != 3:

@@ -475,6 +475,8 @@ MOE_B200_API int moe_b200_a2a_read_status(const void* area, uint32_t* status, in
  * of x, the weights and the output. For up to MOE_B200_FFN_TWO_PART_TOKENS
  * tokens, which stream the weights through other kernels, what that rounding
  * left is kept as well, as a second number of that type, and enters output.
+ * With more tokens a hidden value carries that one rounding more; in fp16 one
+ * beyond 65504 becomes infinite, at any number of tokens.
  *   x [T, H], w13 [2I, H], w2 [H, I], output [T, H]; H and I multiples of 8
  *   preact   fp32 [T, 2I] or NULL: receives u and g, for the gradients (kept
  *            in 32 bits, because their rounding would enter du and dg)
@@ -499,6 +501,10 @@ MOE_B200_API int moe_b200_gated_ffn(const void* x, int64_t x_pitch, const void* 
  * only it needs may be NULL, and the workspace for grad_w2 alone). Written in
  * full, not added to; no atomics, so repeated calls agree bit for bit. With no
  * tokens the weights' gradients are set to zero.
+ * fp16: du and dg are rounded as they are, so that away from that second part
+ * (grad_w13 always, grad_x of more tokens) values below 2^-14 lose bits and
+ * those up to 2^-25 become zero. As in any fp16 training, scale the loss so
+ * that the gradients stay above that.
  */
 MOE_B200_API size_t moe_b200_gated_ffn_backward_workspace_bytes(int64_t num_tokens, int64_t hidden_size,
                                                                 int64_t inter_size);
