@@ -86,11 +86,14 @@ __global__ void __launch_bounds__(256, kType == kTypeFp32 ? 2 : 4)
         *reinterpret_cast<const uint4*>(s_scale + tid * 16);
 }
 
-// h = act(gate) * up of fp32 sums [rows, 2 n] (up, then gate), in 4 bits.
+// h = act(gate) * up of fp32 sums [rows, 2 n] (up, then gate), in 4 bits. (Lets
+// the next kernel start after its own wait, as every kernel here: 4-bit block
+// of H = 7168, I = 2048 at 16 tokens 15.45 -> 15.19 us against before it, at
+// 64 the same.)
 __global__ void __launch_bounds__(256)
     mxfp4_gate_kernel(const float* sums, int rows, int blocks, int k_tiles, int act, uint8_t* q, uint8_t* scale) {
-  pdl_launch_next();
   pdl_wait();
+  pdl_launch_next();
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   const int per_row = 4 * k_tiles;
   const int row = static_cast<int>(i / per_row);

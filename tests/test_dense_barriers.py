@@ -8,6 +8,9 @@ have ended is then exactly what nobody waited for, and must be nothing.
 """
 from __future__ import annotations
 
+import os
+import re
+
 import pytest
 
 
@@ -103,3 +106,24 @@ def test_every_accumulator_is_awaited(shared_columns):
             if it + (1 if shared_columns else 2) < tiles:        # a tile to come needs the columns
                 handed[0 if shared_columns else buf].post()
         assert on_the_way(complete + handed) == 0
+
+
+def _kernels():
+    """(name, text) of every kernel of the dense operators."""
+    here = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    for name in ("dense_gemm.cu", "dense_skinny.cu", "mxfp4.cu"):
+        with open(os.path.join(here, "flashinfer-bench-avengers_b200", "csrc", name)) as f:
+            text = f.read()
+        for m in re.finditer(r"^(__global__[^;{]*?(\w+_kernel)\([^;{]*\) \{\n)(.*?)^\}", text, re.M | re.S):
+            yield m.group(2), m.group(3)
+
+
+def test_kernels_wait_before_they_let_the_next_one_start():
+    """Weights are read ahead of a kernel's wait, behind another kernel of the
+    same call: whatever wrote them is complete because that one has waited
+    before it let this one start."""
+    seen = dict(_kernels())
+    assert set(seen) == {"dense_pair_kernel", "dense_skinny_kernel", "mxfp4_quantize_kernel", "mxfp4_gate_kernel",
+                         "mxfp4_dequantize_kernel"}
+    for name, body in seen.items():
+        assert 0 <= body.find("pdl_wait();") < body.find("pdl_launch_next();"), name
