@@ -51,7 +51,7 @@ struct DenseParams {
   const void* x;       // its rows, x_pitch bytes apart
   int64_t x_pitch;
   // derived by the launcher
-  int bn, n_step, b_half, m_tiles, n_tiles, k_iters, vec32, a_mn, copy_bytes;
+  int bn, n_step, b_half, m_tiles, n_tiles, k_iters, vec32, vec16, a_mn, copy_bytes;
   int early;           // B may be read before the kernel before has finished
 };
 

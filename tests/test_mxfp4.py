@@ -470,3 +470,26 @@ def test_c_abi_refusals():
     for call, empty in ((quantize, {"R": 0}), (dequantize, {"R": 0}), (matmul, {"M": 0}), (linear, {"T": 0}),
                         (block, {"T": 0})):
         assert call(**empty) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N", [136, 264, 260, 520, 257])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_product_rows_by_their_alignment(cuda_device, N, dtype):
+    """Over CTA pairs, rows of an output that start on 32 bytes, on 16 only, or
+    anywhere, and outputs that begin 16 bytes into a larger buffer: the same
+    numbers, and what lies around is left."""
+    import ffn_host
+
+    M, K = 140, 96
+    a, b = _matrix(M, K, 5), _matrix(N, K, 6)
+    args = [t.cuda() for t in (*a, *b)]
+    value, bound = ref.mx_product(ref.mx_values(*a), ref.mx_values(*b), dtype)
+    keep = (value.abs() + bound < 65000.0) if dtype == torch.float16 else torch.ones_like(value, dtype=torch.bool)
+    pad = 16 // torch.empty(0, dtype=dtype).element_size()
+    for first in (0, pad, 2 * pad):
+        buf = torch.full((first + M * N + 3 * pad,), 5.0, dtype=dtype, device="cuda")
+        out = buf[first:first + M * N].view(M, N)
+        assert ffn_host.mxfp4_matmul(*args, dtype, output=out) is out
+        ref.assert_within(out.cpu()[keep], (value[keep], bound[keep]), "product")
+        assert (buf[:first] == 5).all() and (buf[first + M * N:] == 5).all()
