@@ -924,7 +924,7 @@ int launch_dense_backward(const DenseProduct* products, int count, const DensePl
     p.bn = plan.bn[i > 0];
     p.a_mn = products[i].a_mn;
     finish(&p, false, true);
-    // kEpiDact writes du and, n columns on, dg
+    // dh is written as du and, n columns on, dg
     p.vec32 = aligned(p.out, 32) && (p.ldo * 2) % 32 == 0 && (p.preact == nullptr || p.n % 16 == 0);
     grp.tiles += p.m_tiles * p.n_tiles;
     if (i == 0) grp.tiles0 = grp.tiles;

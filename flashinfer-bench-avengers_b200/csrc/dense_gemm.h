@@ -100,11 +100,10 @@ int launch_dense_backward(const DenseProduct* products, int count, const DensePl
 int launch_mx_pair(DenseEpi epi, const MxOperand& a, const MxOperand& b, const DenseParams& p, int sm_count,
                    bool dependent, cudaStream_t s);
 
-// Few rows of A: out = A B^T streaming B, K split over a cluster
-// (kEpiStore and kEpiGated; kEpiBackward with B stored K x N; 4-bit:
-// kEpiStore).
-// With a_lo set the operand is the sum of the two matrices a and a_lo (at most
-// 128 rows).
+// Few rows of A (16 bits: up to 64; 4 bits: up to 128): out = A B^T streaming
+// B, K split over a cluster (kEpiStore and kEpiGated; kEpiBackward with B
+// stored K x N; 4-bit: kEpiStore). With a_lo set the operand is a and what its
+// rounding left, a_lo / rest_scale.
 int launch_dense_skinny(DenseEpi epi, const DenseOperand& a, const void* a_lo, const DenseOperand& b, DenseParams p,
                         int sm_count, bool dependent, cudaStream_t s);
 int launch_mx_skinny(const MxOperand& a, const MxOperand& b, DenseParams p, int sm_count, bool dependent,

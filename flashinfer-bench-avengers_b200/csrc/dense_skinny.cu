@@ -74,7 +74,7 @@ constexpr int kQuantMaxRows = 4;
 constexpr int kQuantMaxBytes = 48 * 1024;
 
 struct SkinnyShape {
-  int bn;            // tokens per tile (multiple of 16)
+  int bn;            // the tokens, rounded up to a multiple of 16 (at most 128)
   int x_rows;        // rows of a staged token tile: bn, or 2 bn of a two-part operand
   int splits;        // CTAs per cluster
   int stages;
@@ -90,7 +90,7 @@ struct SkinnyShape {
 // columns each; the loads of a batch of blocks are issued together.
 template <int kSrc, int kType>
 __device__ __forceinline__ void stage_tokens(const DenseParams& p, const SkinnyShape& sh, uint8_t* codes,
-                                             uint8_t* exponents, int t0, int live, int kb0, int iters, int tid) {
+                                             uint8_t* exponents, int live, int kb0, int iters, int tid) {
   constexpr int kBatch = kType == kTypeFp32 ? 2 : 4;
   const int chunks = iters * 32;               // of eight columns per row; past K: zero codes and exponents
   const int k_chunks = p.k >> 3;
@@ -107,7 +107,7 @@ __device__ __forceinline__ void stage_tokens(const DenseParams& p, const SkinnyS
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
       if (e < total && c < k_chunks) {
-        const uint8_t* src = static_cast<const uint8_t*>(p.x) + (t0 + row[i]) * p.x_pitch;
+        const uint8_t* src = static_cast<const uint8_t*>(p.x) + row[i] * p.x_pitch;
         if constexpr (kType == kTypeFp32) {
           const float4* f = reinterpret_cast<const float4*>(src + static_cast<int64_t>(c) * 32);
           const float4 lo = f[0], hi = f[1];
@@ -203,11 +203,10 @@ __global__ void __launch_bounds__(kThreads)
   const int lane = threadIdx.x & 31;
   const int rank = static_cast<int>(cluster_cta_rank());
   const int n0 = static_cast<int>(blockIdx.x) / sh.splits * kUnit;   // first feature of the tile
-  const int t0 = static_cast<int>(blockIdx.y) * sh.bn;
   const int kb0 = static_cast<int>(static_cast<int64_t>(p.k_iters) * rank / sh.splits);
   const int kb1 = static_cast<int>(static_cast<int64_t>(p.k_iters) * (rank + 1) / sh.splits);
   const int iters = kb1 - kb0;
-  const int live = static_cast<int>(p.m - t0 < sh.bn ? p.m - t0 : sh.bn);   // tokens of this tile
+  const int live = static_cast<int>(p.m);      // tokens, at most sh.bn
   const int x_bytes = kQuantX ? 0 : sh.x_rows * 128;                        // of a stage
 
   if (warp == 0 && lane == 0) {
@@ -261,9 +260,9 @@ __global__ void __launch_bounds__(kThreads)
       if (kQuantX) return;
       const uint32_t bar = full0 + 8u * stage;
       const uint32_t sx = base + stage * sh.stage_bytes + kWeightTile;
-      tma_load_2d(sx, &tm_x, bar, (kb0 + i) * (kMx ? 128 : 64), t0);
-      if (!kMx && sh.x_rows != sh.bn) tma_load_2d(sx + sh.bn * 128, &tm_sfx, bar, (kb0 + i) * 64, t0);
-      if (kMx) tma_load_2d(sx + x_bytes + 1024, &tm_sfx, bar, 0, (t0 >> 7) * kt + 2 * (kb0 + i));
+      tma_load_2d(sx, &tm_x, bar, (kb0 + i) * (kMx ? 128 : 64), 0);
+      if (!kMx && sh.x_rows != sh.bn) tma_load_2d(sx + sh.bn * 128, &tm_sfx, bar, (kb0 + i) * 64, 0);
+      if (kMx) tma_load_2d(sx + x_bytes + 1024, &tm_sfx, bar, 0, 2 * (kb0 + i));
     };
     const int first = min(sh.stages, iters);
     // The next kernel of the call may start once this CTA requests its last
@@ -361,11 +360,11 @@ __global__ void __launch_bounds__(kThreads)
     uint8_t* exponents = codes + sh.xq_iters * sh.bn * 128;
     const int tid = static_cast<int>(threadIdx.x) - 64;
     if (kSrc == kFromSums || p.type == kTypeFp32)
-      stage_tokens<kSrc, kTypeFp32>(p, sh, codes, exponents, t0, live, kb0, iters, tid);
+      stage_tokens<kSrc, kTypeFp32>(p, sh, codes, exponents, live, kb0, iters, tid);
     else if (p.type == kTypeBf16)
-      stage_tokens<kSrc, kTypeBf16>(p, sh, codes, exponents, t0, live, kb0, iters, tid);
+      stage_tokens<kSrc, kTypeBf16>(p, sh, codes, exponents, live, kb0, iters, tid);
     else
-      stage_tokens<kSrc, kTypeFp16>(p, sh, codes, exponents, t0, live, kb0, iters, tid);
+      stage_tokens<kSrc, kTypeFp16>(p, sh, codes, exponents, live, kb0, iters, tid);
     fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) mbar_arrive(smem_u32(xq_bar));
@@ -427,7 +426,7 @@ __global__ void __launch_bounds__(kThreads)
       const int f = rank * share + i / sh.bn * 4;   // first of the four features in the tile
       if (t < live && n0 + f < p.n) {
         float4 sum = sums(t, f);
-        const int64_t row = static_cast<int64_t>(t0) + t;
+        const int64_t row = t;
         if (kGate) {
           const float4 gate = sums(t, 64 + f);
           if (p.preact != nullptr) {
@@ -480,7 +479,7 @@ namespace {
 
 template <bool kMx, int kEpi, int kSrc>
 int launch_skinny(const CUtensorMap& w, const CUtensorMap& x, const CUtensorMap& sfw, const CUtensorMap& sfx,
-                  DenseParams p, const SkinnyShape& sh, int units, int token_tiles, bool dependent, cudaStream_t s) {
+                  DenseParams p, const SkinnyShape& sh, int units, bool dependent, cudaStream_t s) {
   p.early = dependent;
   auto kern = dense_skinny_kernel<kMx, kEpi, kSrc>;
   static OncePerDevice ready;
@@ -490,7 +489,7 @@ int launch_skinny(const CUtensorMap& w, const CUtensorMap& x, const CUtensorMap&
       }))
     return MOE_B200_ERR_CUDA;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(units * sh.splits), static_cast<unsigned>(token_tiles));
+  cfg.gridDim = dim3(static_cast<unsigned>(units * sh.splits));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = sh.smem_bytes;
   cfg.stream = s;
@@ -506,7 +505,6 @@ int launch_skinny(const CUtensorMap& w, const CUtensorMap& x, const CUtensorMap&
   return cudaLaunchKernelEx(&cfg, kern, w, x, sfw, sfx, p, sh) == cudaSuccess ? MOE_B200_OK : MOE_B200_ERR_CUDA;
 }
 
-int token_tile(int64_t m) { return m >= 128 ? 128 : static_cast<int>(div_up(m, 16) * 16); }
 
 // K parts: a power of two up to 8, at most one per K step, as many as keep
 // the grid within one CTA per SM; up to 64 tokens within two per SM while a
@@ -518,9 +516,9 @@ int token_tile(int64_t m) { return m >= 128 ? 128 : static_cast<int>(div_up(m, 1
 // this one's tail (27.5 -> 25.5 us).
 SkinnyShape choose_shape(const DenseParams& p, bool mx, bool gate, bool quant_x, int sm_count, bool two_part = false) {
   SkinnyShape sh;
-  sh.bn = token_tile(p.m);
+  sh.bn = static_cast<int>(div_up(p.m, 16) * 16);
   sh.x_rows = two_part ? 2 * sh.bn : sh.bn;
-  const int64_t ctas = div_up(p.n, gate ? 64 : 128) * div_up(p.m, sh.bn);
+  const int64_t ctas = div_up(p.n, gate ? 64 : 128);
   sh.splits = 1;
   while (sh.splits < 8 && 2 * sh.splits <= p.k_iters) {
     const int next = 2 * sh.splits;
@@ -562,16 +560,15 @@ int launch_dense_skinny(DenseEpi epi, const DenseOperand& a, const void* a_lo, c
   p.vec32 = 1;   // four columns at a time: n and ldo are multiples of 8
   const SkinnyShape sh = choose_shape(p, false, gate, false, sm_count, a_lo != nullptr);
   const int units = static_cast<int>(div_up(p.n, gate ? 64 : 128));
-  const int token_tiles = static_cast<int>(div_up(p.m, sh.bn));
   CUtensorMap tw, tx, tlo;
   if (!encode_2d(&tw, b.base, 2, b.cols, b.rows, b.pitch, 64, 64) ||
       !encode_2d(&tx, a.base, 2, a.cols, a.rows, a.pitch, 64, sh.bn) ||
       !encode_2d(&tlo, a_lo != nullptr ? a_lo : a.base, 2, a.cols, a.rows, a.pitch, 64, sh.bn))
     return MOE_B200_ERR_DRIVER;
   if (epi == kEpiBackward)
-    return launch_skinny<false, kEpiBackward, kFromMatrix>(tw, tx, tw, tlo, p, sh, units, token_tiles, dependent, s);
-  return gate ? launch_skinny<false, kEpiGated, kFromMatrix>(tw, tx, tw, tlo, p, sh, units, token_tiles, dependent, s)
-              : launch_skinny<false, kEpiStore, kFromMatrix>(tw, tx, tw, tlo, p, sh, units, token_tiles, dependent, s);
+    return launch_skinny<false, kEpiBackward, kFromMatrix>(tw, tx, tw, tlo, p, sh, units, dependent, s);
+  return gate ? launch_skinny<false, kEpiGated, kFromMatrix>(tw, tx, tw, tlo, p, sh, units, dependent, s)
+              : launch_skinny<false, kEpiStore, kFromMatrix>(tw, tx, tw, tlo, p, sh, units, dependent, s);
 }
 
 // Up to kQuantMaxRows tokens, while the staged tokens of a CTA's K range leave room
@@ -594,20 +591,19 @@ int launch_mx_skinny(const MxOperand& a, const MxOperand& b, DenseParams p, int 
   p.vec32 = p.n % 4 == 0 && p.ldo % 4 == 0;   // four columns at a time
   const SkinnyShape sh = choose_shape(p, true, false, p.x_source != kFromMatrix, sm_count);
   const int units = static_cast<int>(div_up(p.n, 128));
-  const int token_tiles = static_cast<int>(div_up(p.m, sh.bn));
   const int64_t kt = div_up(p.k, 128);
   CUtensorMap tw, tx, tsw, tsx;
   if (!encode_2d(&tw, b.q, 1, p.k / 2, b.rows, p.k / 2, 128, 128) ||
       !encode_2d(&tsw, b.scale, 2, 256, div_up(b.rows, 128) * kt, 512, 256, 2, false))
     return MOE_B200_ERR_DRIVER;
   if (p.x_source == kFromRows)
-    return launch_skinny<true, kEpiStore, kFromRows>(tw, tw, tsw, tsw, p, sh, units, token_tiles, dependent, s);
+    return launch_skinny<true, kEpiStore, kFromRows>(tw, tw, tsw, tsw, p, sh, units, dependent, s);
   if (p.x_source == kFromSums)
-    return launch_skinny<true, kEpiStore, kFromSums>(tw, tw, tsw, tsw, p, sh, units, token_tiles, dependent, s);
+    return launch_skinny<true, kEpiStore, kFromSums>(tw, tw, tsw, tsw, p, sh, units, dependent, s);
   if (!encode_2d(&tx, a.q, 1, p.k / 2, a.rows, p.k / 2, 128, sh.bn) ||
       !encode_2d(&tsx, a.scale, 2, 256, div_up(a.rows, 128) * kt, 512, 256, 2, false))
     return MOE_B200_ERR_DRIVER;
-  return launch_skinny<true, kEpiStore, kFromMatrix>(tw, tx, tsw, tsx, p, sh, units, token_tiles, dependent, s);
+  return launch_skinny<true, kEpiStore, kFromMatrix>(tw, tx, tsw, tsx, p, sh, units, dependent, s);
 }
 
 }  // namespace moe
