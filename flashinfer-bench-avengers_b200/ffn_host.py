@@ -63,8 +63,12 @@ _SIGNATURES = {
     "moe_b200_dense_read_status": (_INT, [ctypes.POINTER(ctypes.c_uint32), _P]),
     "moe_b200_dense_status_address": (_INT, [ctypes.POINTER(_P)]),
 }
-# Those the binding calls, in the order it takes them.
-_BINDING_CALLS = tuple(_SIGNATURES)[:11]
+# Those the binding calls, in the order it takes them (torch_binding.cpp, Library).
+_BINDING_CALLS = (
+    "moe_b200_gated_ffn", "moe_b200_gated_ffn_workspace_bytes", "moe_b200_gated_ffn_backward",
+    "moe_b200_gated_ffn_backward_workspace_bytes", "moe_b200_mxfp4_quantize", "moe_b200_mxfp4_dequantize",
+    "moe_b200_mxfp4_matmul", "moe_b200_mxfp4_linear", "moe_b200_mxfp4_linear_workspace_bytes",
+    "moe_b200_mxfp4_gated_ffn", "moe_b200_mxfp4_gated_ffn_workspace_bytes")
 
 _library_bound = None
 _native = None
