@@ -48,7 +48,7 @@ __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
 // that this warp has read (its loads are complete). Relaxed: a release would
 // wait for the warp's stores to global memory, which nobody there reads
 // (gradients at 128 tokens, H = 7168, I = 2048, 70 -> 57 us; 4-bit block at
-// 4096 tokens 91 -> 84).
+// 4096 tokens 91 -> 84). Not for handing over anything that was stored.
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_bar) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }

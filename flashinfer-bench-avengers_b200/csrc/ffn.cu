@@ -26,7 +26,9 @@ constexpr int64_t kMaxDim = 65536;
 // 31.7 / 31.2. 4 bits, the same block: at 80 tokens 14.1 / 15.7, 18.8 / 17.3
 // and 21.5 / 20.1, at 128 14.9 / 18.2, 19.3 / 21.0 and 22.3 / 24.1. A 4-bit
 // product alone, whose sums take no further kernel, streams for longer (4096 x
-// 7168 at 128 tokens 15.4 / 12.2, 1024 x 2048 9.1 / 7.8).
+// 7168 at 128 tokens 15.4 / 12.2, 1024 x 2048 9.1 / 7.8). One limit for weights
+// of any size, because the block's rounding hangs on it too: the largest lose up
+// to 10 % at 65 to 96 tokens by it, where small ones would lose 30 %.
 constexpr int64_t kStreamTokens = MOE_B200_FFN_TWO_PART_TOKENS;
 constexpr int64_t kMxStreamTokens = 128;
 
